@@ -20,7 +20,8 @@ EXPORTS = ("corm_vectorop", "corm_matmul_workspace_size", "corm_matmul", "corm_m
            "corm_matmul_post", "corm_matmul_groups", "corm_split_b_planes", "corm_matmul_bplanes", "corm_conv_post", "corm_gemm_strided_workspace_size", "corm_gemm_strided",
            "corm_copy_nd", "corm_llm_attn_softmax", "corm_greedy_embed", "corm_llm_embed", "corm_llm_dequant",
            "corm_llm_resadd", "corm_llm_rmsnorm", "corm_llm_act_mul", "corm_llm_attn_prep_host",
-           "corm_llm_decode_attn", "corm_rowops_chain", "corm_rowops_chain_dev",
+           "corm_llm_decode_attn", "corm_llm_paged_prep", "corm_llm_paged_attn", "corm_llm_paged_read",
+           "corm_rowops_chain", "corm_rowops_chain_dev",
            "corm_stream_done",
            "corm_pool", "corm_rowops", "corm_act_table", "corm_smx_table", "corm_rowops_table_image",
            "corm_bind_device", "corm_device_status", "corm_set_wait_limit", "corm_launch_count", "corm_profile_enable",
@@ -136,6 +137,28 @@ class DecodeAttnDesc(C.Structure):
                 ("pq", C.c_void_p), ("pk", C.c_void_p), ("pv", C.c_void_p), ("prep", C.c_uint32)]
 
 
+class PagedCacheDesc(C.Structure):
+    """corm_paged_cache: the pages and the batch a paged entry works on."""
+    _fields_ = [(nm, C.c_void_p) for nm in ("kc", "vc", "ks", "vs", "table", "cu", "pos")] + _u32_fields(
+        ["pages", "page", "bits", "KV", "HD", "B", "table_width", "rows"])
+
+
+class PagedPrepDesc(C.Structure):
+    _fields_ = [("c", PagedCacheDesc)] + [(nm, C.c_void_p) for nm in ("q0", "k0", "v0", "q", "rope", "pq", "pk", "pv",
+                                                                      "nq", "nk")] + [
+        (nm, C.c_uint64) for nm in ("eps_q", "eps_k", "ldq0", "ldk", "ldv", "ldq")] + _u32_fields(
+        ["H", "rot", "interleaved", "rope_rows", "flags"])
+
+
+class PagedAttnDesc(C.Structure):
+    _fields_ = [("c", PagedCacheDesc)] + [(nm, C.c_void_p) for nm in ("q", "o", "smx")] + [
+        ("ldq", C.c_uint64), ("ldo", C.c_uint64)] + _u32_fields(["H", "max_q", "max_keys", "window"])
+
+
+class PagedReadDesc(C.Structure):
+    _fields_ = [("c", PagedCacheDesc), ("k", C.c_void_p), ("v", C.c_void_p), ("ldk", C.c_uint64), ("ldv", C.c_uint64)]
+
+
 class PoolDesc(C.Structure):
     _fields_ = [("x", C.c_void_p), ("y", C.c_void_p)] + _u32_fields(
         ["batch", "channels", "in_h", "in_w", "out_h", "out_w", "pool_h", "pool_w", "stride_h", "stride_w",
@@ -194,6 +217,9 @@ def lib() -> C.CDLL:
                        ("corm_llm_act_mul", [C.POINTER(LlmActMulDesc), C.c_void_p]),
                        ("corm_llm_attn_prep_host", [C.POINTER(LlmPrepDesc), C.c_void_p]),
                        ("corm_llm_decode_attn", [C.POINTER(DecodeAttnDesc), C.c_void_p]),
+                       ("corm_llm_paged_prep", [C.POINTER(PagedPrepDesc), C.c_void_p]),
+                       ("corm_llm_paged_attn", [C.POINTER(PagedAttnDesc), C.c_void_p]),
+                       ("corm_llm_paged_read", [C.POINTER(PagedReadDesc), C.c_void_p]),
                        ("corm_pool", [C.POINTER(PoolDesc), C.c_void_p]),
                        ("corm_rowops", [C.POINTER(RowOpsDesc), C.c_void_p]),
                        ("corm_rowops_chain", [C.POINTER(RowOpsDesc), C.c_uint32, C.c_void_p]),

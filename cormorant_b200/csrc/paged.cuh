@@ -1,0 +1,144 @@
+// Shared pieces of the paged KV-cache operators (paged.cu, paged_tile.cu):
+// the geometry checks, a row's place in the batch, the softmax unit's integers
+// and the warp-level byte shuffles.
+//
+// The cache: [pages][KV][page][row] bytes, a row of 16-bit words as two byte
+// planes side by side (hi = v >> 8 signed, HD bytes; lo = v & 255, HD bytes) —
+// the operands of the int8 tensor cores, so attention splits no word — or of
+// 8-bit codes (HD bytes) with one shift per (page, KV head, row) in a second
+// array: the word is code << shift.
+#pragma once
+
+#include "corm_common.cuh"
+#include "corm_sm100.cuh"
+
+namespace paged {
+
+// The descriptor's host checks every entry shares; what: the entry's name.
+int check_cache(const corm_paged_cache* c, const char* what);
+
+struct SeqRows {
+  uint32_t lo, n;    // first packed row and rows of the sequence
+  uint32_t pos, cap; // position of its first row; positions the table covers
+};
+
+// Sequence b, with the device arrays' values brought into range: cu within
+// [0, rows] and not descending, pos not negative.
+__device__ __forceinline__ SeqRows seq_rows(const corm_paged_cache& c, uint32_t b, uint32_t rows) {
+  const int32_t a = c.cu[b], e = c.cu[b + 1], p = c.pos[b];
+  SeqRows s;
+  s.lo = min((uint32_t)max(a, 0), rows);
+  const uint32_t hi = min((uint32_t)max(e, 0), rows);
+  s.n = hi > s.lo ? hi - s.lo : 0u;
+  s.cap = c.table_width * c.page;
+  s.pos = (uint32_t)max(p, 0);
+  return s;
+}
+
+// ---------------------------------------------------------------- the softmax unit's integers
+// e of a score d below the row's maximum: y = (d Cm) >> Cs, TAB[y mod 4096] >>
+// (y / 4096).  The table is held less one in 16 bits (TAB is 32774 .. 65536).
+struct SmxScale {
+  uint32_t cm8;  // Cm << 8
+  uint32_t sh;   // Cs - 8
+};
+// 8 <= Cs: (d << 16)(Cm << 8) >> 32 = (d Cm) >> 8 fits 32 bits (d < 2^16, Cm < 2^24),
+// and from Cs = 40 on y is 0
+__device__ __forceinline__ SmxScale smx_scale(uint32_t cm, uint32_t cs) {
+  SmxScale s;
+  s.cm8 = cs >= 40u ? 0u : (cm & 0xFFFFFFu) << 8;
+  s.sh = cs >= 40u ? 0u : cs - 8u;
+  return s;
+}
+__device__ __forceinline__ uint32_t smx_e(uint32_t d, SmxScale s, const uint16_t* tab) {
+  const uint32_t y = __umulhi(d << 16, s.cm8) >> s.sh;
+  const uint32_t o = y >> 12;
+  const uint32_t t = (uint32_t)tab[y & 4095u] + 1u;
+  return o > 16u ? 0u : t >> o;
+}
+// Cs < 8: y may pass 32 bits
+__device__ __forceinline__ uint32_t smx_e_wide(uint32_t d, uint32_t cm, uint32_t cs, const uint16_t* tab) {
+  const uint64_t y = ((uint64_t)d * (cm & 0xFFFFFFu)) >> cs;
+  return (y >> 12) > 16u ? 0u : ((uint32_t)tab[y & 4095u] + 1u) >> (uint32_t)(y >> 12);
+}
+// e in 16 bits: TAB[0] = 65536 is the only value past 65535, and no entry is 65535
+__device__ __forceinline__ uint32_t e_pack(uint32_t e) { return min(e, 65535u); }
+__device__ __forceinline__ uint32_t e_unpack(uint32_t h) { return h + (h == 65535u ? 1u : 0u); }
+
+// P = min((e R + 2^(39 - f_p)) >> (40 - f_p), 32767); e R < 2^41
+__device__ __forceinline__ uint32_t smx_p(uint32_t e, uint32_t R, uint32_t fp) {
+  const uint64_t v = ((uint64_t)e * R + (1ull << (39u - fp))) >> (40u - fp);
+  return v > 32767ull ? 32767u : (uint32_t)v;
+}
+// R = floor(2^40 / S) (S >= 2^16 wherever a row sees a key, so R <= 2^24)
+__device__ __forceinline__ uint32_t smx_r(unsigned long long S) {
+  return S ? (uint32_t)min((1ull << 40) / S, 1ull << 24) : 0u;
+}
+
+// four 4-byte rows -> four words of one byte column each
+__device__ __forceinline__ void transpose4(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t (&o)[4]) {
+  const uint32_t a = __byte_perm(w0, w1, 0x5140), b = __byte_perm(w2, w3, 0x5140);
+  const uint32_t c = __byte_perm(w0, w1, 0x7362), d = __byte_perm(w2, w3, 0x7362);
+  o[0] = __byte_perm(a, b, 0x5410);
+  o[1] = __byte_perm(a, b, 0x7632);
+  o[2] = __byte_perm(c, d, 0x5410);
+  o[3] = __byte_perm(c, d, 0x7632);
+}
+
+// an exact sum modulo 2^32 as the kernels round it: floor / 2^8, saturated
+__device__ __forceinline__ int32_t out16(uint32_t acc) {
+  const int32_t y = (int32_t)acc >> 8;
+  return min(max(y, -32768), 32767);
+}
+__device__ __forceinline__ uint32_t pack16(int32_t lo, int32_t hi) {  // both already in int16
+  return ((uint32_t)hi << 16) | ((uint32_t)lo & 0xFFFFu);
+}
+
+// C[16 x 8] += A[16 x 32] B[32 x 8] on 8-bit operands, int32 sums modulo 2^32
+// (warp-level; used where a tile has 16 rows at most)
+#define CORM_MMA_I8(NAME, TA, TB)                                                                                      \
+  __device__ __forceinline__ void NAME(uint32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {           \
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." TA "." TB                                                    \
+                 ".s32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"                                             \
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])                                                      \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));                                      \
+  }
+CORM_MMA_I8(mma_ss, "s8", "s8")
+CORM_MMA_I8(mma_su, "s8", "u8")
+CORM_MMA_I8(mma_us, "u8", "s8")
+CORM_MMA_I8(mma_uu, "u8", "u8")
+#undef CORM_MMA_I8
+
+// ---------------------------------------------------------------- bulk copies and clusters
+__device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   sm100::smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address of this CTA's shared variable p in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(sm100::smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ uint32_t cluster_ld32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned long long cluster_ld64(uint32_t a) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+  return v;
+}
+
+}  // namespace paged

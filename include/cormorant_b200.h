@@ -411,6 +411,101 @@ typedef struct {
 
 int corm_llm_decode_attn(const corm_llm_decode_attn_desc* d, corm_stream_t stream);
 
+/* ---------------------------------------------------------------- paged KV cache
+ * No counterpart in the reference, whose entries run one sequence over one
+ * contiguous cache: a batch of sequences of any lengths at any positions, their
+ * K / V rows in pages of a shared pool.  The numerics are the nodes': the
+ * row-ops NORM and ROPE jobs, the MatMul rule with the int32 wrap and the
+ * softmax unit.
+ *
+ * Cache: kc / vc [pages][KV][page][row] bytes; bits 16: a row is HD high bytes
+ * (v >> 8) then HD low bytes (v & 255) of its int16 words; bits 8: HD codes,
+ * with ks / vs [pages][KV][page] one shift each — the word is code << shift,
+ * shift = max(0, bits of max(x, ~x) - 7) over the row, code = the word / 2^shift
+ * rounded half to even, within [-128, 127].
+ * Batch: sequence b has the packed rows cu[b] .. cu[b + 1] - 1 at positions
+ * pos[b], pos[b] + 1, ..; position p is row p % page of page table[b *
+ * table_width + p / page].  cu [B + 1], pos [B] and table are read on the device
+ * (a captured launch replays with their new values); values out of range are
+ * brought into it: cu to [0, rows], a negative pos to 0; a table entry outside
+ * [0, pages) stands for a page of zeros that is not written, and a position
+ * past the table is neither written nor seen.  Packed rows of no sequence are
+ * left as they were.  Two rows must not share a (page, row).
+ * page 16, 32, 64, 128 or 256; HD 16, 32, 64, 128 or 256; every array on 16
+ * bytes. */
+typedef struct {
+  int8_t* kc;
+  int8_t* vc;
+  uint8_t* ks; /* bits 8 only */
+  uint8_t* vs;
+  const int32_t* table;
+  const int32_t* cu;
+  const int32_t* pos;
+  uint32_t pages, page, bits, KV, HD;
+  uint32_t B, table_width, rows; /* rows: packed rows of the arrays below */
+} corm_paged_cache;
+
+/* corm_llm_paged_prep: per packed row the q / k heads of q0 [rows][ldq0 >= H
+ * HD] and k0 [rows][ldk >= KV HD] optionally normed (nq / nk: HD 16-byte entries,
+ * G and sh_c used, eps_q / eps_k < 2^62: the row-ops RMS NORM of each head, as
+ * norm_params writes its entries), then rotated at the row's position over
+ * their first rot dimensions (rot even; pairs (i, i + rot / 2), or (2 i, 2 i + 1)
+ * with interleaved) by rope [rope_rows][rot] int32 (cos of the rot / 2 pairs,
+ * then sin, at 2^-23, |value| < 2^24; a position past the table takes its last row): RNE((x c <<
+ * sh_a) -+ (x' s << sh_b), sh_c) with the entries pq [H HD] / pk [KV HD] (one
+ * entry with flag 1 / 2; the remaining dimensions x << sh_a, sh_c), the q heads
+ * into q [rows][ldq] and the k heads into the K pages; v0 [rows][ldv] re-rounded
+ * by pv [KV HD] (RNE(x << sh_a, sh_c); one entry with flag 4; as it is with flag 8)
+ * into the V pages.  Bq' of the entries is not used. */
+typedef struct {
+  corm_paged_cache c;
+  const int16_t* q0;
+  const int16_t* k0;
+  const int16_t* v0;
+  int16_t* q;
+  const int32_t* rope;
+  const void* pq;
+  const void* pk;
+  const void* pv;
+  const void* nq;
+  const void* nk;
+  uint64_t eps_q, eps_k;
+  uint64_t ldq0, ldk, ldv, ldq;
+  uint32_t H, rot, interleaved, rope_rows, flags;
+} corm_llm_paged_prep_desc;
+int corm_llm_paged_prep(const corm_llm_paged_prep_desc* d, corm_stream_t stream);
+
+/* corm_llm_paged_attn: the causal attention of the packed q rows [rows][ldq]
+ * over the cache: per row at position p and query head h (KV head h / (H / KV))
+ * the scores sat16(floor(wrap32(q.K_j) / 2^8)) of the keys j <= p (and j > p -
+ * window with a window), the softmax unit's P with smx[h] = {Cm, Cs | f_p << 8},
+ * and sat16(floor(wrap32(sum P_j V_j) / 2^8)) into o [rows][ldo] (head h at h
+ * HD): what the q.K^T / column softmax / P.V / merge nodes give for that
+ * sequence alone.  A row that sees no key gives zeros.  H / KV <= 16.
+ * max_q: the most rows of a sequence (further rows are left as they were);
+ * max_keys: the most keys (a hint for the split of the work; any value is
+ * right). */
+typedef struct {
+  corm_paged_cache c;
+  const int16_t* q;
+  int16_t* o;
+  const uint32_t* smx; /* [H][2] */
+  uint64_t ldq, ldo;
+  uint32_t H, max_q, max_keys, window;
+} corm_llm_paged_attn_desc;
+int corm_llm_paged_attn(const corm_llm_paged_attn_desc* d, corm_stream_t stream);
+
+/* corm_llm_paged_read: the cached words of the packed rows' positions into k
+ * [rows][ldk] and v [rows][ldv] int16 (either may be NULL; zeros past the
+ * table). */
+typedef struct {
+  corm_paged_cache c;
+  int16_t* k;
+  int16_t* v;
+  uint64_t ldk, ldv;
+} corm_llm_paged_read_desc;
+int corm_llm_paged_read(const corm_llm_paged_read_desc* d, corm_stream_t stream);
+
 /* ---------------------------------------------------------------- Pool
  * Replaces run_pool / XPoolingkernel (inference-scheduler/src/codegen/
  * _source.py:1548-1580; semantics inference-scheduler/src/codegen/
