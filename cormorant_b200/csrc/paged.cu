@@ -4,6 +4,7 @@
 #include "paged.cuh"
 
 #include "gemm_i8x4.h"
+#include "paged_tile.h"
 
 namespace paged {
 
@@ -383,6 +384,7 @@ constexpr uint32_t kT = 64;       // keys of a stage
 constexpr uint32_t kRows = 16;    // rows of a tile
 constexpr uint32_t kWarps = 8;    // computing warps
 constexpr uint32_t kMaxCluster = 8;
+constexpr uint32_t kSplitRows = 32;  // rows of a sequence and KV head up to which this form runs
 
 struct SplitArgs {
   corm_llm_paged_attn_desc d;
@@ -403,24 +405,6 @@ struct SplitShape {
 __host__ __device__ constexpr uint32_t split_pitch(uint32_t win) { return win * kT + 16u; }  // int16 of a score row
 
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* err, int code) {
-  const long long t0 = clock64();
-  for (;;) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(sm100::smem_u32(bar)), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if (clock64() - t0 > 4000000000ll) break;
-  }
-  atomicCAS(err, 0, code);
-  return false;
-}
 
 template <int HD, int BITS>
 __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kernel(const __grid_constant__ SplitArgs A) {
@@ -647,10 +631,7 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
   auto cluster_meet = [&]() {
     consumer_sync();
     if (X > 1) {
-      if (tid < X) {
-        const uint32_t a = cluster_addr(&cbar, tid);
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
-      }
+      if (tid < X) mbar_arrive_remote(&cbar, tid);
       if (ok) ok = mbar_wait_cluster(&cbar, cphase, A.err, 303);
       cphase ^= 1u;
     }
@@ -1023,6 +1004,7 @@ extern "C" int corm_llm_paged_attn(const corm_llm_paged_attn_desc* d, corm_strea
   const uint64_t tiles = (rows + kRows - 1u) / kRows;
   if (tiles > (1ull << 27)) return corm::fail(CORM_ELIMIT, "corm_llm_paged_attn: max_q %u", d->max_q);
   cudaStream_t st = (cudaStream_t)stream;
+  if (rows > kSplitRows && paged::tile_takes(A.d)) return paged::launch_tiles(A.d, A.tab, A.err, st);
   switch (c.HD * 2u + (c.bits == 8u)) {
     case 32: return launch_split<16, 16>(A, (uint32_t)tiles, st);
     case 33: return launch_split<16, 8>(A, (uint32_t)tiles, st);
