@@ -3,6 +3,8 @@
 // of few rows a sequence.
 #include "paged.cuh"
 
+#include <type_traits>
+
 #include "gemm_i8x4.h"
 #include "paged_tile.h"
 
@@ -61,17 +63,28 @@ __device__ __forceinline__ void rsqrt64(uint64_t D, uint64_t& Rm, int& sh, const
   sh = 47 + d / 2;
 }
 
-struct Shifts {  // an element's entry
-  uint8_t a, b, c;
-};
-
-__device__ __forceinline__ int32_t rot_out(int64_t x, int64_t cs, int64_t y, int64_t sn, Shifts s, bool fast) {
-  if (fast) return (int32_t)corm_sat16(corm_rne_shr64f(((x * cs) << s.a) + ((y * sn) << s.b), s.c));
-  return (int32_t)corm_sat16_128(corm_rne_shr128(((__int128)(x * cs) << s.a) + ((__int128)(y * sn) << s.b), s.c));
+// one rotated element with any entry s = sh_a | sh_b << 8 | sh_c << 16; 64-bit
+// while the up-shifts are at most 22 (|c| < 2^24: both terms below 2^61)
+__device__ __noinline__ int32_t rot_any(int32_t x, int32_t cs, int32_t y, int32_t sn, uint32_t s) {
+  const int a = (int)(s & 63u), b = (int)((s >> 8) & 63u), c = (int)(s >> 16);
+  const int64_t u = (int64_t)x * cs, v = (int64_t)y * sn;
+  if (max(a, b) <= 22) return (int32_t)corm_sat16(corm_rne_shr64f((u << a) + (v << b), c));
+  return (int32_t)corm_sat16_128(corm_rne_shr128(((__int128)u << a) + ((__int128)v << b), c));
+}
+// no up-shift, a down-shift k <= 31 whose quotient is below 2^31 (sums stay below
+// 2^40: k >= 9, or an element that is not rotated): both roundings (floor for the
+// parity, then the result) are one funnel shift each.  half1 = 2^(k - 1) - 1 and
+// par = 1, both 0 for k = 0
+__device__ __forceinline__ int32_t rot_plain(int32_t x, int32_t cs, int32_t y, int32_t sn, uint32_t k, uint32_t half1,
+                                             uint32_t par) {
+  const int64_t v = (int64_t)x * cs + (int64_t)y * sn;
+  const uint32_t odd = __funnelshift_r((uint32_t)v, (uint32_t)(v >> 32), k) & par;
+  const int64_t u = v + (int64_t)(half1 + odd);
+  return (int32_t)__funnelshift_r((uint32_t)u, (uint32_t)(u >> 32), k);
 }
 
-template <int HD, bool VEC>
-__global__ void __launch_bounds__(256) paged_prep_kernel(const __grid_constant__ PrepArgs A) {
+template <int HD, bool VEC, bool NORM>
+__global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constant__ PrepArgs A) {
   corm_pdl_wait();
   corm_pdl_trigger();
   constexpr uint32_t LPH = HD / 8;     // lanes per head
@@ -97,34 +110,30 @@ __global__ void __launch_bounds__(256) paged_prep_kernel(const __grid_constant__
     db[k] = split ? p + hr : 2u * p + 1u;
   }
   const bool spl = 4u * lane < hr && !d.interleaved;  // VEC: alike for the lane's four pairs
-  Shifts sa[4], sb[4];
-  uint32_t big = 0;
-  {
-    const uint8_t* e = (const uint8_t*)(is_q ? d.pq : (is_v ? d.pv : d.pk));
-    const bool bc = d.flags & (is_q ? 1u : (is_v ? 4u : 2u));
-    const bool direct = is_v && (d.flags & 8u);
+  // the usual entries: no up-shift and one down-shift for the lane's elements, whose
+  // quotients fit 32 bits; any others are read again where they are used
+  const uint8_t* ent = (const uint8_t*)(is_q ? d.pq : (is_v ? d.pv : d.pk));
+  const bool bc = d.flags & (is_q ? 1u : (is_v ? 4u : 2u)), direct = is_v && (d.flags & 8u);
+  auto shifts = [&](uint32_t dim) -> uint32_t {  // sh_a | sh_b << 8 | sh_c << 16
+    return direct ? 0u : *(const uint32_t*)(ent + 16ull * (bc ? 0u : head * HD + dim) + 8) & 0x3F3F3Fu;
+  };
+  const uint32_t k0 = shifts(da[0]), kd = k0 >> 16;
+  bool plain = (k0 & 0xFFFFu) == 0u && kd <= 31u && (kd >= 9u || 4u * lane >= hr);
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const uint8_t* ea = e + 16ull * (bc ? 0u : head * HD + da[k]) + 8;
-      const uint8_t* eb = e + 16ull * (bc ? 0u : head * HD + db[k]) + 8;
-      sa[k] = direct ? Shifts{0, 0, 0} : Shifts{(uint8_t)(ea[0] & 63u), (uint8_t)(ea[1] & 63u), (uint8_t)(ea[2] & 63u)};
-      sb[k] = direct ? Shifts{0, 0, 0} : Shifts{(uint8_t)(eb[0] & 63u), (uint8_t)(eb[1] & 63u), (uint8_t)(eb[2] & 63u)};
-      big = max(big, max(max(sa[k].a, sa[k].b), max(sb[k].a, sb[k].b)));
-    }
-  }
-  const bool fast = big <= 22u;  // |c| < 2^24: both products below 2^61 after their shifts
+  for (int k = 0; k < 4; k++) plain = plain && shifts(da[k]) == k0 && shifts(db[k]) == k0;
+  const uint32_t half1 = kd ? (1u << (kd & 31u)) / 2u - 1u : 0u, par = kd ? 1u : 0u;
   const uint8_t* ne = (const uint8_t*)(is_q ? d.nq : (is_v ? nullptr : d.nk));
   int32_t ga[4], gb[4];
-  uint8_t na[4], nb[4];
-  if (ne) {
+  uint32_t na = 0, nb = 0;  // the norm's down-shifts, a byte each
+  if (NORM && ne) {
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       const uint8_t* ea = ne + 16u * da[k];
       const uint8_t* eb = ne + 16u * db[k];
       ga[k] = *(const int32_t*)ea;
       gb[k] = *(const int32_t*)eb;
-      na[k] = ea[10] & 63u;
-      nb[k] = eb[10] & 63u;
+      na |= (ea[10] & 63u) << (8 * k);
+      nb |= (eb[10] & 63u) << (8 * k);
     }
   }
   const uint64_t eps = is_q ? d.eps_q : d.eps_k;
@@ -175,7 +184,7 @@ __global__ void __launch_bounds__(256) paged_prep_kernel(const __grid_constant__
         vb[k] = x[db[k]];
       }
     }
-    if (ne) {
+    if (NORM && ne) {
       uint64_t s2 = 0;
 #pragma unroll
       for (int k = 0; k < 4; k++) s2 += (uint64_t)(uint32_t)(va[k] * va[k]) + (uint32_t)(vb[k] * vb[k]);
@@ -187,8 +196,8 @@ __global__ void __launch_bounds__(256) paged_prep_kernel(const __grid_constant__
       sh -= 24;
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        va[k] = (int32_t)corm_sat16(corm_rne_shr64f((((int64_t)va[k] * (int64_t)Rm) >> sh) * ga[k], na[k]));
-        vb[k] = (int32_t)corm_sat16(corm_rne_shr64f((((int64_t)vb[k] * (int64_t)Rm) >> sh) * gb[k], nb[k]));
+        va[k] = (int32_t)corm_sat16(corm_rne_shr64f((((int64_t)va[k] * (int64_t)Rm) >> sh) * ga[k], (int)(na >> (8 * k)) & 63));
+        vb[k] = (int32_t)corm_sat16(corm_rne_shr64f((((int64_t)vb[k] * (int64_t)Rm) >> sh) * gb[k], (int)(nb >> (8 * k)) & 63));
       }
     }
     const int32_t* tr = d.rope + (uint64_t)min(p, (uint64_t)(d.rope_rows - 1u)) * d.rot;
@@ -205,11 +214,20 @@ __global__ void __launch_bounds__(256) paged_prep_kernel(const __grid_constant__
         sn[k] = pr < hr ? __ldg(tr + hr + pr) : 0;
       }
     }
+    if (plain) {
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const int32_t a = va[k], bb = vb[k];
-      va[k] = rot_out(a, cs[k], -(int64_t)bb, sn[k], sa[k], fast);
-      vb[k] = rot_out(bb, cs[k], a, sn[k], sb[k], fast);
+      for (int k = 0; k < 4; k++) {
+        const int32_t a = va[k], bb = vb[k];
+        va[k] = min(max(rot_plain(a, cs[k], -bb, sn[k], kd, half1, par), -32768), 32767);
+        vb[k] = min(max(rot_plain(bb, cs[k], a, sn[k], kd, half1, par), -32768), 32767);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int32_t a = va[k], bb = vb[k];
+        va[k] = rot_any(a, cs[k], -bb, sn[k], shifts(da[k]));
+        vb[k] = rot_any(bb, cs[k], a, sn[k], shifts(db[k]));
+      }
     }
     if (is_q) {
       int16_t* y = d.q + row * d.ldq + (uint64_t)head * HD;
@@ -907,7 +925,8 @@ extern "C" int corm_llm_paged_prep(const corm_llm_paged_prep_desc* d, corm_strea
     return corm::fail(CORM_EINVAL, "corm_llm_paged_prep: row strides below the row lengths");
   if ((d->nq && d->eps_q >> 62) || (d->nk && d->eps_k >> 62))
     return corm::fail(CORM_ELIMIT, "corm_llm_paged_prep: eps beyond 2^62");
-  if ((((uintptr_t)d->nq | (uintptr_t)d->nk | (uintptr_t)d->rope) & 3u) ||
+  if ((((uintptr_t)d->nq | (uintptr_t)d->nk | (uintptr_t)d->rope | (uintptr_t)d->pq | (uintptr_t)d->pk |
+        (uintptr_t)d->pv) & 3u) ||
       (((uintptr_t)d->q0 | (uintptr_t)d->k0 | (uintptr_t)d->v0 | (uintptr_t)d->q) & 1u))
     return corm::fail(CORM_EINVAL, "corm_llm_paged_prep: unaligned buffers");
   if (int rc = corm::check_device()) return rc;
@@ -934,17 +953,22 @@ extern "C" int corm_llm_paged_prep(const corm_llm_paged_prep_desc* d, corm_strea
   auto launch = [&](auto kern) { corm_launch_pdl(kern, dim3((unsigned)grid), dim3(256), 0, st, A); };
   {
     corm::ProfScope prof_("paged_prep_kernel", st);
-    switch (c.HD * 2u + A.vec) {
-      case 32: launch(paged_prep_kernel<16, false>); break;
-      case 33: launch(paged_prep_kernel<16, true>); break;
-      case 64: launch(paged_prep_kernel<32, false>); break;
-      case 65: launch(paged_prep_kernel<32, true>); break;
-      case 128: launch(paged_prep_kernel<64, false>); break;
-      case 129: launch(paged_prep_kernel<64, true>); break;
-      case 256: launch(paged_prep_kernel<128, false>); break;
-      case 257: launch(paged_prep_kernel<128, true>); break;
-      case 512: launch(paged_prep_kernel<256, false>); break;
-      default: launch(paged_prep_kernel<256, true>); break;
+    auto pick = [&](auto hd) {
+      constexpr int W = decltype(hd)::value;
+      if (d->nq || d->nk) {
+        if (A.vec) launch(paged_prep_kernel<W, true, true>);
+        else launch(paged_prep_kernel<W, false, true>);
+      } else {
+        if (A.vec) launch(paged_prep_kernel<W, true, false>);
+        else launch(paged_prep_kernel<W, false, false>);
+      }
+    };
+    switch (c.HD) {
+      case 16: pick(std::integral_constant<int, 16>()); break;
+      case 32: pick(std::integral_constant<int, 32>()); break;
+      case 64: pick(std::integral_constant<int, 64>()); break;
+      case 128: pick(std::integral_constant<int, 128>()); break;
+      default: pick(std::integral_constant<int, 256>()); break;
     }
   }
   return corm::cuda_status("llm_paged_prep");

@@ -69,10 +69,59 @@ __device__ __forceinline__ uint32_t shr_clamp(uint32_t x, uint32_t s) {  // 0 fr
   asm("shr.u32 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(s));
   return r;
 }
-__device__ __forceinline__ uint32_t lds_u16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-  return v;
+// two values saturated to 16 bits in a word (lo in the low half)
+__device__ __forceinline__ uint32_t pack_s16(uint32_t lo, uint32_t hi) {
+  uint32_t r;
+  asm("cvt.pack.sat.s16.s32 %0, %1, %2;" : "=r"(r) : "r"(hi), "r"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_u16(uint32_t lo, uint32_t hi) {
+  uint32_t r;
+  asm("cvt.pack.sat.u16.s32 %0, %1, %2;" : "=r"(r) : "r"(hi), "r"(lo));
+  return r;
+}
+// any registers, out of line
+__device__ __noinline__ uint32_t e_any(uint32_t d, uint32_t cm, uint32_t cs, const uint32_t* tab) {
+  const uint64_t y = ((uint64_t)d * (cm & 0xFFFFFFu)) >> cs;
+  return (y >> 12) > 16u ? 0u : tab[y & 4095u] >> (uint32_t)(y >> 12);
+}
+__device__ __noinline__ uint32_t p_any(uint32_t e, uint32_t R, uint32_t fp) { return smx_p(e, R, fp); }
+
+// A row's softmax registers and maximum as e of a packed score pair wants them
+struct RowE {
+  uint32_t mode;       // 0: 10 <= Cs <= 26; 1: Cs >= 27; 2: any (alike over the warp)
+  uint32_t cm8, cm, cs;
+  int32_t mul;         // mode 0: -2^(26 - Cs)
+  uint32_t m0;         // mode 0: m 2^(26 - Cs); 1: m 2^16; 2: m
+};
+// e of 8 scores (4 packed words).  t = floor(d Cm / 2^(Cs - 2)) = 4 y and two bits:
+// the table's byte offset is t mod 2^14 without them, the octave t / 2^14.  Mode 0
+// brings d to 2^(26 - Cs) as it subtracts, so the product's high word is t itself;
+// mode 1 shifts it down (from Cs = 40 on Cm counts as 0: y is 0)
+__device__ __forceinline__ void e_of8(const RowE& r, const uint32_t* x, uint32_t* e, const uint32_t* tab) {
+  if (r.mode == 2u) {
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      e[k] = e_any((r.m0 - (k & 1 ? x[k >> 1] >> 16 : x[k >> 1])) & 0xFFFFu, r.cm, r.cs, tab);
+    return;
+  }
+  uint32_t t[8];
+  if (r.mode == 0u) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      t[2 * k] = __umulhi((uint32_t)((int32_t)(int16_t)x[k] * r.mul) + r.m0, r.cm8);
+      t[2 * k + 1] = __umulhi((uint32_t)(((int32_t)x[k] >> 16) * r.mul) + r.m0, r.cm8);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      t[2 * k] = __umulhi(r.m0 - (x[k] << 16), r.cm8) >> (r.cs - 10u);
+      t[2 * k + 1] = __umulhi(r.m0 - (x[k] & 0xFFFF0000u), r.cm8) >> (r.cs - 10u);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; k++)
+    e[k] = shr_clamp(*(const uint32_t*)((const uint8_t*)tab + (t[k] & 0x3FFCu)), t[k] >> 14);
 }
 
 template <int HD, int BITS>
@@ -85,6 +134,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ int32_t s_pm[4][BMR], s_m[BMR];
   __shared__ unsigned long long s_s[BMR];
+  __shared__ __align__(16) uint32_t tab[4096];  // the softmax unit's table
   const corm_paged_cache& c = A.d.c;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint32_t X = A.X, G = A.G, g = blockIdx.y, b = blockIdx.z, rank = blockIdx.x % X;
@@ -92,8 +142,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t NST = A.stages, WIN = A.win;
   uint8_t* ring = (uint8_t*)(((uintptr_t)pt_sm + 1023) & ~(uintptr_t)1023);
   uint8_t* s_S = ring + NST * Sh::STAGE;                    // [tile of the window][4][512] 16-byte words
-  uint16_t* tab = (uint16_t*)(s_S + WIN * (BMR * BK * 2u));
-  uint8_t* s_kshift = (uint8_t*)(tab + 4096);               // 8 bits: shifts of the window's K and V rows
+  uint8_t* s_kshift = s_S + WIN * (BMR * BK * 2u);          // 8 bits: shifts of the window's K and V rows
   uint8_t* s_vshift = s_kshift + WIN * BK;
 
   corm_pdl_wait();
@@ -353,7 +402,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     load_q();
     release();
-    for (uint32_t i = tid; i < 4096u; i += ROW_THREADS) tab[i] = (uint16_t)(A.tab[i] - 1);
+    for (uint32_t i = tid; i < 1024u; i += ROW_THREADS) ((int4*)tab)[i] = ((const int4*)A.tab)[i];
     if (tid < BMR) s_s[tid] = 0;
     if (!again) load_shifts(t0, t1);
 
@@ -384,13 +433,15 @@ __global__ void __launch_bounds__(THREADS, 1)
             acc = ((hh[k + x] << 8) + mid[k + x]) << ((shw[k / 4] >> (8u * ((k + x) & 3u))) & 31u);
           y[x] = (int32_t)acc >> 8;
         }
-        asm("cvt.pack.sat.s16.s32 %0, %1, %2;" : "=r"(out[k / 2]) : "r"(y[1]), "r"(y[0]));
+        out[k / 2] = pack_s16((uint32_t)y[0], (uint32_t)y[1]);
       }
     };
     auto masked = [&](uint32_t t) { return t * BK < all_lo || t * BK + BK > all_hi; };
-    // the keys of a packed word seen by this row: 0xFFFF a seen half
-    auto seen = [&](uint32_t key) -> uint32_t {
-      return ((key >= klo && key < khi) ? 0xFFFFu : 0u) | ((key + 1u >= klo && key + 1u < khi) ? 0xFFFF0000u : 0u);
+    // this thread's keys of tile t that the row sees, a bit each
+    auto seen = [&](uint32_t t) -> uint32_t {
+      const uint32_t kb = t * BK + part * 32u;
+      const uint32_t h = khi > kb ? min(khi - kb, 32u) : 0u, l = klo > kb ? min(klo - kb, 32u) : 0u;
+      return (h ? 0xFFFFFFFFu >> (32u - h) : 0u) & (l < 32u ? 0xFFFFFFFFu << l : 0u);
     };
     uint4* S4 = (uint4*)s_S + tid;  // word j of tile i of the window: [(4 i + j) 512]
 
@@ -410,10 +461,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             S4[((t - a) * 4u + 2u * j + 1u) * ROW_THREADS] = make_uint4(o[4], o[5], o[6], o[7]);
           }
           if (masked(t)) {
+            const uint32_t sk = seen(t) >> (16u * j);
 #pragma unroll
             for (uint32_t k = 0; k < 8; k++) {
-              const uint32_t mk = seen(t * BK + part * 32u + j * 16u + 2u * k);
-              o[k] = (o[k] & mk) | (0x80008000u & ~mk);
+              const uint32_t lo16 = (sk >> (2u * k)) & 1u ? o[k] : 0x8000u, hi16 = (sk >> (2u * k)) & 2u ? o[k] : 0x80000000u;
+              o[k] = __byte_perm(lo16, hi16, 0x7610);
             }
           }
 #pragma unroll
@@ -439,23 +491,21 @@ __global__ void __launch_bounds__(THREADS, 1)
       meet();
       for (uint32_t i = 0; i < X; i++) m = max(m, (int32_t)cluster_ld32(cluster_addr(&s_m[row], i)));
     }
-    const uint32_t m2 = ((uint32_t)m & 0xFFFFu) * 0x10001u;
-
-    // e of the packed scores x (two), packed the same way; the sum of both
-    const bool fast = cs >= 9u;
-    const uint32_t cm8 = cs >= 40u ? 0u : (cm & 0xFFFFFFu) << 8, sh1 = cs >= 40u ? 0u : cs - 9u;
-    const uint32_t tab_a = sm100::smem_u32(tab);
-    auto e_of = [&](uint32_t x, uint32_t& e0, uint32_t& e1) {
-      const uint32_t d = __vsub2(m2, x);
-      if (fast) {
-        // 2 y and a bit: the table's byte offset is 2 (y mod 4096), the octave y / 4096
-        const uint32_t y0 = __umulhi(d << 16, cm8) >> sh1, y1 = __umulhi(d & 0xFFFF0000u, cm8) >> sh1;
-        e0 = shr_clamp(lds_u16(tab_a + (y0 & 8190u)) + 1u, y0 >> 13);
-        e1 = shr_clamp(lds_u16(tab_a + (y1 & 8190u)) + 1u, y1 >> 13);
-      } else {
-        e0 = smx_e_wide(d & 0xFFFFu, cm, cs, tab);
-        e1 = smx_e_wide(d >> 16, cm, cs, tab);
+    RowE re;
+    re.cm = cm, re.cs = cs;
+    re.cm8 = cs >= 40u ? 0u : (cm & 0xFFFFFFu) << 8;
+    re.mode = __reduce_max_sync(0xffffffffu, cs < 10u ? 2u : (cs > 26u ? 1u : 0u));
+    re.mul = -(int32_t)(1u << ((26u - min(cs, 26u)) & 31u));
+    re.m0 = re.mode == 0u ? (uint32_t)(-m * re.mul) : (re.mode == 1u ? (uint32_t)m << 16 : (uint32_t)m);
+    if (re.mode == 1u) re.cs = cs >= 40u ? 10u : cs;
+    // e of keys 8 j .. 8 j + 7 of this thread's 32, those unseen 0; their sum
+    auto e_seen = [&](const uint32_t* x, uint32_t* e, bool mk, uint32_t sk) -> uint32_t {
+      e_of8(re, x, e, tab);
+      if (mk) {
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) e[k] = (sk >> k) & 1u ? e[k] : 0u;
       }
+      return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
     };
     // phase 2: e in place (one window), the row's sum
     unsigned long long sum = 0;
@@ -463,25 +513,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       rows_sync();  // the table is there
       for (uint32_t t = t0; t < t1; t++) {
         const bool mk = masked(t);
+        const uint32_t sk = mk ? seen(t) : 0u;
         uint32_t part_sum = 0;
-#pragma unroll
+#pragma unroll 2
         for (uint32_t j = 0; j < 4; j++) {
           uint4& v = S4[((t - t0) * 4u + j) * ROW_THREADS];
-          uint4 x = v;
-          uint32_t* xw = (uint32_t*)&x;
-#pragma unroll
-          for (uint32_t k = 0; k < 4; k++) {
-            uint32_t e0, e1;
-            e_of(xw[k], e0, e1);
-            if (mk) {
-              const uint32_t sk = seen(t * BK + part * 32u + j * 8u + 2u * k);
-              e0 = (sk & 1u) ? e0 : 0u;
-              e1 = (sk >> 31) ? e1 : 0u;
-            }
-            part_sum += e0 + e1;
-            xw[k] = min(e0, 65535u) | (min(e1, 65535u) << 16);
-          }
-          v = x;
+          const uint4 x4 = v;
+          const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w};
+          uint32_t ev[8];
+          part_sum += e_seen(x, ev, mk, sk >> (8u * j));
+          v = make_uint4(pack_u16(ev[0], ev[1]), pack_u16(ev[2], ev[3]), pack_u16(ev[4], ev[5]), pack_u16(ev[6], ev[7]));
         }
         sum += part_sum;
       }
@@ -493,22 +534,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (uint32_t t = a; t < e; t++) {
           acc_wait();
           const bool mk = masked(t);
+          const uint32_t sk = mk ? seen(t) : 0u;
           uint32_t part_sum = 0;
 #pragma unroll
           for (uint32_t j = 0; j < 2; j++) {
-            uint32_t o[8];
+            uint32_t o[8], ev[8];
             scores16(t, a, j, o, j == 1);
-#pragma unroll
-            for (uint32_t k = 0; k < 8; k++) {
-              uint32_t e0, e1;
-              e_of(o[k], e0, e1);
-              if (mk) {
-                const uint32_t sk = seen(t * BK + part * 32u + j * 16u + 2u * k);
-                e0 = (sk & 1u) ? e0 : 0u;
-                e1 = (sk >> 31) ? e1 : 0u;
-              }
-              part_sum += e0 + e1;
-            }
+            part_sum += e_seen(o, ev, mk, sk >> (16u * j));
+            part_sum += e_seen(o + 4, ev, mk, sk >> (16u * j + 8u));
           }
           sum += part_sum;
         }
@@ -522,12 +555,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     else
       total = s_s[row];
     const uint32_t R = smx_r(total);
-    const bool pfast = fp >= 8u && fp <= 15u;
-    const uint32_t Rp = pfast ? R << (fp - 8u) : 0u;
-    auto p_of = [&](uint32_t h) -> uint32_t {  // P of a packed e
-      const uint32_t e = e_unpack(h);
+    // P of a packed e: with 8 <= f_p <= 15 the high word of e R 2^(f_p - 8) + 2^31
+    const bool pfast = __all_sync(0xffffffffu, fp >= 8u && fp <= 15u);
+    const uint32_t Rp = pfast ? R << (fp - 8u) : R;
+    auto p_of = [&](uint32_t h) -> uint32_t {
+      const uint32_t e = h + ((h + 1u) >> 16);
       if (pfast) return (uint32_t)(((uint64_t)e * Rp + (1ull << 31)) >> 32);
-      return smx_p(e, R, fp);
+      return p_any(e, R, fp);
     };
 
     // phase 3
@@ -542,19 +576,17 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (uint32_t t = a; t < e; t++) {
           acc_wait();
           const bool mk = masked(t);
+          const uint32_t sk = mk ? seen(t) : 0u;
 #pragma unroll
           for (uint32_t j = 0; j < 2; j++) {
-            uint32_t o[8];
+            uint32_t o[8], ev[8];
             scores16(t, a, j, o, j == 1);
 #pragma unroll
-            for (uint32_t k = 0; k < 8; k++) {
-              uint32_t e0, e1;
-              e_of(o[k], e0, e1);
-              o[k] = min(e0, 65535u) | (min(e1, 65535u) << 16);
-              if (mk) o[k] &= seen(t * BK + part * 32u + j * 16u + 2u * k);
+            for (uint32_t h = 0; h < 2; h++) {
+              e_seen(o + 4 * h, ev, mk, sk >> (16u * j + 8u * h));
+              S4[((t - a) * 4u + 2u * j + h) * ROW_THREADS] =
+                  make_uint4(pack_u16(ev[0], ev[1]), pack_u16(ev[2], ev[3]), pack_u16(ev[4], ev[5]), pack_u16(ev[6], ev[7]));
             }
-            S4[((t - a) * 4u + 2u * j) * ROW_THREADS] = make_uint4(o[0], o[1], o[2], o[3]);
-            S4[((t - a) * 4u + 2u * j + 1u) * ROW_THREADS] = make_uint4(o[4], o[5], o[6], o[7]);
           }
         }
         rows_sync();  // every warp has read the scores: P goes over their columns
@@ -579,9 +611,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (uint32_t h = 0; h < 2; h++) {
             if (BITS == 16) {
               // saturated to 32767 as signed halves
-              uint32_t w0, w1;
-              asm("cvt.pack.sat.s16.s32 %0, %1, %2;" : "=r"(w0) : "r"(p[4 * h + 1]), "r"(p[4 * h]));
-              asm("cvt.pack.sat.s16.s32 %0, %1, %2;" : "=r"(w1) : "r"(p[4 * h + 3]), "r"(p[4 * h + 2]));
+              const uint32_t w0 = pack_s16(p[4 * h], p[4 * h + 1]), w1 = pack_s16(p[4 * h + 2], p[4 * h + 3]);
               pl[0][2 * j + h] = __byte_perm(w0, w1, 0x6420);
               pl[1][2 * j + h] = __byte_perm(w0, w1, 0x7531);
             } else {
@@ -718,12 +748,12 @@ int launch(TileArgs A, uint32_t tiles, cudaStream_t st) {
   A.X = X;
   A.stages = 3u * 16384u / Sh::STAGE < 2u ? 2u : (3u * 16384u / Sh::STAGE > 6u ? 6u : 3u * 16384u / Sh::STAGE);
   const uint32_t tile_bytes = BMR * BK * 2u + (BITS == 8 ? 2u * BK : 0u);
-  const uint32_t room = 220u * 1024u - 1024u - A.stages * Sh::STAGE - 8192u;
+  const uint32_t room = 206u * 1024u - 1024u - A.stages * Sh::STAGE;  // beside 20 KB of static arrays
   const uint32_t most = room / tile_bytes, need = (ktiles + X - 1u) / X;
   // a cluster's sums use the scores' memory: HD KB / 2
   const uint32_t least = (HD * 512u + BMR * BK * 2u - 1u) / (BMR * BK * 2u);
   A.win = need < least ? least : (need < most ? need : most);
-  const size_t smem = 1024u + A.stages * Sh::STAGE + (size_t)A.win * tile_bytes + 8192u;
+  const size_t smem = 1024u + A.stages * Sh::STAGE + (size_t)A.win * tile_bytes;
   auto kern = paged_attn_tile_kernel<HD, BITS>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return corm::cuda_status("llm_paged_attn");

@@ -53,13 +53,17 @@ class PagedCache:
         self.device = self.kc.device
 
     def desc(self, batch: "PagedBatch") -> _lib.PagedCacheDesc:
-        if batch.device != self.device:
-            _bad(f"paged: the batch is on {batch.device}, the cache on {self.device}")
-        return _lib.PagedCacheDesc(self.kc.data_ptr(), self.vc.data_ptr(),
-                                   None if self.ks is None else self.ks.data_ptr(),
-                                   None if self.vs is None else self.vs.data_ptr(), batch.table.data_ptr(),
-                                   batch.cu.data_ptr(), batch.pos.data_ptr(), self.pages, self.page, self.bits, self.KV,
-                                   self.HD, batch.B, batch.width, batch.rows)
+        """The cache and the batch as the library takes them (made once for a
+        pair: both keep their tensors)."""
+        if batch._pair is not self:
+            if batch.device != self.device:
+                _bad(f"paged: the batch is on {batch.device}, the cache on {self.device}")
+            ptr = [None if t is None else t.data_ptr() for t in (self.kc, self.vc, self.ks, self.vs, batch.table,
+                                                                 batch.cu, batch.pos)]
+            batch._desc = _lib.PagedCacheDesc(*ptr, self.pages, self.page, self.bits, self.KV, self.HD, batch.B,
+                                              batch.width, batch.rows)
+            batch._pair = self
+        return batch._desc
 
 
 class PagedBatch:
@@ -67,7 +71,8 @@ class PagedBatch:
     every block, ``cu`` int32 [B + 1] the row ranges, ``pos`` int32 [B] the
     position of each sequence's first row; ``rows`` the packed rows, ``max_q``
     the most of one sequence, ``max_keys`` the most positions up to a row (a
-    hint)."""
+    hint).  A batch keeps its three tensors; their contents may change between
+    calls."""
 
     def __init__(self, table: torch.Tensor, cu: torch.Tensor, pos: torch.Tensor, rows: int, max_q: Optional[int] = None,
                  max_keys: Optional[int] = None):
@@ -82,6 +87,7 @@ class PagedBatch:
         self.max_q = self.rows if max_q is None else int(max_q)
         self.max_keys = 0x7FFFFFFF if max_keys is None else int(max_keys)
         self.device = table.device
+        self._pair = self._desc = None
 
     @classmethod
     def of(cls, tables: Sequence[Sequence[int]], new: Sequence[int], pos: Sequence[int], device=None,
