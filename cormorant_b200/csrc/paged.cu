@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
   using Sh = SplitShape<HD, BITS>;
   constexpr uint32_t RB = Sh::RB, STB = Sh::STB, NKS = Sh::NKS, DW = Sh::DW, DG = Sh::DG, KG = Sh::KG, NT = Sh::NT;
   extern __shared__ __align__(128) uint8_t pa_sm[];
-  __shared__ uint64_t full[8], empty_k[8], empty_v[8], cbar;
+  __shared__ uint64_t full[8], empty[8], cbar;
   __shared__ int32_t s_wmax[kWarps][kRows], s_m[kRows], s_gm[kRows];
   __shared__ unsigned long long s_s[kRows];
   __shared__ uint32_t s_R[kRows], s_lo[kRows], s_hi[kRows], s_cm[kRows], s_cs[kRows], s_fp[kRows];
@@ -445,8 +445,7 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
   if (tid == 0) {
     for (uint32_t i = 0; i < NST; i++) {
       sm100::mbar_init(&full[i], 1);
-      sm100::mbar_init(&empty_k[i], kWarps);
-      sm100::mbar_init(&empty_v[i], 2u * DG);
+      sm100::mbar_init(&empty[i], kWarps);
     }
     sm100::mbar_init(&cbar, X);
     sm100::fence_mbar_init();
@@ -474,20 +473,13 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
     const uint32_t sub = min(c.page, kT), pieces = kT / sub;
     const int32_t* tb = c.table + (uint64_t)b * c.table_width;
     const uint32_t psh = 31u - __clz(c.page);
-    uint32_t gi = 0, base = 0xFFFFFF00u, used_v = 0;  // used_v: bit i, slot i last held V rows
-    uint32_t par_k = 0, par_v = 0;                    // the parity of each slot's next wait
+    uint32_t gi = 0, base = 0xFFFFFF00u;
     int32_t ids = -1;
     bool ok = true;
     auto emit = [&](bool is_v, uint32_t t) {
       const uint32_t s = gi % NST;
-      if (gi >= NST) {
-        const bool pv = (used_v >> s) & 1u;
-        if (ok) ok = sm100::mbar_wait(pv ? &empty_v[s] : &empty_k[s], ((pv ? par_v : par_k) >> s) & 1u, A.err, 301);
-        if (pv) par_v ^= 1u << s;
-        else par_k ^= 1u << s;
-      }
+      if (gi >= NST && ok) ok = wait_for(&empty[s], ((gi / NST) - 1u) & 1u, A.err, 301);
       ok = __all_sync(0xffffffffu, ok);
-      used_v = (used_v & ~(1u << s)) | ((is_v ? 1u : 0u) << s);
       gi++;
       if (!ok) return;
       const uint32_t b0 = (t * kT) >> psh, b1 = (t * kT + kT - 1u) >> psh;
@@ -515,18 +507,19 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
         if (BITS == 8) bulk_g2s(ring + s * STB + kT * RB + lane * sub, (is_v ? c.vs : c.ks) + line, sub, &full[s]);
       }
     };
-    for (uint32_t t = t0; t < t1; t++) emit(false, t);
-    if (nwin > 1)
-      for (uint32_t t = t0; t < t1; t++) emit(false, t);
-    for (uint32_t a = t0; a < t1; a += A.win) {
-      const uint32_t e = min(a + A.win, t1);
-      if (nwin > 1)
-        for (uint32_t t = a; t < e; t++) emit(false, t);
-      for (uint32_t t = a; t < e; t++) emit(true, t);
-    }
+    // K (v = 0) for the first pass and, in windows, again for the other two; V (v = 1)
+    // behind each window's K of the last
+#pragma unroll 1
+    for (uint32_t pass = 0; pass < 3; pass++)
+#pragma unroll 1
+      for (uint32_t a = t0; a < t1; a += A.win)
+#pragma unroll 1
+        for (uint32_t v = (pass == 0 || nwin > 1) ? 0u : 1u; v < (pass == 2 ? 2u : 1u); v++)
+#pragma unroll 1
+          for (uint32_t t = a; t < min(a + A.win, t1); t++) emit(v == 1u, t);
     // every copy lands before the CTA's shared memory goes away
     for (uint32_t q = gi > NST ? gi - NST : 0u; ok && q < gi; q++)
-      sm100::mbar_wait(&full[q % NST], (q / NST) & 1u, nullptr, 0);
+      wait_for(&full[q % NST], (q / NST) & 1u, nullptr, 0);
     __syncwarp();
     if (X > 1) cluster_sync();
     return;
@@ -573,7 +566,8 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
   int32_t mx0 = INT32_MIN, mx1 = INT32_MIN;
   auto scores = [&](uint32_t t, uint32_t a) {
     const uint32_t s = gi % NST;
-    if (ok) ok = sm100::mbar_wait(&full[s], (gi / NST) & 1u, A.err, 302);
+    if (ok) ok = wait_for(&full[s], (gi / NST) & 1u, A.err, 302);
+    __syncwarp();
     gi++;
     const uint8_t* row = ring + s * STB + (8u * warp + qn) * RB;
     uint32_t hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
@@ -628,7 +622,7 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
       s1 = (sh >> 8) & 31u;
     }
     __syncwarp();
-    if (lane == 0) sm100::mbar_arrive(&empty_k[s]);
+    if (lane == 0) sm100::mbar_arrive(&empty[s]);
     int32_t v[4];
 #pragma unroll
     for (int x = 0; x < 4; x++) {
@@ -766,7 +760,10 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
     consumer_sync();
     for (uint32_t t = a; t < e; t++) {
       const uint32_t s = gi % NST;
-      if (ok) ok = sm100::mbar_wait(&full[s], (gi / NST) & 1u, A.err, 304);  // (every warp, every tile: the parities in order)
+      // every warp takes and leaves every tile, its own 32-key blocks or not: a slot is
+      // not filled again before all have seen it, so no wait falls a phase behind
+      if (ok) ok = wait_for(&full[s], (gi / NST) & 1u, A.err, 304);
+      __syncwarp();
       gi++;
 #pragma unroll
       for (uint32_t half = 0; half < 2; half++) {
@@ -836,9 +833,9 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
             mma_us(acc[j][2], p2, vh[0][j], vh[1][j]);
           }
         }
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&empty_v[s]);
       }
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&empty[s]);
     }
   }
   // the key groups' sums (modulo 2^32: any order), then the cluster's

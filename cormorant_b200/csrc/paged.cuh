@@ -70,9 +70,20 @@ __device__ __forceinline__ uint32_t smx_p(uint32_t e, uint32_t R, uint32_t fp) {
   const uint64_t v = ((uint64_t)e * R + (1ull << (39u - fp))) >> (40u - fp);
   return v > 32767ull ? 32767u : (uint32_t)v;
 }
-// R = floor(2^40 / S) (S >= 2^16 wherever a row sees a key, so R <= 2^24)
+// R = floor(2^40 / S) for 2^16 <= S <= 2^40 (S >= 2^16 wherever a row sees a key).  The
+// single-precision reciprocal is within 2^-22: R0 is within 5 of the quotient (below
+// 2^24), and the exact remainder corrects it: first by its own quotient, then by one
 __device__ __forceinline__ uint32_t smx_r(unsigned long long S) {
-  return S ? (uint32_t)min((1ull << 40) / S, 1ull << 24) : 0u;
+  if (S < 65536ull || S > (1ull << 40)) return 0u;
+  const float inv = __frcp_rn((float)S);
+  uint32_t r = (uint32_t)(1099511627776.0f * inv);
+  long long rem = (1ll << 40) - (long long)(r * S);
+  const int q = (int)((float)rem * inv);  // (towards zero)
+  r += (uint32_t)q;
+  rem -= q * (long long)S;
+  if (rem < 0) r--;
+  else if (rem >= (long long)S) r++;
+  return r;
 }
 
 // four 4-byte rows -> four words of one byte column each
@@ -108,6 +119,32 @@ CORM_MMA_I8(mma_su, "s8", "u8")
 CORM_MMA_I8(mma_us, "u8", "s8")
 CORM_MMA_I8(mma_uu, "u8", "u8")
 #undef CORM_MMA_I8
+
+// ---------------------------------------------------------------- waits
+// Bounded like sm100::mbar_wait; each look may suspend the warp for up to 20 us, so
+// that the many warps that wait here leave the issue slots to those that work.
+__device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(sm100::smem_u32(bar)), "r"(parity), "r"(20000u)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* err, int code) {
+  if (try_wait_long(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!try_wait_long(bar, parity)) {
+    if (clock64() - t0 > 4000000000ll) {
+      if (err) atomicCAS(err, 0, code);
+      return false;
+    }
+  }
+  return true;
+}
 
 // ---------------------------------------------------------------- bulk copies and clusters
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
