@@ -1,30 +1,32 @@
 // corm_llm_paged_attn on 128-row tiles (prompts and chunks): tcgen05 kind::i8
 // on the cache's byte planes.
 //
-// A CTA per (sequence, KV head, 128 rows), a row being (token, head of the
-// group), token-major; with few tiles a cluster of CTAs shares the keys.  As in
-// the 16-row kernel, the unit's e(d) is a table of d = m - score, so nothing can
-// be rescaled as a running maximum moves: three phases over the scores, which
-// stay in shared memory (int16, then e in place) where the CTA's keys fit, and
-// are formed again in windows where they do not.
-//   warps 0..15  rows: thread = (row = TMEM lane, 32 of a tile's 128 keys).  Its
-//                scores, e and P are its own, so the phases meet only at the
-//                row's maximum and sum.  q goes to TMEM as the A operand.
-//     phase 1    tcgen05.ld of the three accumulators (HH, MID, LL), the score
-//                rule, the maximum
-//     phase 2    e by the unit's table, its sum
-//     phase 3    P's bytes into TMEM as the A operand of P.V; at the end the
-//                output rule on P.V's accumulators
-//   warp 16      TMA: per 128 keys the pages' rows (a box per page piece) into a
-//                ring, K tiles then V tiles, running ahead across the phases
-//   warp 17      owns TMEM, issues the MMAs: q.K^T (B K-major, N = 128 keys) and
-//                P.V (the V rows as they are: B MN-major, N = HD)
+// Persistent: a CTA an SM takes items = (128-row tile, sequence, KV head), the rows that
+// see most first, a row being (token, head of the group), token-major; with few items a
+// cluster of CTAs shares an item's keys.  As in the 16-row kernel, the unit's e(d) is a
+// table of d = m - score, so nothing can be rescaled as a running maximum moves: three
+// phases over the scores, which stay in shared memory (int16, then e in place) where the
+// CTA's keys fit, and are formed again in windows where they do not.
+//   row warps    thread = (row = TMEM lane, 32 of a tile's 128 keys).  Its scores, e and
+//                P are its own, so the phases meet only at the row's maximum and sum.
+//                q goes to TMEM as the A operand.
+//     phase 0    tcgen05.ld of the three accumulators (HH, MID, LL), the score rule,
+//                the maximum
+//     phase 1    e by the unit's table, its sum
+//     phase 2    P's bytes into TMEM as the A operand of P.V; at the end the output
+//                rule on P.V's accumulators, while the next item's first scores form
+//   a copy warp  TMA: per tile of keys the pages' rows (a box per page piece) into a
+//                ring, K tiles then V tiles, running ahead across phases and items
+//   an MMA warp  owns TMEM, issues the MMAs: q.K^T (B K-major, N = 128 keys: N = 64 takes
+//                58 cycles against 65, so halves of a tile would double its time) and P.V
+//                (the V rows as they are: B MN-major, N = HD)
 // 16 bits: 2 x 2 planes, sums HH 2^16 + MID 2^8 + LL.  8 bits: the codes are one
 // plane; a K row's shift applies to the score, a V row's to P (three planes).
 // Every sum is modulo 2^32, the rule's own wrap.
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "gemm_i8x4.h"
 #include "paged.cuh"
@@ -33,27 +35,31 @@
 namespace paged {
 namespace {
 
-constexpr uint32_t BMR = 128, BK = 128;  // rows and keys of a tile
-constexpr uint32_t ROW_WARPS = 16, ROW_THREADS = 512, THREADS = 576;
+constexpr uint32_t BMR = 128, BK = 128;              // rows and keys of a tile
+constexpr uint32_t PARTS = 4;                        // row warps a TMEM quarter: 32 keys of a tile a thread
+constexpr uint32_t RW = 4 * PARTS, RT = 32 * RW, THREADS = RT + 64;
+constexpr uint32_t TILE_BYTES = BMR * BK * 2;        // a tile's scores
+constexpr uint32_t ITEMS = 4;                        // items known ahead
 
 template <int HD, int BITS>
 struct Shape {
   static constexpr uint32_t RB = HD * (BITS / 8);       // bytes of a cached row
-  static constexpr uint32_t XB = RB < 128 ? RB : 128;   // bytes of a box row
+  static constexpr uint32_t XB = RB < 128 ? RB : 128;   // bytes of a box row, the swizzle's span
   static constexpr uint32_t HALVES = RB / XB;           // 128 dimensions at 16 bits: the planes apart
   static constexpr uint32_t HALF_BYTES = BK * XB;
   static constexpr uint32_t STAGE = BK * RB;
   static constexpr uint32_t LO = HALVES == 2 ? HALF_BYTES : HD;  // the low plane's offset in a stage
-  static constexpr uint32_t SW = XB;                    // swizzle span
   static constexpr uint32_t NP = BITS == 16 ? 2 : 3;    // planes of P
-  // TMEM columns: scores at 0 (128 each); P.V sums at 0 (HD each), P after them, q last
-  static constexpr uint32_t PCH = HD == 64 ? 128 : 64;  // keys of a P buffer
+  static constexpr uint32_t D = HD / PARTS;             // a thread's dimensions of q and of the output
+  // TMEM columns: the scores' sums at 0 (BK each); P.V's sums at 0 (HD each), P's
+  // buffers of PCH keys after them, q last
+  static constexpr uint32_t PCH = HD == 64 ? 128 : 64;  // keys of a P buffer (two buffers)
+  static constexpr uint32_t CH = BK / PCH;              // buffers a tile fills
   static constexpr uint32_t PCOLS = NP * PCH / 4;
   static constexpr uint32_t P0 = 3 * HD;
   static constexpr uint32_t QC = HD / 4;                // columns of a q plane
   static constexpr uint32_t Q0 = 512 - 2 * QC;
   static constexpr bool Q_OVER = P0 + 2 * PCOLS > Q0;   // P lies over q: q again before scores are formed again
-  static constexpr uint32_t PW = HD == 64 ? ROW_WARPS : ROW_WARPS / 2;  // warps that fill a P buffer
 };
 
 struct TileArgs {
@@ -61,9 +67,11 @@ struct TileArgs {
   const int32_t* tab;
   int* err;
   uint32_t G, X, stages, win;  // win: tiles of a window
+  uint32_t tiles;              // row tiles of the longest sequence
+  uint32_t k8, k16;            // 2^8 and 2^16, as operands (shifts would go to the busier pipe)
 };
 
-__device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+__device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(RT) : "memory"); }
 __device__ __forceinline__ uint32_t shr_clamp(uint32_t x, uint32_t s) {  // 0 from 32 up
   uint32_t r;
   asm("shr.u32 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(s));
@@ -80,48 +88,127 @@ __device__ __forceinline__ uint32_t pack_u16(uint32_t lo, uint32_t hi) {
   asm("cvt.pack.sat.u16.s32 %0, %1, %2;" : "=r"(r) : "r"(hi), "r"(lo));
   return r;
 }
-// any registers, out of line
-__device__ __noinline__ uint32_t e_any(uint32_t d, uint32_t cm, uint32_t cs, const uint32_t* tab) {
-  const uint64_t y = ((uint64_t)d * (cm & 0xFFFFFFu)) >> cs;
-  return (y >> 12) > 16u ? 0u : tab[y & 4095u] >> (uint32_t)(y >> 12);
-}
-__device__ __noinline__ uint32_t p_any(uint32_t e, uint32_t R, uint32_t fp) { return smx_p(e, R, fp); }
-
-// A row's softmax registers and maximum as e of a packed score pair wants them
+// A row's softmax registers and maximum as e of a packed score pair wants them.
+// t = floor(d Cm / 2^(Cs - 2)) = 4 y and two bits: the table's byte offset is t mod
+// 2^14 without them, the octave t / 2^14.
+//   mode 0  19 <= Cs <= 26 (scales of 2^-3 to 2^4): a two-way dot product picks a half
+//           of the pair, multiplies it by -2^(26 - Cs) and adds m 2^(26 - Cs); the
+//           product with Cm 2^8 has t as its high word
+//   mode 1  10 <= Cs: the product of d 2^16 and Cm 2^8, shifted down (from Cs = 40 on
+//           Cm counts as 0: y is 0)
+//   mode 2  any: a Cs below 10 as 10 with Cm 2^(10 - Cs).  Past 24 bits that is a
+//           scale of 2^14 and more, where e is 0 from d = 5 on: d up to 31 is enough,
+//           and Cm up to 2^27 (e is 0 for every d > 0 there)
 struct RowE {
-  uint32_t mode;       // 0: 10 <= Cs <= 26; 1: Cs >= 27; 2: any (alike over the warp)
-  uint32_t cm8, cm, cs;
-  int32_t mul;         // mode 0: -2^(26 - Cs)
-  uint32_t m0;         // mode 0: m 2^(26 - Cs); 1: m 2^16; 2: m
+  uint32_t mode;  // alike over the warp
+  uint32_t cm, sh;
+  int32_t mul;
+  uint32_t m0;
 };
-// e of 8 scores (4 packed words).  t = floor(d Cm / 2^(Cs - 2)) = 4 y and two bits:
-// the table's byte offset is t mod 2^14 without them, the octave t / 2^14.  Mode 0
-// brings d to 2^(26 - Cs) as it subtracts, so the product's high word is t itself;
-// mode 1 shifts it down (from Cs = 40 on Cm counts as 0: y is 0)
-__device__ __forceinline__ void e_of8(const RowE& r, const uint32_t* x, uint32_t* e, const uint32_t* tab) {
-  if (r.mode == 2u) {
-#pragma unroll
-    for (int k = 0; k < 8; k++)
-      e[k] = e_any((r.m0 - (k & 1 ? x[k >> 1] >> 16 : x[k >> 1])) & 0xFFFFu, r.cm, r.cs, tab);
-    return;
+__device__ __forceinline__ RowE row_e(uint32_t cm, uint32_t cs, int32_t m) {
+  RowE r;
+  const uint32_t want = cs < 10u ? 2u : ((cs > 26u || cs < 19u) ? 1u : 0u);
+  r.mode = __reduce_max_sync(0xffffffffu, want);
+  r.cm = cs >= 40u ? 0u : cm << 8;
+  r.sh = cs >= 40u ? 0u : max(cs, 10u) - 10u;
+  r.mul = 0;
+  if (r.mode == 0u) {
+    const uint32_t k = 26u - cs;  // up to 7
+    const uint32_t c8 = (0u - (1u << k)) & 0xFFu;
+    r.mul = (int32_t)(c8 | c8 << 24);
+    r.m0 = (uint32_t)m << k;
+  } else if (r.mode == 1u) {
+    r.m0 = (uint32_t)m << 16;
+  } else {
+    // narrow: 16 bits of d at 2^16 by 24 of Cm at 2^8, down by sh; wide: 5 at 2^19 by 27 at 2^5
+    const uint64_t wide = cs < 10u ? (uint64_t)cm << (10u - cs) : cm;
+    const bool w = wide >> 24;
+    r.m0 = (uint32_t)m;
+    r.mul = w ? 19 : 16;
+    r.cm = w ? (uint32_t)(wide < (1ull << 27) ? wide : (1ull << 27) - 1u) << 5 : (cs >= 40u ? 0u : (uint32_t)wide << 8);
   }
+  return r;
+}
+__device__ __forceinline__ void e_of8(const RowE& r, const uint32_t* x, uint32_t* e, const uint32_t* tab) {
   uint32_t t[8];
   if (r.mode == 0u) {
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      t[2 * k] = __umulhi((uint32_t)((int32_t)(int16_t)x[k] * r.mul) + r.m0, r.cm8);
-      t[2 * k + 1] = __umulhi((uint32_t)(((int32_t)x[k] >> 16) * r.mul) + r.m0, r.cm8);
+      t[2 * k] = __umulhi((uint32_t)__dp2a_lo((int)x[k], r.mul, (int)r.m0), r.cm);
+      t[2 * k + 1] = __umulhi((uint32_t)__dp2a_hi((int)x[k], r.mul, (int)r.m0), r.cm);
     }
-  } else {
+  } else if (r.mode == 1u) {
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      t[2 * k] = __umulhi(r.m0 - (x[k] << 16), r.cm8) >> (r.cs - 10u);
-      t[2 * k + 1] = __umulhi(r.m0 - (x[k] & 0xFFFF0000u), r.cm8) >> (r.cs - 10u);
+      t[2 * k] = __umulhi(r.m0 - (x[k] << 16), r.cm) >> r.sh;
+      t[2 * k + 1] = __umulhi(r.m0 - (x[k] & 0xFFFF0000u), r.cm) >> r.sh;
+    }
+  } else {
+    const uint32_t top = r.mul == 19 ? 31u : 65535u;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const uint32_t d = (r.m0 - (k & 1 ? x[k >> 1] >> 16 : x[k >> 1])) & 0xFFFFu;
+      t[k] = __umulhi(min(d, top) << r.mul, r.cm) >> r.sh;
     }
   }
 #pragma unroll
   for (int k = 0; k < 8; k++)
     e[k] = shr_clamp(*(const uint32_t*)((const uint8_t*)tab + (t[k] & 0x3FFCu)), t[k] >> 14);
+}
+
+// An item: a tile of rows of one sequence and KV head, and this CTA's keys of it
+struct Item {
+  uint32_t b, g, r0, nr, lo_row;  // rows r0 .. r0 + nr - 1 of the sequence, whose first packed row is lo_row
+  uint32_t pos, cap, hi;          // the first row's position; positions of the table; keys seen end before hi
+  uint32_t t0, t1;                // key tiles
+};
+// Item i (tiles of the last rows first, as they see most); false: its tile has no rows.
+__device__ __forceinline__ bool item_at(const TileArgs& A, uint32_t i, uint32_t rank, Item& o) {
+  const corm_paged_cache& c = A.d.c;
+  const uint32_t per_tile = c.B * c.KV, tile = A.tiles - 1u - i / per_tile, rem = i % per_tile, G = A.G, w = A.d.window;
+  o.b = rem / c.KV;
+  o.g = rem % c.KV;
+  const SeqRows s = seq_rows(c, o.b, c.rows);
+  const uint32_t all = min(s.n, A.d.max_q) * G;  // < 2^31 (the host checks)
+  o.r0 = tile * BMR;
+  if (o.r0 >= all) return false;
+  o.nr = min(BMR, all - o.r0);
+  o.lo_row = s.lo;
+  o.pos = s.pos;
+  o.cap = s.cap;
+  const uint32_t i0 = o.r0 / G, i1 = (o.r0 + o.nr - 1u) / G;
+  o.hi = min(s.pos + i1 + 1u, s.cap);
+  const uint32_t lo = (w && s.pos + i0 + 1u > w) ? s.pos + i0 + 1u - w : 0u;
+  const uint32_t tile0 = lo / BK, n = o.hi > lo ? (o.hi + BK - 1u) / BK - tile0 : 0u, per = (n + A.X - 1u) / A.X;
+  o.t0 = tile0 + min(rank * per, n);
+  o.t1 = tile0 + min(rank * per + per, n);
+  return true;
+}
+
+// The grid has a CTA (cluster) an item; those that run take over the ones not yet
+// launched, one at a time (cluster launch control): no counter in memory, none shared
+// by two launches, and whoever is free takes the next.
+__device__ __forceinline__ void ask_next(uint4* answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          sm100::smem_u32(answer)),
+      "r"(sm100::smem_u32(bar))
+      : "memory");
+}
+// the CTA index taken over, or -1: none is left (and none may be asked for again)
+__device__ __forceinline__ int32_t next_taken(const uint4* answer) {
+  uint32_t some, x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t.reg .b32 y, z, u;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, u}, r;\n\t}"
+      : "=&r"(some), "=&r"(x)
+      : "r"(sm100::smem_u32(answer))
+      : "memory");
+  return some ? (int32_t)x : -1;
 }
 
 template <int HD, int BITS>
@@ -130,201 +217,292 @@ __global__ void __launch_bounds__(THREADS, 1)
                            const __grid_constant__ TileArgs A) {
   using Sh = Shape<HD, BITS>;
   extern __shared__ uint8_t pt_sm[];
-  __shared__ uint64_t kv_full[8], kv_empty[8], acc_full, tmem_free, p_full[2], p_empty[2], mma_done, cbar;
+  __shared__ uint64_t kv_full[8], kv_empty[8], s_full, s_free, o_full, p_full[2], p_empty[2], mma_done, cbar;
   __shared__ uint32_t tmem_slot;
-  __shared__ int32_t s_pm[4][BMR], s_m[BMR];
-  __shared__ unsigned long long s_s[BMR];
+  __shared__ int32_t s_pm[PARTS][BMR], s_m[BMR];
+  __shared__ unsigned long long s_ps[PARTS][BMR], s_s[BMR];
   __shared__ __align__(16) uint32_t tab[4096];  // the softmax unit's table
+  __shared__ Item s_item[ITEMS];                // written by the copy warp
+  __shared__ uint32_t s_more[ITEMS];            // 0: the end
+  __shared__ uint64_t item_full[ITEMS], item_free[ITEMS], taken_bar;
+  __shared__ uint32_t s_go;                     // the rows go on with the next item
+  __shared__ __align__(16) uint4 s_taken;
   const corm_paged_cache& c = A.d.c;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-  const uint32_t X = A.X, G = A.G, g = blockIdx.y, b = blockIdx.z, rank = blockIdx.x % X;
-  const uint32_t tile = gridDim.x / X - 1u - blockIdx.x / X;  // the last rows see most: first
-  const uint32_t NST = A.stages, WIN = A.win;
+  const uint32_t X = A.X, G = A.G, rank = blockIdx.x % X, NST = A.stages, WIN = A.win;
   uint8_t* ring = (uint8_t*)(((uintptr_t)pt_sm + 1023) & ~(uintptr_t)1023);
-  uint8_t* s_S = ring + NST * Sh::STAGE;                    // [tile of the window][4][512] 16-byte words
-  uint8_t* s_kshift = s_S + WIN * (BMR * BK * 2u);          // 8 bits: shifts of the window's K and V rows
+  uint8_t* s_S = ring + NST * Sh::STAGE;           // [tile of the window][4][row threads] 16-byte words
+  uint8_t* s_kshift = s_S + WIN * TILE_BYTES;      // 8 bits: shifts of the window's K and V rows
   uint8_t* s_vshift = s_kshift + WIN * BK;
-
-  corm_pdl_wait();
-  corm_pdl_trigger();
-  const SeqRows sq = seq_rows(c, b, c.rows);
-  const uint32_t n = min(sq.n, A.d.max_q);
-  const uint64_t all = (uint64_t)n * G, first = (uint64_t)tile * BMR;
-  if (first >= all) return;  // the cluster's CTAs alike
-  const uint32_t r0 = (uint32_t)first, nr = (uint32_t)min((uint64_t)BMR, all - first);
-  const uint32_t i0 = r0 / G, i1 = (r0 + nr - 1u) / G, w = A.d.window;
-  const uint32_t hi = min(sq.pos + i1 + 1u, sq.cap);
-  const uint32_t lo = (w && sq.pos + i0 + 1u > w) ? sq.pos + i0 + 1u - w : 0u;
-  const uint32_t tile0 = lo / BK, ntile = hi > lo ? (hi + BK - 1u) / BK - tile0 : 0u;
-  const uint32_t per = (ntile + X - 1u) / X;
-  const uint32_t t0 = tile0 + min(rank * per, ntile), t1 = tile0 + min(rank * per + per, ntile);
-  const bool again = t1 - t0 > WIN;  // more than a window
-  // the keys every row of the tile sees: no element is masked there
-  const uint32_t all_lo = (w && sq.pos + i1 + 1u > w) ? sq.pos + i1 + 1u - w : 0u;
-  const uint32_t all_hi = nr == BMR ? min(sq.pos + i0 + 1u, sq.cap) : 0u;
 
   if (tid == 0) {
     for (uint32_t i = 0; i < NST; i++) {
       sm100::mbar_init(&kv_full[i], 1);
       sm100::mbar_init(&kv_empty[i], 1);
     }
-    sm100::mbar_init(&acc_full, 1);
-    sm100::mbar_init(&tmem_free, ROW_WARPS);
+    sm100::mbar_init(&s_full, 1);
+    sm100::mbar_init(&s_free, RW);
+    sm100::mbar_init(&o_full, 1);
     for (int i = 0; i < 2; i++) {
-      sm100::mbar_init(&p_full[i], Sh::PW);
+      sm100::mbar_init(&p_full[i], RW / Sh::CH);
       sm100::mbar_init(&p_empty[i], 1);
     }
+    for (uint32_t i = 0; i < ITEMS; i++) {
+      sm100::mbar_init(&item_full[i], 1);
+      sm100::mbar_init(&item_free[i], RW + 1);
+    }
+    sm100::mbar_init(&taken_bar, 1);
     sm100::mbar_init(&mma_done, 1);
     sm100::mbar_init(&cbar, X);
     sm100::fence_mbar_init();
   }
-  if (warp == 17) sm100::tmem_alloc<512>(&tmem_slot);
+  if (warp == RW + 1u) sm100::tmem_alloc<512>(&tmem_slot);
   sm100::tc_fence_before();
   __syncthreads();
   if (X > 1) cluster_sync();
   sm100::tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  // the prologue above overlaps the kernel before; global memory only after it
+  corm_pdl_wait();
+  corm_pdl_trigger();
+  uint32_t islot = 0, ipar = 0;  // the next item's slot and its parity
 
-  if (warp == 16) {
+  if (warp == RW) {
     // ---------------- the copies
     if (lane == 0) {
       sm100::prefetch_tmap(&map_k);
       sm100::prefetch_tmap(&map_v);
     }
     const uint32_t sub = min(c.page, BK), pieces = BK / sub, psh = 31u - __clz(c.page);
-    const int32_t* tb = c.table + (uint64_t)b * c.table_width;
-    uint32_t gi = 0, base = 0xFFFFFF00u;
-    int32_t ids = -1;
+    uint32_t gi = 0, asked = 0, answered = 0;
     bool ok = true;
-    auto emit = [&](bool is_v, uint32_t t) {
-      const uint32_t s = gi % NST;
-      if (gi >= NST && ok) ok = sm100::mbar_wait(&kv_empty[s], ((gi / NST) - 1u) & 1u, A.err, 311);
+    auto item_slot = [&]() {  // the slot's readers of ITEMS items ago are done
+      if (ok) ok = wait_for(&item_free[islot], ipar ^ 1u, A.err, 321);
       ok = __all_sync(0xffffffffu, ok);
-      gi++;
-      if (!ok) return;
-      const uint32_t b0 = (t * BK) >> psh, b1 = (t * BK + BK - 1u) >> psh;
-      if (b0 < base || b1 >= base + 32u) {  // 32 table entries at a time
-        base = b0;
-        ids = base + lane < c.table_width ? tb[base + lane] : -1;
-      }
-      const uint32_t key = t * BK + lane * sub;
-      const bool in = lane < pieces && key < hi;
-      const int32_t id = __shfl_sync(0xffffffffu, ids, in ? (key >> psh) - base : 0u);
-      const bool good = in && (uint32_t)id < c.pages;
-      uint8_t* dst = ring + s * Sh::STAGE + lane * sub * Sh::XB;
-      if (in && !good) {  // a page of zeros
-        for (uint32_t h = 0; h < Sh::HALVES; h++)
-          for (uint32_t i = 0; i < sub * Sh::XB; i += 16u)
-            *(int4*)(dst + h * Sh::HALF_BYTES + i) = make_int4(0, 0, 0, 0);
-        sm100::fence_proxy_async_smem();
-      }
-      const uint32_t cnt = __popc(__ballot_sync(0xffffffffu, good));
-      if (lane == 0) sm100::mbar_expect_tx(&kv_full[s], cnt * sub * Sh::RB);
-      __syncwarp();
-      if (good) {
-        const uint32_t line = ((uint32_t)id * c.KV + g) * c.page + (key & (c.page - 1u));  // < 2^31 (the host checks)
-        for (uint32_t h = 0; h < Sh::HALVES; h++)
-          sm100::tma_load_2d(dst + h * Sh::HALF_BYTES, is_v ? &map_v : &map_k, &kv_full[s], (int)(h * 128u), (int)line);
-      }
     };
-    for (uint32_t t = t0; t < t1; t++) emit(false, t);
-    if (again)
-      for (uint32_t t = t0; t < t1; t++) emit(false, t);
-    for (uint32_t a = t0; a < t1; a += WIN) {
-      const uint32_t e = min(a + WIN, t1);
-      if (again)
-        for (uint32_t t = a; t < e; t++) emit(false, t);
-      for (uint32_t t = a; t < e; t++) emit(true, t);
+    auto publish = [&](const Item* o) {
+      if (lane == 0) {
+        s_more[islot] = o != nullptr;
+        if (o) s_item[islot] = *o;
+        sm100::mbar_arrive(&item_full[islot]);
+      }
+      __syncwarp();
+      if (++islot == ITEMS) islot = 0, ipar ^= 1u;
+    };
+    auto ask = [&]() {
+      if (X > 1) return;
+      if (lane == 0) {
+        sm100::mbar_expect_tx(&taken_bar, 16);
+        ask_next(&s_taken, &taken_bar);
+      }
+      asked++;
+    };
+    auto taken = [&]() -> int32_t {
+      if (asked == answered) return -1;
+      ok = __all_sync(0xffffffffu, wait_for(&taken_bar, answered & 1u, A.err, 322)) && ok;
+      answered++;
+      const int32_t at = ok ? next_taken(&s_taken) : -1;
+      __syncwarp();
+      sm100::fence_proxy_async_smem();
+      return at;
+    };
+    // publishes the first item with rows from number `at` on, or the end
+    auto find = [&](int32_t at, Item& o) {
+      while (at >= 0 && !item_at(A, (uint32_t)at, rank, o)) {
+        ask();
+        at = taken();
+      }
+      item_slot();
+      const bool some = at >= 0 && ok;
+      publish(some ? &o : nullptr);
+      return some;
+    };
+    Item it;
+    bool more = find((int32_t)(blockIdx.x / X), it);
+    while (more) {
+      ask();
+      const int32_t* tb = c.table + (uint64_t)it.b * c.table_width;
+      uint32_t base = 0xFFFFFF00u;
+      int32_t ids = -1;
+      auto emit = [&](bool is_v, uint32_t t) {
+        const uint32_t s = gi % NST;
+        if (gi >= NST && ok) ok = wait_for(&kv_empty[s], ((gi / NST) - 1u) & 1u, A.err, 311);
+        ok = __all_sync(0xffffffffu, ok);
+        gi++;
+        if (!ok) return;
+        const uint32_t b0 = (t * BK) >> psh, b1 = (t * BK + BK - 1u) >> psh;
+        if (b0 < base || b1 >= base + 32u) {  // 32 table entries at a time
+          base = b0;
+          ids = base + lane < c.table_width ? tb[base + lane] : -1;
+        }
+        const uint32_t key = t * BK + lane * sub;
+        const bool in = lane < pieces && key < it.hi;
+        const int32_t id = __shfl_sync(0xffffffffu, ids, in ? (key >> psh) - base : 0u);
+        const bool good = in && (uint32_t)id < c.pages;
+        uint8_t* dst = ring + s * Sh::STAGE + lane * sub * Sh::XB;
+        if (in && !good) {  // a page of zeros
+          for (uint32_t h = 0; h < Sh::HALVES; h++)
+            for (uint32_t i = 0; i < sub * Sh::XB; i += 16u)
+              *(int4*)(dst + h * Sh::HALF_BYTES + i) = make_int4(0, 0, 0, 0);
+          sm100::fence_proxy_async_smem();
+        }
+        const uint32_t cnt = __popc(__ballot_sync(0xffffffffu, good));
+        if (lane == 0) sm100::mbar_expect_tx(&kv_full[s], cnt * sub * Sh::RB);
+        __syncwarp();
+        if (good) {
+          const uint32_t line = ((uint32_t)id * c.KV + it.g) * c.page + (key & (c.page - 1u));  // < 2^31 (the host checks)
+          for (uint32_t h = 0; h < Sh::HALVES; h++)
+            sm100::tma_load_2d(dst + h * Sh::HALF_BYTES, is_v ? &map_v : &map_k, &kv_full[s], (int)(h * 128u), (int)line);
+        }
+      };
+      const bool again = it.t1 - it.t0 > WIN;
+      // K (v = 0) for the first phase and, in windows, again for the other two; V (v = 1)
+      // behind each window's K of the last
+#pragma unroll 1
+      for (uint32_t t = it.t0; t < it.t1; t++) emit(false, t);
+      // the next item is known before this one's values are read: the rows look for it then
+      Item nx;
+      const bool some = find(taken(), nx);
+#pragma unroll 1
+      for (uint32_t phase = 1; phase < 3; phase++)
+#pragma unroll 1
+        for (uint32_t a = it.t0; a < it.t1; a += WIN)
+#pragma unroll 1
+          for (uint32_t v = again ? 0u : 1u; v < phase; v++)
+#pragma unroll 1
+            for (uint32_t t = a; t < min(a + WIN, it.t1); t++) emit(v == 1u, t);
+      it = nx;
+      more = some;
     }
     // every copy lands before the CTA's shared memory goes away
-    for (uint32_t q = gi > NST ? gi - NST : 0u; ok && q < gi; q++)
-      sm100::mbar_wait(&kv_full[q % NST], (q / NST) & 1u, nullptr, 0);
+    for (uint32_t q = gi > NST ? gi - NST : 0u; ok && q < gi; q++) wait_for(&kv_full[q % NST], (q / NST) & 1u, nullptr, 0);
     __syncwarp();
-  } else if (warp == 17) {
-    // ---------------- the MMAs (one thread)
+  } else if (warp == RW + 1u) {
+    // ---------------- the MMAs (one lane)
     if (lane == 0) {
       constexpr uint32_t MN = 1u << 16;  // B MN-major
-      const uint32_t KSS = sm100::idesc_i8(BMR, BK, 1, 1), KSU = sm100::idesc_i8(BMR, BK, 1, 0);
-      const uint32_t KUS = sm100::idesc_i8(BMR, BK, 0, 1), KUU = sm100::idesc_i8(BMR, BK, 0, 0);
-      const uint32_t VUS = sm100::idesc_i8(BMR, HD, 0, 1) | MN, VUU = sm100::idesc_i8(BMR, HD, 0, 0) | MN;
+      constexpr uint32_t KSS = sm100::idesc_i8(BMR, BK, 1, 1), KSU = sm100::idesc_i8(BMR, BK, 1, 0);
+      constexpr uint32_t KUS = sm100::idesc_i8(BMR, BK, 0, 1), KUU = sm100::idesc_i8(BMR, BK, 0, 0);
+      constexpr uint32_t VUS = sm100::idesc_i8(BMR, HD, 0, 1) | MN, VUU = sm100::idesc_i8(BMR, HD, 0, 0) | MN;
       const uint32_t qh = tmem + Sh::Q0, ql = qh + Sh::QC;
-      uint32_t gi = 0, unit = 0, pt = 0;
+      // a stage's descriptors: the words of its address 0, K-major and MN-major, then
+      // every operand a constant away (16-byte units)
+      const uint64_t k0 = Sh::XB == 128 ? sm100::sdesc_sw128(0) : sm100::sdesc_sw64(0);
+      const uint64_t v0 = Sh::XB == 128 ? sm100::sdesc_sw128_mn(0) : sm100::sdesc_sw64(0);
+      const uint32_t khi = (uint32_t)(k0 >> 32), vhi = (uint32_t)(v0 >> 32);
+      const uint32_t ring_a = sm100::smem_u32(ring);
+      uint32_t s = 0, sp = 0;            // the next ring stage and its parity
+      uint32_t use = 0, pu = 0;          // uses of the scores' columns; P buffers
       bool ok = true;
-      auto desc_k = [&](uint32_t a) { return Sh::SW == 128 ? sm100::sdesc_sw128(a) : sm100::sdesc_sw64(a); };
-      auto desc_v = [&](uint32_t a) { return Sh::SW == 128 ? sm100::sdesc_sw128_mn(a) : sm100::sdesc_sw64(a); };
-      auto stage_in = [&]() -> uint32_t {
-        const uint32_t s = gi % NST;
-        if (ok) ok = sm100::mbar_wait(&kv_full[s], (gi / NST) & 1u, A.err, 312);
-        gi++;
-        return s;
+      auto stage_in = [&]() -> uint32_t {  // the next stage, full: its address / 16
+        if (ok) ok = wait_for(&kv_full[s], sp, A.err, 312);
+        return (ring_a + s * Sh::STAGE) >> 4;
+      };
+      auto stage_out = [&]() {
+        if (ok) sm100::mma_commit(&kv_empty[s]);
+        if (++s == NST) s = 0, sp ^= 1u;
       };
       auto scores = [&]() {  // one tile's q.K^T
-        const uint32_t s = stage_in();
-        if (ok) ok = sm100::mbar_wait(&tmem_free, unit & 1u, A.err, 313);
-        unit++;
-        if (!ok) return;
-        sm100::tc_fence_after();
-        const uint32_t base = sm100::smem_u32(ring + s * Sh::STAGE);
-#pragma unroll
-        for (uint32_t ks = 0; ks < HD / 32; ks++) {
-          const uint64_t kh = desc_k(base + 32u * ks);
-          const uint32_t acc = ks ? 1u : 0u;
-          if (BITS == 16) {
-            const uint64_t kl = desc_k(base + Sh::LO + 32u * ks);
-            sm100::mma_i8_ta(tmem, qh + 8u * ks, kh, KSS, acc);
-            sm100::mma_i8_ta(tmem + 128u, qh + 8u * ks, kl, KSU, acc);
-            sm100::mma_i8_ta(tmem + 128u, ql + 8u * ks, kh, KUS, 1u);
-            sm100::mma_i8_ta(tmem + 256u, ql + 8u * ks, kl, KUU, acc);
-          } else {
-            sm100::mma_i8_ta(tmem, qh + 8u * ks, kh, KSS, acc);
-            sm100::mma_i8_ta(tmem + 128u, ql + 8u * ks, kh, KUS, acc);
-          }
-        }
-        sm100::mma_commit(&kv_empty[s]);
-        sm100::mma_commit(&acc_full);
-      };
-      for (uint32_t t = t0; t < t1; t++) scores();
-      if (again)
-        for (uint32_t t = t0; t < t1; t++) scores();
-      for (uint32_t a = t0; a < t1; a += WIN) {
-        const uint32_t e = min(a + WIN, t1);
-        if (again)
-          for (uint32_t t = a; t < e; t++) scores();
-        if (ok) ok = sm100::mbar_wait(&tmem_free, unit & 1u, A.err, 314);
-        unit++;
-        for (uint32_t t = a; t < e; t++, pt++) {
-          const uint32_t s = stage_in();
-          const uint32_t base = sm100::smem_u32(ring + s * Sh::STAGE);
-#pragma unroll
-          for (uint32_t ch = 0; ch < BK / Sh::PCH; ch++) {
-            const uint32_t buf = HD == 64 ? (pt & 1u) : ch;
-            if (ok) ok = sm100::mbar_wait(&p_full[buf], (HD == 64 ? pt >> 1 : pt) & 1u, A.err, 315);
-            if (!ok) continue;
-            sm100::tc_fence_after();
-            const uint32_t p = tmem + Sh::P0 + buf * Sh::PCOLS;
-#pragma unroll
-            for (uint32_t ks = 0; ks < Sh::PCH / 32; ks++) {
-              const uint32_t k = ch * (Sh::PCH / 32) + ks;  // 32 V rows
-              const uint64_t vh = desc_v(base + k * 32u * Sh::XB);
-              const uint32_t acc = (t != a || k) ? 1u : 0u;
-              const uint32_t p0 = p + 8u * ks, p1 = p0 + Sh::PCH / 4, p2 = p1 + Sh::PCH / 4;
-              if (BITS == 16) {  // P low, P high against V's planes
-                const uint64_t vl = desc_v(base + Sh::LO + k * 32u * Sh::XB);
-                sm100::mma_i8_ta(tmem, p1, vh, VUS, acc);
-                sm100::mma_i8_ta(tmem + HD, p0, vh, VUS, acc);
-                sm100::mma_i8_ta(tmem + HD, p1, vl, VUU, 1u);
-                sm100::mma_i8_ta(tmem + 2 * HD, p0, vl, VUU, acc);
-              } else {
-                sm100::mma_i8_ta(tmem, p2, vh, VUS, acc);
-                sm100::mma_i8_ta(tmem + HD, p1, vh, VUS, acc);
-                sm100::mma_i8_ta(tmem + 2 * HD, p0, vh, VUS, acc);
-              }
+        const uint32_t b = (uint32_t)k0 + stage_in();
+        if (ok) ok = wait_for(&s_free, use & 1u, A.err, 313);
+        use++;
+        if (ok) {
+          sm100::tc_fence_after();
+          auto step = [&](auto ks, auto keep) {
+            constexpr uint32_t K = decltype(ks)::value;
+            constexpr bool KEEP = decltype(keep)::value;
+            const uint32_t bh = b + 2u * K;
+            sm100::mma_i8_tb<KEEP>(tmem, qh + 8u * K, bh, khi, KSS);
+            if constexpr (BITS == 16) {
+              const uint32_t bl = bh + Sh::LO / 16;
+              sm100::mma_i8_tb<KEEP>(tmem + BK, qh + 8u * K, bl, khi, KSU);
+              sm100::mma_i8_tb<true>(tmem + BK, ql + 8u * K, bh, khi, KUS);
+              sm100::mma_i8_tb<KEEP>(tmem + 2 * BK, ql + 8u * K, bl, khi, KUU);
+            } else {
+              sm100::mma_i8_tb<KEEP>(tmem + BK, ql + 8u * K, bh, khi, KUS);
             }
-            sm100::mma_commit(&p_empty[buf]);
+          };
+          using std::integral_constant;
+          step(integral_constant<uint32_t, 0>(), std::false_type());
+          step(integral_constant<uint32_t, 1>(), std::true_type());
+          if constexpr (HD == 128) {
+            step(integral_constant<uint32_t, 2>(), std::true_type());
+            step(integral_constant<uint32_t, 3>(), std::true_type());
           }
-          if (ok) sm100::mma_commit(&kv_empty[s]);
+          sm100::mma_commit(&s_full);
         }
-        if (ok) sm100::mma_commit(&acc_full);
+        stage_out();
+      };
+      auto values = [&](auto first) {  // one tile's P.V, into new sums or the ones there are
+        const uint32_t b = (uint32_t)v0 + stage_in();
+#pragma unroll
+        for (uint32_t ch = 0; ch < Sh::CH; ch++, pu++) {
+          const uint32_t buf = pu & 1u;
+          if (ok) ok = wait_for(&p_full[buf], (pu >> 1) & 1u, A.err, 315);
+          if (!ok) continue;
+          sm100::tc_fence_after();
+          const uint32_t p = tmem + Sh::P0 + buf * Sh::PCOLS;
+          auto step = [&](auto k32, auto keep) {
+            constexpr uint32_t K = decltype(k32)::value;  // 32 V rows
+            constexpr bool KEEP = decltype(keep)::value;
+            const uint32_t bh = b + (ch * Sh::PCH + K * 32u) * Sh::XB / 16u;
+            const uint32_t p0 = p + 8u * K, p1 = p0 + Sh::PCH / 4, p2 = p1 + Sh::PCH / 4;
+            if constexpr (BITS == 16) {  // P low, P high against V's planes
+              const uint32_t bl = bh + Sh::LO / 16;
+              sm100::mma_i8_tb<KEEP>(tmem, p1, bh, vhi, VUS);
+              sm100::mma_i8_tb<KEEP>(tmem + HD, p0, bh, vhi, VUS);
+              sm100::mma_i8_tb<true>(tmem + HD, p1, bl, vhi, VUU);
+              sm100::mma_i8_tb<KEEP>(tmem + 2 * HD, p0, bl, vhi, VUU);
+            } else {
+              sm100::mma_i8_tb<KEEP>(tmem, p2, bh, vhi, VUS);
+              sm100::mma_i8_tb<KEEP>(tmem + HD, p1, bh, vhi, VUS);
+              sm100::mma_i8_tb<KEEP>(tmem + 2 * HD, p0, bh, vhi, VUS);
+            }
+          };
+          using std::integral_constant;
+          if (ch == 0)
+            step(integral_constant<uint32_t, 0>(), std::integral_constant<bool, !decltype(first)::value>());
+          else
+            step(integral_constant<uint32_t, 0>(), std::true_type());
+          step(integral_constant<uint32_t, 1>(), std::true_type());
+          if constexpr (Sh::PCH == 128) {
+            step(integral_constant<uint32_t, 2>(), std::true_type());
+            step(integral_constant<uint32_t, 3>(), std::true_type());
+          }
+          sm100::mma_commit(&p_empty[buf]);
+        }
+        stage_out();
+      };
+      // (one lane walks the items: the others' candidates by itself)
+      while (true) {
+        if (ok) ok = wait_for(&item_full[islot], ipar, A.err, 320);
+        const Item& it = s_item[islot];
+        const bool end = !ok || !s_more[islot];
+        const uint32_t t0 = it.t0, t1 = it.t1;
+        if (end) break;
+        sm100::mbar_arrive(&item_free[islot]);
+        if (++islot == ITEMS) islot = 0, ipar ^= 1u;
+        const bool again = t1 - t0 > WIN;
+        auto taken = [&]() {
+          if (ok) ok = wait_for(&s_free, use & 1u, A.err, 314);
+          use++;
+        };
+        if (t0 == t1) taken();  // no key is seen: the next item's q comes with the next release
+#pragma unroll 1
+        for (uint32_t phase = 0; phase < 3; phase++)
+#pragma unroll 1
+          for (uint32_t a = t0; a < t1; a += WIN) {
+            const uint32_t e = min(a + WIN, t1);
+            if (phase == 0 || again)
+#pragma unroll 1
+              for (uint32_t t = a; t < e; t++) scores();
+            if (phase < 2) continue;
+            taken();  // P.V's sums go over the scores'
+            values(std::true_type());
+#pragma unroll 1
+            for (uint32_t t = a + 1u; t < e; t++) values(std::false_type());
+            if (ok) sm100::mma_commit(&o_full);
+          }
       }
       // every MMA issued has completed before TMEM is freed
       sm100::mma_commit(&mma_done);
@@ -333,146 +511,70 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncwarp();
   } else {
     // ---------------- the rows
-    const uint32_t quarter = warp & 3u, part = warp >> 2, row = quarter * 32u + lane;  // part: 32 of a tile's keys
+    const uint32_t quarter = warp & 3u, part = warp >> 2, row = quarter * 32u + lane;
     const uint32_t lane_base = tmem + ((quarter * 32u) << 16);
-    const uint32_t rr = r0 + min(row, nr - 1u), tok = rr / G, head = g * G + rr % G;
-    const uint32_t pp = sq.pos + tok;
-    const uint32_t khi = row < nr ? min(pp + 1u, sq.cap) : 0u, klo = (w && pp + 1u > w) ? pp + 1u - w : 0u;
-    const uint32_t cm = A.d.smx[2u * head], cfg = A.d.smx[2u * head + 1u], cs = cfg & 63u, fp = (cfg >> 8) & 31u;
-    const int16_t* qrow = A.d.q + (uint64_t)(sq.lo + tok) * A.d.ldq + (uint64_t)head * HD;
+    constexpr uint32_t D = Sh::D;
     const bool q16 = !(((uintptr_t)A.d.q & 15u) | (A.d.ldq & 7u));
-    // q's bytes into TMEM: this warp's quarter of the dimensions of its 32 rows
-    auto load_q = [&]() {
-      constexpr uint32_t D = HD / 4, W = D / 4;  // dimensions and plane words of a part
-      uint32_t h[8], l[8];
+    const bool o16 = !(((uintptr_t)A.d.o & 15u) | (A.d.ldo & 7u));
+    uint4* S4 = (uint4*)s_S + tid;  // word j of tile i of the window: [(4 i + j) RT]
+    bool ok = true;
+    uint32_t su = 0, ou = 0, pt = 0;  // tiles scored, P.V sums taken, tiles of P handed over
+    // q: this part's dimensions of an item's row, from memory and into TMEM
+    auto fetch_q = [&](const Item& o, uint4 (&v)[D / 8]) {
 #pragma unroll
-      for (uint32_t k = 0; k < W; k += 2) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        const int16_t* q = qrow + part * D + 4u * k;
-        if (row < nr) {
-          if (q16)
-            v = *(const uint4*)q;
-          else
-            v = make_uint4(pack16(q[0], q[1]), pack16(q[2], q[3]), pack16(q[4], q[5]), pack16(q[6], q[7]));
-        }
-        h[k] = __byte_perm(v.x, v.y, 0x7531), h[k + 1] = __byte_perm(v.z, v.w, 0x7531);
-        l[k] = __byte_perm(v.x, v.y, 0x6420), l[k + 1] = __byte_perm(v.z, v.w, 0x6420);
+      for (uint32_t k = 0; k < D / 8; k++) v[k] = make_uint4(0, 0, 0, 0);
+      if (row >= o.nr) return;
+      const uint32_t rr = o.r0 + row;
+      const int16_t* q = A.d.q + (uint64_t)(o.lo_row + rr / G) * A.d.ldq + (uint64_t)(o.g * G + rr % G) * HD + part * D;
+#pragma unroll
+      for (uint32_t k = 0; k < D / 8; k++, q += 8) {
+        if (q16)
+          v[k] = *(const uint4*)q;
+        else
+          v[k] = make_uint4(pack16(q[0], q[1]), pack16(q[2], q[3]), pack16(q[4], q[5]), pack16(q[6], q[7]));
       }
-      const uint32_t ta = lane_base + Sh::Q0 + part * W;
+    };
+    auto store_q = [&](const uint4 (&v)[D / 8]) {
+      uint32_t h[D / 4], l[D / 4];
+#pragma unroll
+      for (uint32_t k = 0; k < D / 8; k++) {
+        h[2 * k] = __byte_perm(v[k].x, v[k].y, 0x7531), h[2 * k + 1] = __byte_perm(v[k].z, v[k].w, 0x7531);
+        l[2 * k] = __byte_perm(v[k].x, v[k].y, 0x6420), l[2 * k + 1] = __byte_perm(v[k].z, v[k].w, 0x6420);
+      }
+      const uint32_t ta = lane_base + Sh::Q0 + part * (D / 4);
       __syncwarp();
-      if (W == 8) {
+      if constexpr (D == 32) {
         sm100::tmem_st8(ta, h);
         sm100::tmem_st8(ta + Sh::QC, l);
       } else {
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(ta), "r"(h[0]), "r"(h[1]),
-                     "r"(h[2]), "r"(h[3])
-                     : "memory");
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(ta + Sh::QC), "r"(l[0]),
-                     "r"(l[1]), "r"(l[2]), "r"(l[3])
-                     : "memory");
+        sm100::tmem_st4(ta, h);
+        sm100::tmem_st4(ta + Sh::QC, l);
       }
       sm100::tmem_st_wait();
     };
-    bool ok = true;
-    uint32_t unit = 0;
-    auto release = [&]() {  // TMEM's accumulators (and q) are the MMAs' again
+    auto release = [&]() {  // the scores' columns (and q) are the MMAs' again
       sm100::tc_fence_before();
       __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&tmem_free);
+      if (lane == 0) sm100::mbar_arrive(&s_free);
     };
-    auto acc_wait = [&]() {
-      if (ok) ok = sm100::mbar_wait(&acc_full, unit & 1u, A.err, 316);
-      unit++;
-      __syncwarp();
-      sm100::tc_fence_after();
+    for (uint32_t i = tid; i < 1024u; i += RT) ((int4*)tab)[i] = ((const int4*)A.tab)[i];
+    // whether a slot holds an item: the first row warp waits for it and tells the others
+    // across a barrier, so that all leave together whatever ran out
+    auto look = [&](uint32_t slot, uint32_t par) {
+      if (warp != 0) return;
+      if (ok) ok = wait_for(&item_full[slot], par, A.err, 323);
+      const bool some = __all_sync(0xffffffffu, ok && s_more[slot] != 0u);
+      if (lane == 0) s_go = some;
     };
-    // the shifts of the window's cached rows (8 bits)
-    auto load_shifts = [&](uint32_t a, uint32_t e) {
-      if (BITS == 16) return;
-      rows_sync();
-      for (uint32_t i = tid; i < (e - a) * BK; i += ROW_THREADS) {
-        const uint32_t key = a * BK + i;
-        const int32_t id = key < hi ? c.table[(uint64_t)b * c.table_width + key / c.page] : -1;
-        const bool good = (uint32_t)id < c.pages;
-        const uint64_t line = good ? ((uint64_t)(uint32_t)id * c.KV + g) * c.page + key % c.page : 0u;
-        s_kshift[i] = good ? c.ks[line] & 31u : 0u;
-        s_vshift[i] = good ? c.vs[line] & 31u : 0u;
-      }
-      rows_sync();
-    };
-    load_q();
-    release();
-    for (uint32_t i = tid; i < 1024u; i += ROW_THREADS) ((int4*)tab)[i] = ((const int4*)A.tab)[i];
-    if (tid < BMR) s_s[tid] = 0;
-    if (!again) load_shifts(t0, t1);
-
-    // 16 scores of this thread's keys (half j of its 32) in tile t: 8 packed words
-    auto scores16 = [&](uint32_t t, uint32_t a, uint32_t j, uint32_t (&out)[8], bool last) {
-      uint32_t hh[16], mid[16], ll[16];
-      const uint32_t col = lane_base + part * 32u + j * 16u;
-      __syncwarp();
-      sm100::tmem_ld16(col, hh);
-      sm100::tmem_ld16(col + 128u, mid);
-      if (BITS == 16) sm100::tmem_ld16(col + 256u, ll);
-      sm100::tmem_ld_wait();
-      if (last) release();
-      uint32_t shw[4];
-      if (BITS == 8) {
-        const uint4 v = *(const uint4*)(s_kshift + (t - a) * BK + part * 32u + j * 16u);
-        shw[0] = v.x, shw[1] = v.y, shw[2] = v.z, shw[3] = v.w;
-      }
-#pragma unroll
-      for (uint32_t k = 0; k < 16; k += 2) {
-        int32_t y[2];
-#pragma unroll
-        for (uint32_t x = 0; x < 2; x++) {
-          uint32_t acc;
-          if (BITS == 16)
-            acc = (hh[k + x] << 16) + (mid[k + x] << 8) + ll[k + x];
-          else
-            acc = ((hh[k + x] << 8) + mid[k + x]) << ((shw[k / 4] >> (8u * ((k + x) & 3u))) & 31u);
-          y[x] = (int32_t)acc >> 8;
-        }
-        out[k / 2] = pack_s16((uint32_t)y[0], (uint32_t)y[1]);
-      }
-    };
-    auto masked = [&](uint32_t t) { return t * BK < all_lo || t * BK + BK > all_hi; };
-    // this thread's keys of tile t that the row sees, a bit each
-    auto seen = [&](uint32_t t) -> uint32_t {
-      const uint32_t kb = t * BK + part * 32u;
-      const uint32_t h = khi > kb ? min(khi - kb, 32u) : 0u, l = klo > kb ? min(klo - kb, 32u) : 0u;
-      return (h ? 0xFFFFFFFFu >> (32u - h) : 0u) & (l < 32u ? 0xFFFFFFFFu << l : 0u);
-    };
-    uint4* S4 = (uint4*)s_S + tid;  // word j of tile i of the window: [(4 i + j) 512]
-
-    // phase 1
-    uint32_t mx = 0x80008000u;
-    for (uint32_t a = t0; a < t1; a += WIN) {
-      const uint32_t e = min(a + WIN, t1);
-      if (again) load_shifts(a, e);
-      for (uint32_t t = a; t < e; t++) {
-        acc_wait();
-#pragma unroll
-        for (uint32_t j = 0; j < 2; j++) {
-          uint32_t o[8];
-          scores16(t, a, j, o, j == 1);
-          if (!again) {
-            S4[((t - a) * 4u + 2u * j) * ROW_THREADS] = make_uint4(o[0], o[1], o[2], o[3]);
-            S4[((t - a) * 4u + 2u * j + 1u) * ROW_THREADS] = make_uint4(o[4], o[5], o[6], o[7]);
-          }
-          if (masked(t)) {
-            const uint32_t sk = seen(t) >> (16u * j);
-#pragma unroll
-            for (uint32_t k = 0; k < 8; k++) {
-              const uint32_t lo16 = (sk >> (2u * k)) & 1u ? o[k] : 0x8000u, hi16 = (sk >> (2u * k)) & 2u ? o[k] : 0x80000000u;
-              o[k] = __byte_perm(lo16, hi16, 0x7610);
-            }
-          }
-#pragma unroll
-          for (uint32_t k = 0; k < 8; k++) mx = __vmaxs2(mx, o[k]);
-        }
-      }
+    look(0, 0);
+    rows_sync();
+    bool more = s_go != 0u;
+    if (more) {
+      uint4 v[D / 8];
+      fetch_q(s_item[0], v);
+      store_q(v);
     }
+    release();
     uint32_t cphase = 0;
     // every CTA of the cluster is here, and what it wrote before is visible
     auto meet = [&]() {
@@ -483,221 +585,382 @@ __global__ void __launch_bounds__(THREADS, 1)
         cphase ^= 1u;
       }
     };
-    s_pm[part][row] = max((int32_t)(int16_t)(mx & 0xFFFFu), (int32_t)mx >> 16);
-    rows_sync();
-    int32_t m = max(max(s_pm[0][row], s_pm[1][row]), max(s_pm[2][row], s_pm[3][row]));
-    if (X > 1) {
-      if (part == 0) s_m[row] = m;
-      meet();
-      for (uint32_t i = 0; i < X; i++) m = max(m, (int32_t)cluster_ld32(cluster_addr(&s_m[row], i)));
-    }
-    RowE re;
-    re.cm = cm, re.cs = cs;
-    re.cm8 = cs >= 40u ? 0u : (cm & 0xFFFFFFu) << 8;
-    re.mode = __reduce_max_sync(0xffffffffu, cs < 10u ? 2u : (cs > 26u ? 1u : 0u));
-    re.mul = -(int32_t)(1u << ((26u - min(cs, 26u)) & 31u));
-    re.m0 = re.mode == 0u ? (uint32_t)(-m * re.mul) : (re.mode == 1u ? (uint32_t)m << 16 : (uint32_t)m);
-    if (re.mode == 1u) re.cs = cs >= 40u ? 10u : cs;
-    // e of keys 8 j .. 8 j + 7 of this thread's 32, those unseen 0; their sum
-    auto e_seen = [&](const uint32_t* x, uint32_t* e, bool mk, uint32_t sk) -> uint32_t {
-      e_of8(re, x, e, tab);
-      if (mk) {
-#pragma unroll
-        for (uint32_t k = 0; k < 8; k++) e[k] = (sk >> k) & 1u ? e[k] : 0u;
-      }
-      return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-    };
-    // phase 2: e in place (one window), the row's sum
-    unsigned long long sum = 0;
-    if (!again) {
-      rows_sync();  // the table is there
-      for (uint32_t t = t0; t < t1; t++) {
-        const bool mk = masked(t);
-        const uint32_t sk = mk ? seen(t) : 0u;
-        uint32_t part_sum = 0;
-#pragma unroll 2
-        for (uint32_t j = 0; j < 4; j++) {
-          uint4& v = S4[((t - t0) * 4u + j) * ROW_THREADS];
-          const uint4 x4 = v;
-          const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w};
-          uint32_t ev[8];
-          part_sum += e_seen(x, ev, mk, sk >> (8u * j));
-          v = make_uint4(pack_u16(ev[0], ev[1]), pack_u16(ev[2], ev[3]), pack_u16(ev[4], ev[5]), pack_u16(ev[6], ev[7]));
+#pragma unroll 1
+    while (more) {
+      const uint32_t cur = islot;
+      if (++islot == ITEMS) islot = 0, ipar ^= 1u;
+      const Item& it = s_item[cur];
+      const uint32_t t0 = it.t0, t1 = it.t1;
+      const bool again = t1 - t0 > WIN;  // more than a window
+      const uint32_t rr = it.r0 + min(row, it.nr - 1u), head = it.g * G + rr % G, pp = it.pos + rr / G, w = A.d.window;
+      const uint32_t khi = row < it.nr ? min(pp + 1u, it.cap) : 0u, klo = (w && pp + 1u > w) ? pp + 1u - w : 0u;
+      // the rows of this warp see all, or none, of its 32 keys: known without a look at the elements
+      auto unseen = [&](uint32_t key) { return __all_sync(0xffffffffu, key >= khi || key + 32u <= klo); };
+      auto whole = [&](uint32_t key) { return __all_sync(0xffffffffu, key + 32u <= khi && key >= klo); };
+      // the keys of [key, key + 32) that this row sees, a bit each
+      auto seen = [&](uint32_t key) -> uint32_t {
+        const uint32_t h = khi > key ? min(khi - key, 32u) : 0u, l = klo > key ? min(klo - key, 32u) : 0u;
+        return (h ? 0xFFFFFFFFu >> (32u - h) : 0u) & (l < 32u ? 0xFFFFFFFFu << l : 0u);
+      };
+      // the shifts of the window's cached rows (8 bits)
+      auto load_shifts = [&](uint32_t a, uint32_t e) {
+        if (BITS == 16) return;
+        rows_sync();
+        for (uint32_t i = tid; i < (e - a) * BK; i += RT) {
+          const uint32_t key = a * BK + i;
+          const int32_t id = key < it.hi ? c.table[(uint64_t)it.b * c.table_width + key / c.page] : -1;
+          const bool good = (uint32_t)id < c.pages;
+          const uint64_t line = good ? ((uint64_t)(uint32_t)id * c.KV + it.g) * c.page + key % c.page : 0u;
+          s_kshift[i] = good ? c.ks[line] & 31u : 0u;
+          s_vshift[i] = good ? c.vs[line] & 31u : 0u;
         }
-        sum += part_sum;
-      }
-    } else {
-      for (uint32_t a = t0; a < t1; a += WIN) {
-        const uint32_t e = min(a + WIN, t1);
-        load_shifts(a, e);
-        if (BITS == 16) rows_sync();
-        for (uint32_t t = a; t < e; t++) {
-          acc_wait();
-          const bool mk = masked(t);
-          const uint32_t sk = mk ? seen(t) : 0u;
-          uint32_t part_sum = 0;
-#pragma unroll
-          for (uint32_t j = 0; j < 2; j++) {
-            uint32_t o[8], ev[8];
-            scores16(t, a, j, o, j == 1);
-            part_sum += e_seen(o, ev, mk, sk >> (16u * j));
-            part_sum += e_seen(o + 4, ev, mk, sk >> (16u * j + 8u));
-          }
-          sum += part_sum;
-        }
-      }
-    }
-    atomicAdd(&s_s[row], sum);
-    meet();
-    unsigned long long total = 0;
-    if (X > 1)
-      for (uint32_t i = 0; i < X; i++) total += cluster_ld64(cluster_addr(&s_s[row], i));
-    else
-      total = s_s[row];
-    const uint32_t R = smx_r(total);
-    // P of a packed e: with 8 <= f_p <= 15 the high word of e R 2^(f_p - 8) + 2^31
-    const bool pfast = __all_sync(0xffffffffu, fp >= 8u && fp <= 15u);
-    const uint32_t Rp = pfast ? R << (fp - 8u) : R;
-    auto p_of = [&](uint32_t h) -> uint32_t {
-      const uint32_t e = h + ((h + 1u) >> 16);
-      if (pfast) return (uint32_t)(((uint64_t)e * Rp + (1ull << 31)) >> 32);
-      return p_any(e, R, fp);
-    };
+        rows_sync();
+      };
+      if (!again) load_shifts(t0, t1);
 
-    // phase 3
-    uint32_t oacc[HD / 4];
+      RowE re{};
+      uint32_t mx = 0x80008000u;
+      unsigned long long sum = 0;
+      auto packed_e = [&](const uint32_t* e) {
+        return make_uint4(pack_u16(e[0], e[1]), pack_u16(e[2], e[3]), pack_u16(e[4], e[5]), pack_u16(e[6], e[7]));
+      };
+      // tile t's scores.  Phase 0: their maximum, and the scores into the window where it
+      // holds all; in windows, phase 1: the sum of e, 2: e into the window
+      auto score_pass = [&](uint32_t t, uint32_t a, const uint32_t phase) {
+        if (ok) ok = wait_for(&s_full, su & 1u, A.err, 316);
+        su++;
+        __syncwarp();
+        sm100::tc_fence_after();
+        const uint32_t key = t * BK + part * 32u;
+        if (unseen(key)) {
+          release();
+          return;
+        }
+        const bool mk = !whole(key);
+        const uint32_t sk = mk ? seen(key) : 0u;
+        uint32_t tile_sum = 0;
 #pragma unroll
-    for (uint32_t k = 0; k < HD / 4; k++) oacc[k] = 0;
-    uint32_t pt = 0;
-    for (uint32_t a = t0; a < t1; a += WIN) {
-      const uint32_t e = min(a + WIN, t1);
-      if (again) {
-        load_shifts(a, e);
-        for (uint32_t t = a; t < e; t++) {
-          acc_wait();
-          const bool mk = masked(t);
-          const uint32_t sk = mk ? seen(t) : 0u;
+        for (uint32_t j = 0; j < 2; j++) {
+          uint32_t hh[16], mid[16], ll[16], o[8];
+          const uint32_t col = lane_base + part * 32u + j * 16u;
+          sm100::tmem_ld16(col, hh);
+          sm100::tmem_ld16(col + BK, mid);
+          if (BITS == 16) sm100::tmem_ld16(col + 2 * BK, ll);
+          sm100::tmem_ld_wait();
+          if (j == 1) release();
+          uint32_t shw[4];
+          if (BITS == 8) {
+            const uint4 v = *(const uint4*)(s_kshift + (key - a * BK) + j * 16u);
+            shw[0] = v.x, shw[1] = v.y, shw[2] = v.z, shw[3] = v.w;
+          }
 #pragma unroll
-          for (uint32_t j = 0; j < 2; j++) {
-            uint32_t o[8], ev[8];
-            scores16(t, a, j, o, j == 1);
+          for (uint32_t k = 0; k < 16; k += 2) {
+            uint32_t y[2];
 #pragma unroll
-            for (uint32_t h = 0; h < 2; h++) {
-              e_seen(o + 4 * h, ev, mk, sk >> (16u * j + 8u * h));
-              S4[((t - a) * 4u + 2u * j + h) * ROW_THREADS] =
-                  make_uint4(pack_u16(ev[0], ev[1]), pack_u16(ev[2], ev[3]), pack_u16(ev[4], ev[5]), pack_u16(ev[6], ev[7]));
+            for (uint32_t x = 0; x < 2; x++) {
+              uint32_t acc;
+              if (BITS == 16)
+                acc = hh[k + x] * A.k16 + (mid[k + x] * A.k8 + ll[k + x]);
+              else
+                acc = (hh[k + x] * A.k8 + mid[k + x]) << ((shw[k / 4] >> (8u * ((k + x) & 3u))) & 31u);
+              y[x] = (uint32_t)((int32_t)acc >> 8);
+            }
+            o[k / 2] = pack_s16(y[0], y[1]);
+          }
+          uint4* dst = S4 + ((t - a) * 4u + 2u * j) * RT;
+          if (phase == 0) {
+            if (!again) {
+              dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+              dst[RT] = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+            if (mk) {
+#pragma unroll
+              for (uint32_t k = 0; k < 8; k++) {
+                const uint32_t two = sk >> (16u * j + 2u * k);
+                o[k] = __byte_perm((two & 1u) ? o[k] : 0x8000u, (two & 2u) ? o[k] : 0x80000000u, 0x7610);
+              }
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++) mx = __vmaxs2(mx, o[k]);
+          } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 2; i++) {
+              uint32_t ev[8];
+              e_of8(re, o + 4 * i, ev, tab);
+              if (mk) {
+#pragma unroll
+                for (uint32_t k = 0; k < 8; k++) ev[k] = (sk >> (16u * j + 8u * i + k)) & 1u ? ev[k] : 0u;
+              }
+              if (phase == 1) {
+#pragma unroll
+                for (uint32_t k = 0; k < 8; k++) tile_sum += ev[k];
+              } else {
+                dst[i * RT] = packed_e(ev);
+              }
             }
           }
         }
-        rows_sync();  // every warp has read the scores: P goes over their columns
-      }
-      for (uint32_t t = a; t < e; t++, pt++) {
-        const uint32_t buf = HD == 64 ? (pt & 1u) : part >> 1;
-        const uint32_t uses = HD == 64 ? pt >> 1 : pt;  // of this buffer, before
-        if (uses && ok) ok = sm100::mbar_wait(&p_empty[buf], (uses - 1u) & 1u, A.err, 318);
-        sm100::tc_fence_after();
-        uint32_t pl[3][8];
+        sum += tile_sum;
+      };
+      // one window: tile t's scores to e in place (0 where unseen), their sum
+      auto e_pass = [&](uint32_t t, uint32_t a) {
+        const uint32_t key = t * BK + part * 32u;
+        uint4* w4 = S4 + (t - a) * 4u * RT;
+        if (unseen(key)) return;
+        const bool mk = !whole(key);
+        const uint32_t sk = mk ? seen(key) : 0u;
+        uint32_t tile_sum = 0;
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
-          const uint4 v = S4[((t - a) * 4u + j) * ROW_THREADS];
-          const uint32_t xw[4] = {v.x, v.y, v.z, v.w};
-          uint32_t p[8];
+          uint32_t ev[8];
+          const uint4 v = w4[j * RT];
+          e_of8(re, (const uint32_t*)&v, ev, tab);
+          if (mk) {
 #pragma unroll
-          for (uint32_t k = 0; k < 4; k++) {
-            p[2 * k] = p_of(xw[k] & 0xFFFFu);
-            p[2 * k + 1] = p_of(xw[k] >> 16);
+            for (uint32_t k = 0; k < 8; k++) ev[k] = (sk >> (8u * j + k)) & 1u ? ev[k] : 0u;
           }
 #pragma unroll
-          for (uint32_t h = 0; h < 2; h++) {
-            if (BITS == 16) {
-              // saturated to 32767 as signed halves
-              const uint32_t w0 = pack_s16(p[4 * h], p[4 * h + 1]), w1 = pack_s16(p[4 * h + 2], p[4 * h + 3]);
-              pl[0][2 * j + h] = __byte_perm(w0, w1, 0x6420);
-              pl[1][2 * j + h] = __byte_perm(w0, w1, 0x7531);
-            } else {
-              const uint32_t sw = *(const uint32_t*)(s_vshift + (t - a) * BK + part * 32u + j * 8u + 4u * h);
-              uint32_t y[4];
+          for (uint32_t k = 0; k < 8; k++) tile_sum += ev[k];
+          w4[j * RT] = packed_e(ev);
+        }
+        sum += tile_sum;
+      };
+      uint32_t R = 0, Rp = 0;
+      bool pfast = true;
+      // tile t's e to the bytes of P, into the MMAs' operand.  With 8 <= f_p <= 15 P is
+      // the high word of e R 2^(f_p - 8) + 2^31; with any other f_p P is formed in place
+      // before, and taken as it is
+      auto p_any = [&](uint32_t t, uint32_t a, uint32_t fp) {
+        uint32_t* w = (uint32_t*)(S4 + (t - a) * 4u * RT);
+#pragma unroll 1
+        for (uint32_t i = 0; i < 16 && !unseen(t * BK + part * 32u); i++) {
+          uint32_t& x = w[(i >> 2) * 4u * RT + (i & 3u)];
+          x = smx_p(e_unpack(x & 0xFFFFu), R, fp) | smx_p(e_unpack(x >> 16), R, fp) << 16;
+        }
+      };
+      auto p_pass = [&](uint32_t t, uint32_t a) {
+        const uint32_t pu = pt * Sh::CH + part / (Sh::PCH / 32u), buf = pu & 1u, uses = pu >> 1, key = t * BK + part * 32u;
+        pt++;
+        uint32_t pl[3][8];
+        if (unseen(key)) {
 #pragma unroll
-              for (uint32_t x = 0; x < 4; x++) y[x] = min(p[4 * h + x], 32767u) << ((sw >> (8u * x)) & 31u);
-              const uint32_t f = __byte_perm(y[0], y[1], 0x5140), q = __byte_perm(y[2], y[3], 0x5140);
-              pl[0][2 * j + h] = __byte_perm(f, q, 0x5410);
-              pl[1][2 * j + h] = __byte_perm(f, q, 0x7632);
-              pl[2][2 * j + h] = __byte_perm(__byte_perm(y[0], y[1], 0x0062), __byte_perm(y[2], y[3], 0x0062), 0x5410);
+          for (uint32_t k = 0; k < 24; k++) pl[k / 8][k % 8] = 0;
+        } else {
+#pragma unroll
+          for (uint32_t j = 0; j < 4; j++) {
+            const uint4 v = S4[((t - a) * 4u + j) * RT];
+            const uint32_t xw[4] = {v.x, v.y, v.z, v.w};
+            uint32_t p[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++) {
+              const uint32_t u = k & 1u ? xw[k / 2] >> 16 : xw[k / 2] & 0xFFFFu, ee = u + ((u + 1u) >> 16);
+              p[k] = pfast ? (uint32_t)(((uint64_t)ee * Rp + (1ull << 31)) >> 32) : u;
+            }
+#pragma unroll
+            for (uint32_t q = 0; q < 2; q++) {
+              if (BITS == 16) {
+                // saturated to 32767 as signed halves
+                const uint32_t w0 = pack_s16(p[4 * q], p[4 * q + 1]), w1 = pack_s16(p[4 * q + 2], p[4 * q + 3]);
+                pl[0][2 * j + q] = __byte_perm(w0, w1, 0x6420);
+                pl[1][2 * j + q] = __byte_perm(w0, w1, 0x7531);
+              } else {
+                const uint32_t sw = *(const uint32_t*)(s_vshift + (key - a * BK) + j * 8u + 4u * q);
+                uint32_t y[4];
+#pragma unroll
+                for (uint32_t x = 0; x < 4; x++) y[x] = min(p[4 * q + x], 32767u) << ((sw >> (8u * x)) & 31u);
+                const uint32_t f = __byte_perm(y[0], y[1], 0x5140), z = __byte_perm(y[2], y[3], 0x5140);
+                pl[0][2 * j + q] = __byte_perm(f, z, 0x5410);
+                pl[1][2 * j + q] = __byte_perm(f, z, 0x7632);
+                pl[2][2 * j + q] = __byte_perm(__byte_perm(y[0], y[1], 0x0062), __byte_perm(y[2], y[3], 0x0062), 0x5410);
+              }
             }
           }
         }
-        const uint32_t ta = lane_base + Sh::P0 + buf * Sh::PCOLS + (HD == 64 ? part : part & 1u) * 8u;
+        if (uses && ok) ok = wait_for(&p_empty[buf], (uses - 1u) & 1u, A.err, 318);
         __syncwarp();
+        sm100::tc_fence_after();
+        const uint32_t ta = lane_base + Sh::P0 + buf * Sh::PCOLS + (part % (Sh::PCH / 32u)) * 8u;
 #pragma unroll
         for (uint32_t k = 0; k < Sh::NP; k++) sm100::tmem_st8(ta + k * (Sh::PCH / 4), pl[k]);
         sm100::tmem_st_wait();
         sm100::tc_fence_before();
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(&p_full[buf]);
-      }
-      // the window's P.V: this warp's quarter of the dimensions
-      acc_wait();
+      };
+
+#pragma unroll 1
+      for (uint32_t phase = 0; phase < 2; phase++) {
+#pragma unroll 1
+        for (uint32_t a = t0; a < t1; a += WIN) {
+          const uint32_t e = min(a + WIN, t1);
+          if (again) load_shifts(a, e);
+          if (phase == 0 || again)
+#pragma unroll 1
+            for (uint32_t t = a; t < e; t++) score_pass(t, a, phase);
+          else
+#pragma unroll 1
+            for (uint32_t t = a; t < e; t++) e_pass(t, a);
+        }
+        if (phase == 0) {
+          s_pm[part][row] = max((int32_t)(int16_t)(mx & 0xFFFFu), (int32_t)mx >> 16);
+          rows_sync();
+          int32_t m = s_pm[0][row];
 #pragma unroll
-      for (uint32_t k = 0; k < HD / 4; k += 16) {
-        uint32_t hh[16], mid[16], ll[16];
-        const uint32_t col = lane_base + part * (HD / 4) + k;
-        sm100::tmem_ld16(col, hh);
-        sm100::tmem_ld16(col + HD, mid);
-        sm100::tmem_ld16(col + 2 * HD, ll);
-        sm100::tmem_ld_wait();
-#pragma unroll
-        for (uint32_t x = 0; x < 16; x++) oacc[k + x] += (hh[x] << 16) + (mid[x] << 8) + ll[x];
+          for (uint32_t i = 1; i < PARTS; i++) m = max(m, s_pm[i][row]);
+          if (X > 1) {
+            if (part == 0) s_m[row] = m;
+            meet();
+            for (uint32_t i = 0; i < X; i++) m = max(m, (int32_t)cluster_ld32(cluster_addr(&s_m[row], i)));
+          }
+          re = row_e(A.d.smx[2u * head] & 0xFFFFFFu, A.d.smx[2u * head + 1u] & 63u, m);
+        }
       }
-      if (Sh::Q_OVER && e < t1) load_q();
-      release();
-    }
-    constexpr uint32_t D = HD / 4;  // this thread's dimensions
-    if (X > 1) {
-      // the cluster's sums: every CTA leaves its own in shared memory, and adds up a slice
+      look(islot, ipar);
+      s_ps[part][row] = sum;
       rows_sync();
-      uint4* so = (uint4*)s_S;  // [D / 4][512]
+      {
+        unsigned long long total = s_ps[0][row];
 #pragma unroll
-      for (uint32_t k = 0; k < D; k += 4)
-        so[(k / 4u) * ROW_THREADS + tid] = make_uint4(oacc[k], oacc[k + 1], oacc[k + 2], oacc[k + 3]);
-      meet();
-      // words of (thread's place, 4 dimensions): rank r takes every X-th
-      for (uint32_t i = rank * ROW_THREADS + tid; i < D / 4u * ROW_THREADS; i += X * ROW_THREADS) {
-        uint32_t v[4] = {0, 0, 0, 0};
-        for (uint32_t q = 0; q < X; q++) {
-          const uint32_t ad = cluster_addr(so + i, q);
-#pragma unroll
-          for (uint32_t x = 0; x < 4; x++) v[x] += cluster_ld32(ad + 4u * x);
+        for (uint32_t i = 1; i < PARTS; i++) total += s_ps[i][row];
+        if (X > 1) {
+          if (part == 0) s_s[row] = total;
+          meet();
+          total = 0;
+          for (uint32_t i = 0; i < X; i++) total += cluster_ld64(cluster_addr(&s_s[row], i));
         }
-        const uint32_t th = i % ROW_THREADS, orow = ((th >> 5) & 3u) * 32u + (th & 31u);
-        if (orow < nr) {
-          const uint32_t o_r = r0 + orow, dim = (th >> 7) * D + 4u * (i / ROW_THREADS);
-          int16_t* o = A.d.o + (uint64_t)(sq.lo + o_r / G) * A.d.ldo + (uint64_t)(g * G + o_r % G) * HD + dim;
-#pragma unroll
-          for (uint32_t x = 0; x < 4; x++) o[x] = (int16_t)out16(v[x]);
-        }
+        R = smx_r(total);
       }
-    } else if (row < nr) {
-      int16_t* o = A.d.o + (uint64_t)(sq.lo + tok) * A.d.ldo + (uint64_t)head * HD + part * D;
-      uint32_t ow[D / 2];
+      const uint32_t fp = (A.d.smx[2u * head + 1u] >> 8) & 31u;
+      pfast = __all_sync(0xffffffffu, fp >= 8u && fp <= 15u);
+      Rp = pfast ? R << (fp - 8u) : R;
+      more = s_go != 0u;
+      uint32_t oacc[D];
 #pragma unroll
-      for (uint32_t k = 0; k < D / 2; k++) ow[k] = pack16(out16(oacc[2 * k]), out16(oacc[2 * k + 1]));
-      if (!(((uintptr_t)A.d.o & 15u) | (A.d.ldo & 7u))) {
+      for (uint32_t k = 0; k < D; k++) oacc[k] = 0;
+      uint4 qn[D / 8];  // the q that the next scores take
+#pragma unroll 1
+      for (uint32_t a = t0; a < t1; a += WIN) {
+        const uint32_t e = min(a + WIN, t1);
+        if (again) {
+          load_shifts(a, e);
+#pragma unroll 1
+          for (uint32_t t = a; t < e; t++) score_pass(t, a, 2u);
+        }
+        if (!pfast)
+#pragma unroll 1
+          for (uint32_t t = a; t < e; t++) p_any(t, a, fp);
+        if (again) rows_sync();  // every warp has read the scores: P goes over their columns
+#pragma unroll 1
+        for (uint32_t t = a; t < e; t++) p_pass(t, a);
+        const bool last = e == t1;
+        if (last ? more : Sh::Q_OVER) fetch_q(s_item[last ? islot : cur], qn);  // (its latency under the wait)
+        // the window's P.V: this part's dimensions
+        if (ok) ok = wait_for(&o_full, ou & 1u, A.err, 319);
+        ou++;
+        __syncwarp();
+        sm100::tc_fence_after();
 #pragma unroll
-        for (uint32_t k = 0; k < D / 8; k++)
-          ((uint4*)o)[k] = make_uint4(ow[4 * k], ow[4 * k + 1], ow[4 * k + 2], ow[4 * k + 3]);
+        for (uint32_t k = 0; k < D; k += 16) {
+          uint32_t hh[16], mid[16], ll[16];
+          const uint32_t col = lane_base + part * D + k;
+          sm100::tmem_ld16(col, hh);
+          sm100::tmem_ld16(col + HD, mid);
+          sm100::tmem_ld16(col + 2 * HD, ll);
+          sm100::tmem_ld_wait();
+#pragma unroll
+          for (uint32_t x = 0; x < 16; x++) oacc[k + x] += hh[x] * A.k16 + (mid[x] * A.k8 + ll[x]);
+        }
+        if (last ? more : Sh::Q_OVER) store_q(qn);
+        release();
+      }
+      if (t0 == t1) {  // no key is seen: no P.V to wait for, the next q takes its place here
+        if (more) {
+          fetch_q(s_item[islot], qn);
+          store_q(qn);
+        }
+        release();
+      }
+      if (X > 1) {
+        // the cluster's sums: every CTA leaves its own in shared memory, and adds up a slice
+        rows_sync();
+        uint4* so = (uint4*)s_S;  // [D / 4][RT]
+#pragma unroll
+        for (uint32_t k = 0; k < D; k += 4)
+          so[(k / 4u) * RT + tid] = make_uint4(oacc[k], oacc[k + 1], oacc[k + 2], oacc[k + 3]);
+        meet();
+        // words of (thread's place, 4 dimensions): rank r takes every X-th
+        for (uint32_t i = rank * RT + tid; i < D / 4u * RT; i += X * RT) {
+          uint32_t v[4] = {0, 0, 0, 0};
+          for (uint32_t q = 0; q < X; q++) {
+            const uint32_t ad = cluster_addr(so + i, q);
+#pragma unroll
+            for (uint32_t x = 0; x < 4; x++) v[x] += cluster_ld32(ad + 4u * x);
+          }
+          const uint32_t th = i % RT, orow = ((th >> 5) & 3u) * 32u + (th & 31u);
+          if (orow < it.nr) {
+            const uint32_t o_r = it.r0 + orow, dim = (th >> 7) * D + 4u * (i / RT);
+            int16_t* o = A.d.o + (uint64_t)(it.lo_row + o_r / G) * A.d.ldo + (uint64_t)(it.g * G + o_r % G) * HD + dim;
+#pragma unroll
+            for (uint32_t x = 0; x < 4; x++) o[x] = (int16_t)out16(v[x]);
+          }
+        }
       } else {
+        // a row's D dimensions are W 16-byte words: W lanes trade them, so that each
+        // store writes whole rows' parts (W lanes a row) instead of a word of 32 rows
+        constexpr uint32_t W = D / 8;
+        uint4 ow[W];
 #pragma unroll
-        for (uint32_t k = 0; k < D / 2; k++) {
-          o[2 * k] = (int16_t)ow[k];
-          o[2 * k + 1] = (int16_t)(ow[k] >> 16);
+        for (uint32_t k = 0; k < W; k++) {
+          uint32_t x[4];
+#pragma unroll
+          for (uint32_t i = 0; i < 4; i++)
+            x[i] = pack_s16((uint32_t)((int32_t)oacc[8 * k + 2 * i] >> 8), (uint32_t)((int32_t)oacc[8 * k + 2 * i + 1] >> 8));
+          ow[k] = make_uint4(x[0], x[1], x[2], x[3]);
+        }
+        int16_t* const o = A.d.o + (uint64_t)(it.lo_row + rr / G) * A.d.ldo + (uint64_t)head * HD + part * D;
+        if (o16) {
+#pragma unroll
+          for (uint32_t st = W / 2; st > 0; st >>= 1) {  // after it, word k of lane l is word l % W of row l - l % W + k
+            const bool up = lane & st;
+#pragma unroll
+            for (uint32_t k = 0; k < W; k++) {
+              if (k & st) continue;
+              const uint4 give = up ? ow[k] : ow[k | st];
+              uint4 take;
+              take.x = __shfl_xor_sync(0xffffffffu, give.x, st);
+              take.y = __shfl_xor_sync(0xffffffffu, give.y, st);
+              take.z = __shfl_xor_sync(0xffffffffu, give.z, st);
+              take.w = __shfl_xor_sync(0xffffffffu, give.w, st);
+              if (up) ow[k] = take;
+              else ow[k | st] = take;
+            }
+          }
+          const uint32_t first = row - lane % W;
+#pragma unroll
+          for (uint32_t k = 0; k < W; k++) {
+            int16_t* const p = (int16_t*)__shfl_sync(0xffffffffu, (unsigned long long)o, (lane & ~(W - 1u)) + k);
+            if (first + k < it.nr) *(uint4*)(p + 8u * (lane % W)) = ow[k];
+          }
+        } else if (row < it.nr) {
+#pragma unroll
+          for (uint32_t k = 0; k < W; k++) {
+            const uint32_t x[4] = {ow[k].x, ow[k].y, ow[k].z, ow[k].w};
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+              o[8 * k + 2 * i] = (int16_t)x[i];
+              o[8 * k + 2 * i + 1] = (int16_t)(x[i] >> 16);
+            }
+          }
         }
       }
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&item_free[cur]);
     }
   }
   sm100::tc_fence_before();
   __syncthreads();
   if (X > 1) cluster_sync();  // no CTA leaves while another reads its shared memory
-  if (warp == 17) {
+  if (warp == RW + 1u) {
     sm100::tc_fence_after();
     sm100::tmem_dealloc<512>(tmem);
   }
@@ -739,26 +1002,30 @@ int launch(TileArgs A, uint32_t tiles, cudaStream_t st) {
   const uint32_t sub = c.page < BK ? c.page : BK;
   if (!make_row_map(&mk, c.kc, Sh::RB, lines, sub) || !make_row_map(&mv, c.vc, Sh::RB, lines, sub))
     return corm::fail(CORM_ECUDA, "corm_llm_paged_attn: cuTensorMapEncodeTiled failed");
+  A.tiles = tiles;
+  A.k8 = 1u << 8;
+  A.k16 = 1u << 16;
   const uint32_t cap = c.table_width * c.page, keys = A.d.max_keys < cap ? A.d.max_keys : cap;
   const uint32_t span = A.d.window && A.d.window < keys ? A.d.window + BMR : keys;
   const uint32_t ktiles = ((span < keys ? span : keys) + BK - 1u) / BK + 1u;
   const uint64_t blocks = (uint64_t)c.B * c.KV * tiles;
+  if (blocks > (1ull << 27)) return corm::fail(CORM_ELIMIT, "corm_llm_paged_attn: max_q %u over %u sequences", A.d.max_q, c.B);
+  // two stages of at most 32 KB (a tile's copies are short beside its integer work);
+  // the rest of the 227 KB, less 24 KB of static arrays, for scores
+  A.stages = Sh::STAGE > 16384u ? 2u : 32768u / Sh::STAGE;
+  const uint32_t tile_bytes = TILE_BYTES + (BITS == 8 ? 2u * BK : 0u);
+  const uint32_t most = (203u * 1024u - 1024u - A.stages * Sh::STAGE) / tile_bytes;
   uint32_t X = 1;
   while (X < 8u && blocks * 2u * X <= 148u && ktiles >= 4u * X) X *= 2u;
   A.X = X;
-  A.stages = 3u * 16384u / Sh::STAGE < 2u ? 2u : (3u * 16384u / Sh::STAGE > 6u ? 6u : 3u * 16384u / Sh::STAGE);
-  const uint32_t tile_bytes = BMR * BK * 2u + (BITS == 8 ? 2u * BK : 0u);
-  const uint32_t room = 206u * 1024u - 1024u - A.stages * Sh::STAGE;  // beside 20 KB of static arrays
-  const uint32_t most = room / tile_bytes, need = (ktiles + X - 1u) / X;
-  // a cluster's sums use the scores' memory: HD KB / 2
-  const uint32_t least = (HD * 512u + BMR * BK * 2u - 1u) / (BMR * BK * 2u);
-  A.win = need < least ? least : (need < most ? need : most);
+  const uint32_t need = (ktiles + X - 1u) / X;
+  A.win = need < 2u ? 2u : (need < most ? need : most);  // (a cluster's sums take up to two tiles' memory)
   const size_t smem = 1024u + A.stages * Sh::STAGE + (size_t)A.win * tile_bytes;
   auto kern = paged_attn_tile_kernel<HD, BITS>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return corm::cuda_status("llm_paged_attn");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles * X, c.KV, c.B);
+  cfg.gridDim = dim3((unsigned)blocks * X);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;

@@ -477,6 +477,40 @@ def test_attn_vs_oracle(case, hi):
 
 
 @gpu
+@pytest.mark.parametrize("HD,bits,window", [(64, 16, 0), (64, 8, 0), (128, 16, 0), (128, 8, 130), (64, 16, 1)])
+def test_attn_more_tiles_than_multiprocessors(HD, bits, window):
+    """Several tiles for every CTA, of unlike lengths, sequences without rows
+    between them, contexts in one and in more windows."""
+    rng = np.random.default_rng(HD + bits + window)
+    KV, page, B = 5, 32, 44
+    new = [int(rng.integers(1, 150)) if i % 5 else 0 for i in range(B)]
+    ctx = [int(rng.integers(0, 200)) for i in range(B)]
+    new[7], ctx[7], new[30], ctx[30] = 300, 0, 129, 800
+    pages = sum(-(-(a + n) // page) for a, n in zip(ctx, new)) + 2
+    table, cu, pos, rows = _batch(rng, pages, page, ctx, new, extra=2)
+    c = _random_cache(rng, pages, KV, page, HD, bits, 2500)
+    c.table, c.cu, c.pos = table, cu, pos
+    want = _run_attn(c, rows, KV, _smx(KV, HD, f_s=10), rng, window=window, hi=2500, max_q=max(new),
+                     max_keys=max(a + b for a, b in zip(ctx, new)))
+    assert (want[:rows - 2] != 0).mean() > 0.3
+
+
+@gpu
+@pytest.mark.parametrize("HD,bits,ctx,hint", [(64, 16, 9000, 9001), (64, 8, 15001, 9), (128, 8, 7000, 7001),
+                                              (256, 16, 3001, 1)])
+def test_attn_long_contexts_few_rows(HD, bits, ctx, hint):
+    """Many more tiles of keys than stages of copies, one row and a few."""
+    rng = np.random.default_rng(ctx)
+    page, new = 64, [1, 3]
+    ctxs = [ctx, ctx // 3]
+    pages = sum(-(-(a + n) // page) for a, n in zip(ctxs, new)) + 1
+    table, cu, pos, rows = _batch(rng, pages, page, ctxs, new)
+    c = _random_cache(rng, pages, 2, page, HD, bits, 2500)
+    c.table, c.cu, c.pos = table, cu, pos
+    _run_attn(c, rows, 6, _smx(6, HD, f_s=10), rng, hi=2500, max_q=3, max_keys=hint)
+
+
+@gpu
 @pytest.mark.parametrize("HD,bits,new", [(64, 16, 1), (64, 16, 70), (64, 8, 1), (128, 16, 33), (256, 16, 20)])
 def test_attn_softmax_registers(HD, bits, new):
     """Registers that differ by head: shifts below 8 and from 40 up, P at 0 to
