@@ -382,25 +382,28 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__
 }
 
 // ---------------------------------------------------------------- attention, few rows
-// A cluster of X CTAs per (sequence, KV head, 16 rows), a row being (token,
+// A cluster of X CTAs per (sequence, KV head, 8 rows), a row being (token,
 // head of the group), token-major; the CTAs share the keys.  The unit's e(d) is
 // a table of d = m - score, so sums cannot be rescaled as a running maximum
-// moves; instead the scores stay on the chip: every CTA forms those of its keys
+// moves; instead the scores stay on the chip: those of a CTA's keys are formed
 // once (int16 in shared memory), the maxima meet over the cluster, then e in
 // place and the sums meet, then P in place and P.V over the V rows, whose
 // partial sums (modulo 2^32, so in any order) meet last.  K and V are read once.
 // Keys beyond the shared memory: windows, the scores formed again in each of
 // the three passes.
 //
-// A ninth warp copies the pages (64 keys a stage, one bulk copy per page piece)
-// into a ring, running ahead across the phases, so the V rows arrive under the
-// softmax.  Warp-level MMAs: the 16-row tile is far below the 128 rows of a
-// tcgen05 tile, and the copies bound the kernel.  The contraction over HD takes
-// the dimensions in the order in which a lane's 16-byte pieces hold them (the q
-// fragments alike); V's bytes are transposed 4 x 4 in registers.
-constexpr uint32_t kT = 64;       // keys of a stage
-constexpr uint32_t kRows = 16;    // rows of a tile
-constexpr uint32_t kWarps = 8;    // computing warps
+// The eight warps work apart: a warp has every eighth block of keys (32 or 64),
+// copies them itself into stages of its own (one bulk copy per page piece, the
+// next under way while it computes; the V rows arrive under the softmax), and
+// nothing but the maxima, the sums and the output meets.  Warp-level MMAs with the
+// keys, then the output's dimensions, as the 16 rows of an MMA and the query rows as
+// its 8 columns: a decoded token's group of heads is far below the 128 rows of a
+// tcgen05 tile, and the copies are to bound the kernel.  The contraction over HD
+// takes the dimensions in the order in which a lane's 16-byte pieces hold them (q
+// alike), the one over the keys in the order in which the scores' words hold them
+// (word i of 16 keys: keys i and i + 8); V's bytes are transposed 4 x 4 in registers.
+constexpr uint32_t kRows = 8;     // rows of a tile
+constexpr uint32_t kWarps = 8;
 constexpr uint32_t kMaxCluster = 8;
 constexpr uint32_t kSplitRows = 32;  // rows of a sequence and KV head up to which this form runs
 
@@ -408,48 +411,45 @@ struct SplitArgs {
   corm_llm_paged_attn_desc d;
   const int32_t* tab;
   int* err;
-  uint32_t G, X, stages, win, rcap;  // win: tiles of a window; rcap: rows held
+  uint32_t G, X, stages, win, rcap;  // stages of a warp; win: blocks of a warp's window; rcap: rows held
 };
 
 template <int HD, int BITS>
 struct SplitShape {
-  static constexpr uint32_t RB = HD * (BITS / 8);                     // bytes of a cached row
-  static constexpr uint32_t STB = kT * RB + (BITS == 8 ? 128u : 0u);  // a stage (its shifts last)
-  static constexpr uint32_t NKS = HD < 32 ? 1 : HD / 32;              // MMA steps of a score
-  static constexpr uint32_t DW = HD < 32 ? HD : 32;                   // output dimensions of a warp
-  static constexpr uint32_t DG = HD / DW, KG = kWarps / DG;           // dimension and key groups of warps
-  static constexpr uint32_t NT = DW / 8;
+  static constexpr uint32_t RB = HD * (BITS / 8);             // bytes of a cached row
+  static constexpr uint32_t KS = RB <= 64 ? 64 : 32;          // keys of a block (a stage)
+  static constexpr uint32_t STB = KS * RB + (BITS == 8 ? 128u : 0u);  // a stage (its shifts last)
+  static constexpr uint32_t NKS = HD < 32 ? 1 : HD / 32;      // MMA steps of a score
+  static constexpr uint32_t CH = HD < 32 ? 1 : HD / 32;       // chunks of 32 (HD 16: 16) dimensions
+  static constexpr uint32_t MT = HD / 16;                     // 16-dimension tiles of the output
+  static constexpr uint32_t PW = KS / 2;                      // words of a row's scores in a block
+  static constexpr uint32_t PITCH = PW + 8;                   // a row's words: 8 mod 16, so four rows' reads meet no bank twice
+  static constexpr uint32_t OCC = HD <= 64 ? 3 : (HD == 128 ? 2 : 1);  // CTAs an SM that the registers allow
 };
-__host__ __device__ constexpr uint32_t split_pitch(uint32_t win) { return win * kT + 16u; }  // int16 of a score row
-
-__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 template <int HD, int BITS>
-__global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kernel(const __grid_constant__ SplitArgs A) {
+__global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_split_kernel(const __grid_constant__ SplitArgs A) {
   using Sh = SplitShape<HD, BITS>;
-  constexpr uint32_t RB = Sh::RB, STB = Sh::STB, NKS = Sh::NKS, DW = Sh::DW, DG = Sh::DG, KG = Sh::KG, NT = Sh::NT;
+  constexpr uint32_t RB = Sh::RB, KS = Sh::KS, STB = Sh::STB, NKS = Sh::NKS, PW = Sh::PW, PITCH = Sh::PITCH;
   extern __shared__ __align__(128) uint8_t pa_sm[];
-  __shared__ uint64_t full[8], empty[8], cbar;
+  __shared__ uint64_t full[kWarps][4], cbar;
   __shared__ int32_t s_wmax[kWarps][kRows], s_m[kRows], s_gm[kRows];
-  __shared__ unsigned long long s_s[kRows];
+  __shared__ unsigned long long s_ws[kWarps][kRows], s_s[kRows];
   __shared__ uint32_t s_R[kRows], s_lo[kRows], s_hi[kRows], s_cm[kRows], s_cs[kRows], s_fp[kRows];
   const corm_paged_cache& c = A.d.c;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint32_t X = A.X, tile = blockIdx.x / X, rank = blockIdx.x % X, g = blockIdx.y, b = blockIdx.z, G = A.G;
-  const uint32_t NST = A.stages;
-  uint8_t* ring = pa_sm;
-  int16_t* S = (int16_t*)(ring + NST * STB);
-  const uint32_t pitch = split_pitch(A.win);
-  uint32_t* s_O = (uint32_t*)(S + A.rcap * pitch);
-  uint16_t* tab = (uint16_t*)(s_O + A.rcap * HD);
-  if (tid == 0) {
-    for (uint32_t i = 0; i < NST; i++) {
-      sm100::mbar_init(&full[i], 1);
-      sm100::mbar_init(&empty[i], kWarps);
-    }
-    sm100::mbar_init(&cbar, X);
-    sm100::fence_mbar_init();
-  }
+  const uint32_t NST = A.stages, rcap = A.rcap, WIN = A.win;
+  uint8_t* const ring = pa_sm + warp * NST * STB;                                          // this warp's stages
+  uint32_t* const S = (uint32_t*)(pa_sm + kWarps * NST * STB) + warp * WIN * rcap * PITCH;  // and scores: [block][row][PITCH]
+  uint16_t* const tab = (uint16_t*)(pa_sm + kWarps * (NST * STB + WIN * rcap * PITCH * 4u));
+  uint32_t* const s_O = (uint32_t*)(tab + 4096);
+  uint64_t* const bars = full[warp];
+  if (lane == 0)
+    for (uint32_t i = 0; i < NST; i++) sm100::mbar_init(&bars[i], 1);
+  if (tid == 0) sm100::mbar_init(&cbar, X);
+  sm100::fence_mbar_init();
+  __syncwarp();
   corm_pdl_wait();
   corm_pdl_trigger();
   const SeqRows sq = seq_rows(c, b, c.rows);
@@ -457,73 +457,63 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
   if ((uint64_t)r0 >= (uint64_t)n * G) return;  // the cluster's CTAs alike
   const uint32_t nr = min(kRows, n * G - r0);
   const uint32_t i0 = r0 / G, i1 = (r0 + nr - 1u) / G;
-  // the keys some row of the tile sees: [lo, hi), in tiles from lo rounded down
+  // the keys some row of the tile sees: [lo, hi), in blocks from lo rounded down
   const uint32_t hi = min(sq.pos + i1 + 1u, sq.cap);
   const uint32_t w = A.d.window;
   const uint32_t lo = (w && sq.pos + i0 + 1u > w) ? sq.pos + i0 + 1u - w : 0u;
-  const uint32_t tile0 = lo / kT, ntile = hi > lo ? (hi + kT - 1u) / kT - tile0 : 0u;
+  const uint32_t tile0 = lo / KS, ntile = hi > lo ? (hi + KS - 1u) / KS - tile0 : 0u;
   const uint32_t per = (ntile + X - 1u) / X;
-  const uint32_t t0 = tile0 + min(rank * per, ntile), t1 = tile0 + min(rank * per + per, ntile);
-  const uint32_t nwin = (t1 - t0 + A.win - 1u) / A.win;
-  if (X > 1) cluster_sync();
-  else __syncthreads();
+  const uint32_t first = tile0 + min(rank * per, ntile) + warp, end = tile0 + min(rank * per + per, ntile);
+  const uint32_t own = first < end ? (end - first + kWarps - 1u) / kWarps : 0u;  // blocks first, first + 8, ...
+  const bool again = own > WIN;  // more than a window (a warp's own affair)
 
-  if (warp == kWarps) {
-    // ---------------- the copies
-    const uint32_t sub = min(c.page, kT), pieces = kT / sub;
-    const int32_t* tb = c.table + (uint64_t)b * c.table_width;
-    const uint32_t psh = 31u - __clz(c.page);
-    uint32_t gi = 0, base = 0xFFFFFF00u;
-    int32_t ids = -1;
-    bool ok = true;
-    auto emit = [&](bool is_v, uint32_t t) {
-      const uint32_t s = gi % NST;
-      if (gi >= NST && ok) ok = wait_for(&empty[s], ((gi / NST) - 1u) & 1u, A.err, 301);
-      ok = __all_sync(0xffffffffu, ok);
-      gi++;
-      if (!ok) return;
-      const uint32_t b0 = (t * kT) >> psh, b1 = (t * kT + kT - 1u) >> psh;
-      if (b0 < base || b1 >= base + 32u) {  // 32 table entries at a time
-        base = b0;
-        ids = base + lane < c.table_width ? tb[base + lane] : -1;
-      }
-      const uint32_t key = t * kT + lane * sub;
-      const bool in = lane < pieces && key < hi;
-      const int32_t id = __shfl_sync(0xffffffffu, ids, in ? (key >> psh) - base : 0u);
-      const bool good = in && (uint32_t)id < c.pages;
-      uint8_t* dst = ring + s * STB + lane * sub * RB;
-      if (in && !good) {  // a page of zeros
-        for (uint32_t i = 0; i < sub * RB; i += 16u) *(int4*)(dst + i) = make_int4(0, 0, 0, 0);
-        if (BITS == 8)
-          for (uint32_t i = 0; i < sub; i += 16u) *(int4*)(ring + s * STB + kT * RB + lane * sub + i) = make_int4(0, 0, 0, 0);
-        sm100::fence_proxy_async_smem();
-      }
-      const uint32_t cnt = __popc(__ballot_sync(0xffffffffu, good));
-      if (lane == 0) sm100::mbar_expect_tx(&full[s], cnt * sub * (RB + (BITS == 8 ? 1u : 0u)));
-      __syncwarp();
-      if (good) {
-        const uint64_t line = ((uint64_t)(uint32_t)id * c.KV + g) * c.page + (key & (c.page - 1u));
-        bulk_g2s(dst, (is_v ? c.vc : c.kc) + line * RB, sub * RB, &full[s]);
-        if (BITS == 8) bulk_g2s(ring + s * STB + kT * RB + lane * sub, (is_v ? c.vs : c.ks) + line, sub, &full[s]);
-      }
-    };
-    // K (v = 0) for the first pass and, in windows, again for the other two; V (v = 1)
-    // behind each window's K of the last
-#pragma unroll 1
-    for (uint32_t pass = 0; pass < 3; pass++)
-#pragma unroll 1
-      for (uint32_t a = t0; a < t1; a += A.win)
-#pragma unroll 1
-        for (uint32_t v = (pass == 0 || nwin > 1) ? 0u : 1u; v < (pass == 2 ? 2u : 1u); v++)
-#pragma unroll 1
-          for (uint32_t t = a; t < min(a + A.win, t1); t++) emit(v == 1u, t);
-    // every copy lands before the CTA's shared memory goes away
-    for (uint32_t q = gi > NST ? gi - NST : 0u; ok && q < gi; q++)
-      wait_for(&full[q % NST], (q / NST) & 1u, nullptr, 0);
+  // ---------------- the copies: K's blocks, then V's; in windows K's blocks for each of
+  // the first two passes, then each window's K and V
+  const uint32_t sub = min(c.page, KS), pieces = KS / sub, psh = 31u - __clz(c.page);
+  const int32_t* const tb = c.table + (uint64_t)b * c.table_width;
+  const uint32_t total = again ? 4u * own : 2u * own;
+  uint32_t eq = 0, ej = 0, ea = 0, ep = 0;  // the next copy's number, block, window and pass
+  bool ev = false;                          // of V
+  auto page_of = [&]() -> int32_t {         // the page of this lane's piece of the next copy
+    const uint32_t key = (first + ej * kWarps) * KS + lane * sub;
+    return eq < total && lane < pieces && key < hi ? tb[key >> psh] : -1;
+  };
+  int32_t id = page_of();
+  uint32_t es = 0;
+  auto emit = [&]() {
+    const uint32_t key = (first + ej * kWarps) * KS + lane * sub;
+    const bool in = lane < pieces && key < hi, good = in && (uint32_t)id < c.pages;
+    uint8_t* const st = ring + es * STB;
+    if (in && !good) {  // a page of zeros
+      uint8_t* const dst = st + lane * sub * RB;
+      for (uint32_t i = 0; i < sub * RB; i += 16u) *(int4*)(dst + i) = make_int4(0, 0, 0, 0);
+      if (BITS == 8)
+        for (uint32_t i = 0; i < sub; i += 16u) *(int4*)(st + KS * RB + lane * sub + i) = make_int4(0, 0, 0, 0);
+      sm100::fence_proxy_async_smem();
+    }
+    const uint32_t cnt = __popc(__ballot_sync(0xffffffffu, good));
+    if (lane == 0) sm100::mbar_expect_tx(&bars[es], cnt * sub * (RB + (BITS == 8 ? 1u : 0u)));
     __syncwarp();
-    if (X > 1) cluster_sync();
-    return;
-  }
+    if (good) {
+      const uint64_t line = ((uint64_t)(uint32_t)id * c.KV + g) * c.page + (key & (c.page - 1u));
+      bulk_g2s(st + lane * sub * RB, (ev ? c.vc : c.kc) + line * RB, sub * RB, &bars[es]);
+      if (BITS == 8) bulk_g2s(st + KS * RB + lane * sub, (ev ? c.vs : c.ks) + line, sub, &bars[es]);
+    }
+    if (++es == NST) es = 0;
+    eq++;
+    ej++;
+    if (!again) {
+      if (ej == own) ej = 0, ev = true;
+    } else if (ep < 2u) {
+      if (ej == own) ej = 0, ep++;
+    } else if (ej == min(ea + WIN, own)) {
+      if (ev) ea += WIN;
+      ev = !ev;
+      ej = ea;
+    }
+    id = page_of();
+  };
+  for (uint32_t i = 0; i < min(NST, total); i++) emit();
 
   // ---------------- the rows
   if (tid < kRows) {
@@ -535,113 +525,121 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
     const uint32_t cfg = A.d.smx[2u * h + 1u];
     s_cs[tid] = cfg & 63u;
     s_fp[tid] = (cfg >> 8) & 31u;
-    s_s[tid] = 0;
   }
-  for (uint32_t i = tid; i < 4096u; i += 256u) tab[i] = (uint16_t)(A.tab[i] - 1);
-  for (uint32_t i = tid; i < nr * HD; i += 256u) s_O[i] = 0;
-  const uint32_t qn = lane >> 2, qt = lane & 3u;  // a fragment's row (and row + 8; a key; a column) and quarter
-  uint32_t ah[NKS][4], al[NKS][4];
+  if (tid < kWarps * kRows) ((unsigned long long*)s_ws)[tid] = 0;
+  const uint32_t qn = lane >> 2, qt = lane & 3u;
+  uint32_t bh[NKS][2], bl[NKS][2];  // q's planes: row qn
 #pragma unroll
   for (uint32_t ks = 0; ks < NKS; ks++)
 #pragma unroll
-    for (uint32_t x = 0; x < 4; x++) {
-      const uint32_t row = qn + 8u * (x & 1u), half = x >> 1;  // a0: row, a1: row + 8, a2 / a3: the second half
+    for (uint32_t half = 0; half < 2; half++) {
       // word v of the lane's pieces: dimensions 64 (v / 4) + 16 t + 4 (v % 4) (rows of 64 up)
       const uint32_t v = 2u * ks + half;
       const uint32_t dim = HD >= 64 ? 64u * (v >> 2) + 16u * qt + 4u * (v & 3u) : (HD == 32 ? 8u * qt + 4u * half : 4u * qt);
-      ah[ks][x] = al[ks][x] = 0;
-      if (row < nr && (HD > 16 || half == 0)) {
-        const uint32_t rr = r0 + row;
+      bh[ks][half] = bl[ks][half] = 0;
+      if (qn < nr && (HD > 16 || half == 0)) {
+        const uint32_t rr = r0 + qn;
         const int16_t* q = A.d.q + (uint64_t)(sq.lo + rr / G) * A.d.ldq + (uint64_t)(g * G + rr % G) * HD + dim;
         const uint32_t x0 = pack16(q[0], q[1]), x1 = pack16(q[2], q[3]);
-        ah[ks][x] = __byte_perm(x0, x1, 0x7531);
-        al[ks][x] = __byte_perm(x0, x1, 0x6420);
+        bh[ks][half] = __byte_perm(x0, x1, 0x7531);
+        bl[ks][half] = __byte_perm(x0, x1, 0x6420);
       }
     }
-  consumer_sync();
-  const uint32_t lo0 = s_lo[qn], hi0 = qn < nr ? s_hi[qn] : 0u, lo1 = s_lo[qn + 8u], hi1 = qn + 8u < nr ? s_hi[qn + 8u] : 0u;
-  uint32_t gi = 0;
+  for (uint32_t i = tid; i < 1024u; i += 256u) {
+    const int4 v = ((const int4*)A.tab)[i];
+    ((uint2*)tab)[i] = make_uint2(pack16(v.x - 1, v.y - 1), pack16(v.z - 1, v.w - 1));
+  }
+  if (X > 1) cluster_sync();
+  else __syncthreads();
+
+  const uint32_t lo_last = s_lo[nr - 1u], hi_first = s_hi[0];  // every row sees [lo_last, hi_first)
+  const uint32_t ra = 2u * qt, rb = ra + 1u;                   // the rows of this lane's columns
+  uint32_t cs_ = 0, cp_ = 0;                                   // the next stage and its parity
   bool ok = true;
-  // the scores of tile t into the window's rows; the running maxima of the keys each row sees
-  int32_t mx0 = INT32_MIN, mx1 = INT32_MIN;
-  auto scores = [&](uint32_t t, uint32_t a) {
-    const uint32_t s = gi % NST;
-    if (ok) ok = wait_for(&full[s], (gi / NST) & 1u, A.err, 302);
+  auto stage_in = [&](int code) {
+    if (ok) ok = wait_for(&bars[cs_], cp_, A.err, code);
     __syncwarp();
-    gi++;
-    const uint8_t* row = ring + s * STB + (8u * warp + qn) * RB;
-    uint32_t hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
-    if (HD >= 64) {
+    return ring + cs_ * STB;
+  };
+  auto stage_out = [&]() {
+    __syncwarp();
+    if (++cs_ == NST) cs_ = 0, cp_ ^= 1u;
+    if (eq < total) emit();
+  };
+  // the scores of block t into the window's slot; the running maxima of the keys the rows ra and rb see
+  uint32_t mxa = 0x80008000u, mxb = 0x80008000u;
+  auto scores = [&](uint32_t t, uint32_t slot) {
+    const uint8_t* const st = stage_in(302);
+    uint32_t* const d = S + slot * rcap * PITCH;
+    const bool whole = t * KS >= lo_last && (t + 1u) * KS <= hi_first;
 #pragma unroll
-      for (uint32_t k = 0; k < (HD >= 64 ? HD / 64 : 1); k++) {
-        const uint8_t* p = row + 64u * k + 16u * qt;
-        uint4 h, l = make_uint4(0, 0, 0, 0);
-        if (BITS == 16) {  // odd keys take the planes in the other order: no bank is asked twice
-          const uint4 u = *(const uint4*)(p + ((qn & 1u) ? HD : 0)), v = *(const uint4*)(p + ((qn & 1u) ? 0 : HD));
-          h = (qn & 1u) ? v : u;
-          l = (qn & 1u) ? u : v;
-        } else {
-          h = *(const uint4*)p;
-        }
-        const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-        for (uint32_t j = 0; j < 2; j++) {
-          const uint32_t ks = NKS > 1 ? 2u * k + j : 0u;
-          mma_ss(hh, ah[ks], hw[2 * j], hw[2 * j + 1]);
-          mma_us(mid, al[ks], hw[2 * j], hw[2 * j + 1]);
-          if (BITS == 16) {
-            mma_su(mid, ah[ks], lw[2 * j], lw[2 * j + 1]);
-            mma_uu(ll, al[ks], lw[2 * j], lw[2 * j + 1]);
-          }
-        }
-      }
-    } else {
-      uint32_t h0, h1 = 0, l0 = 0, l1 = 0;
-      if (HD == 32) {
-        const uint2 u = *(const uint2*)(row + 8u * qt);
-        h0 = u.x, h1 = u.y;
+    for (uint32_t k16 = 0; k16 < KS / 16; k16++) {
+      const uint8_t* const row = st + (16u * k16 + qn) * RB;
+      uint32_t hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
+      auto step = [&](uint32_t ks, const uint32_t (&h)[4], const uint32_t (&l)[4]) {
+        mma_ss(hh, h, bh[ks][0], bh[ks][1]);
+        mma_su(mid, h, bl[ks][0], bl[ks][1]);
         if (BITS == 16) {
-          const uint2 v = *(const uint2*)(row + HD + 8u * qt);
-          l0 = v.x, l1 = v.y;
+          mma_us(mid, l, bh[ks][0], bh[ks][1]);
+          mma_uu(ll, l, bl[ks][0], bl[ks][1]);
+        }
+      };
+      if constexpr (HD >= 64) {
+#pragma unroll
+        for (uint32_t k = 0; k < HD / 64; k++) {
+          const uint8_t* const p = row + 64u * k + 16u * qt;
+          const uint4 h0 = *(const uint4*)p, h1 = *(const uint4*)(p + 8u * RB);
+          uint4 l0 = make_uint4(0, 0, 0, 0), l1 = l0;
+          if (BITS == 16) l0 = *(const uint4*)(p + HD), l1 = *(const uint4*)(p + 8u * RB + HD);
+          const uint32_t fh[2][4] = {{h0.x, h1.x, h0.y, h1.y}, {h0.z, h1.z, h0.w, h1.w}};
+          const uint32_t fl[2][4] = {{l0.x, l1.x, l0.y, l1.y}, {l0.z, l1.z, l0.w, l1.w}};
+          step(2u * k, fh[0], fl[0]);
+          step(2u * k + 1u, fh[1], fl[1]);
         }
       } else {
-        h0 = *(const uint32_t*)(row + 4u * qt);
-        if (BITS == 16) l0 = *(const uint32_t*)(row + HD + 4u * qt);
+        uint32_t h[4] = {0, 0, 0, 0}, l[4] = {0, 0, 0, 0};
+        if constexpr (HD == 32) {
+          const uint2 a0 = *(const uint2*)(row + 8u * qt), a1 = *(const uint2*)(row + 8u * RB + 8u * qt);
+          h[0] = a0.x, h[1] = a1.x, h[2] = a0.y, h[3] = a1.y;
+          if (BITS == 16) {
+            const uint2 c0 = *(const uint2*)(row + HD + 8u * qt), c1 = *(const uint2*)(row + 8u * RB + HD + 8u * qt);
+            l[0] = c0.x, l[1] = c1.x, l[2] = c0.y, l[3] = c1.y;
+          }
+        } else {
+          h[0] = *(const uint32_t*)(row + 4u * qt), h[1] = *(const uint32_t*)(row + 8u * RB + 4u * qt);
+          if (BITS == 16) l[0] = *(const uint32_t*)(row + HD + 4u * qt), l[1] = *(const uint32_t*)(row + 8u * RB + HD + 4u * qt);
+        }
+        step(0, h, l);
       }
-      mma_ss(hh, ah[0], h0, h1);
-      mma_us(mid, al[0], h0, h1);
+      // columns ra and rb of keys qn (sums 0, 1) and qn + 8 (2, 3)
+      uint32_t y[4];
       if (BITS == 16) {
-        mma_su(mid, ah[0], l0, l1);
-        mma_uu(ll, al[0], l0, l1);
-      }
-    }
-    uint32_t s0 = 0, s1 = 0;
-    if (BITS == 8) {
-      const uint32_t sh = *(const uint16_t*)(ring + s * STB + kT * RB + 8u * warp + 2u * qt);
-      s0 = sh & 31u;
-      s1 = (sh >> 8) & 31u;
-    }
-    __syncwarp();
-    if (lane == 0) sm100::mbar_arrive(&empty[s]);
-    int32_t v[4];
 #pragma unroll
-    for (int x = 0; x < 4; x++) {
-      uint32_t acc = BITS == 16 ? (hh[x] << 16) + (mid[x] << 8) + ll[x] : ((hh[x] << 8) + mid[x]) << ((x & 1) ? s1 : s0);
-      v[x] = out16(acc);
+        for (int x = 0; x < 4; x++) y[x] = (uint32_t)((int32_t)((hh[x] << 16) + (mid[x] << 8) + ll[x]) >> 8);
+      } else {
+        const uint8_t* const sp = st + KS * RB + 16u * k16 + qn;
+        const uint32_t s0 = sp[0] & 31u, s1 = sp[8] & 31u;
+#pragma unroll
+        for (int x = 0; x < 4; x++) y[x] = (uint32_t)((int32_t)(((hh[x] << 8) + mid[x]) << (x < 2 ? s0 : s1)) >> 8);
+      }
+      uint32_t wa = pack_s16(y[0], y[2]), wb = pack_s16(y[1], y[3]);
+      if (ra < nr) d[ra * PITCH + 8u * k16 + qn] = wa;
+      if (rb < nr) d[rb * PITCH + 8u * k16 + qn] = wb;
+      if (!whole) {
+        const uint32_t k0 = t * KS + 16u * k16 + qn, k1 = k0 + 8u;
+        const uint32_t la = s_lo[ra], ha = s_hi[ra], lb = s_lo[rb], hb = s_hi[rb];
+        wa = __byte_perm(k0 >= la && k0 < ha ? wa : 0x8000u, k1 >= la && k1 < ha ? wa : 0x80000000u, 0x7610);
+        wb = __byte_perm(k0 >= lb && k0 < hb ? wb : 0x8000u, k1 >= lb && k1 < hb ? wb : 0x80000000u, 0x7610);
+      }
+      mxa = __vmaxs2(mxa, wa);
+      mxb = __vmaxs2(mxb, wb);
     }
-    const uint32_t key = t * kT + 8u * warp + 2u * qt;
-    if (key >= lo0 && key < hi0) mx0 = max(mx0, v[0]);
-    if (key + 1u >= lo0 && key + 1u < hi0) mx0 = max(mx0, v[1]);
-    if (key >= lo1 && key < hi1) mx1 = max(mx1, v[2]);
-    if (key + 1u >= lo1 && key + 1u < hi1) mx1 = max(mx1, v[3]);
-    int16_t* d = S + (t - a) * kT + 8u * warp + 2u * qt;
-    if (qn < nr) *(uint32_t*)(d + qn * pitch) = pack16(v[0], v[1]);
-    if (qn + 8u < nr) *(uint32_t*)(d + (qn + 8u) * pitch) = pack16(v[2], v[3]);
+    stage_out();
   };
   uint32_t cphase = 0;
   // every CTA of the cluster is here, and what it wrote before is visible
   auto cluster_meet = [&]() {
-    consumer_sync();
+    __syncthreads();
     if (X > 1) {
       if (tid < X) mbar_arrive_remote(&cbar, tid);
       if (ok) ok = mbar_wait_cluster(&cbar, cphase, A.err, 303);
@@ -650,136 +648,181 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
   };
 
   // pass 1: the maxima
-  for (uint32_t a = t0; a < t1; a += A.win)
-    for (uint32_t t = a; t < min(a + A.win, t1); t++) scores(t, a);
+#pragma unroll 1
+  for (uint32_t j = 0; j < own; j++) scores(first + j * kWarps, again ? 0u : j);
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    mx0 = max(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
-    mx1 = max(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
+  for (int o = 4; o < 32; o <<= 1) {
+    mxa = __vmaxs2(mxa, __shfl_xor_sync(0xffffffffu, mxa, o));
+    mxb = __vmaxs2(mxb, __shfl_xor_sync(0xffffffffu, mxb, o));
   }
-  if (qt == 0) {
-    s_wmax[warp][qn] = mx0;
-    s_wmax[warp][qn + 8u] = mx1;
+  if (qn == 0) {
+    s_wmax[warp][ra] = max((int32_t)(int16_t)(mxa & 0xFFFFu), (int32_t)mxa >> 16);
+    s_wmax[warp][rb] = max((int32_t)(int16_t)(mxb & 0xFFFFu), (int32_t)mxb >> 16);
   }
-  consumer_sync();
+  __syncthreads();
   if (tid < kRows) {
     int32_t m = s_wmax[0][tid];
     for (uint32_t i = 1; i < kWarps; i++) m = max(m, s_wmax[i][tid]);
     s_m[tid] = m;
   }
-  cluster_meet();
+  if (X > 1) cluster_meet();
   if (tid < kRows) {
     int32_t m = s_m[tid];
     if (X > 1)
       for (uint32_t i = 0; i < X; i++) m = max(m, (int32_t)cluster_ld32(cluster_addr(&s_m[tid], i)));
     s_gm[tid] = m;
   }
-  consumer_sync();
+  __syncthreads();
 
-  // rows over the warps: one each from eight rows on, else wpr warps a row
-  const uint32_t wpr = nr > 4u ? 1u : (nr > 2u ? 2u : (nr > 1u ? 4u : 8u)), wgr = kWarps / wpr;
-  const uint32_t rw = warp / wpr, rl = (warp % wpr) * 32u + lane, rstep = 32u * wpr;
-  // pass 2: e of the window [a, e) in place (or only its sum), the sum of the row r
-  auto e_pass = [&](uint32_t a, uint32_t e, bool keep) {
-    for (uint32_t r = rw; r < nr; r += wgr) {
-      uint32_t* row = (uint32_t*)(S + r * pitch);
-      const uint32_t cm = s_cm[r], cs = s_cs[r], klo = s_lo[r], khi = s_hi[r];
-      const int32_t m = s_gm[r];
-      const SmxScale sc = smx_scale(cm, max(cs, 8u));
+  // a word (two keys) a lane, PW lanes a row, the rows in turn
+  const uint32_t rl = lane % PW, rh = lane / PW;
+  constexpr uint32_t RSTEP = 32 / PW;
+  const uint32_t word_key = 16u * (rl >> 3) + (rl & 7u);  // the word's first key in its block; the second is 8 on
+  // e of a word's two scores, 0 where the row does not see the key
+  struct Row {
+    uint32_t cm, cs, klo, khi;
+    int32_t m;
+    SmxScale sc;
+  };
+  auto row_of = [&](uint32_t r) {
+    Row o;
+    o.cm = s_cm[r], o.cs = s_cs[r], o.klo = s_lo[r], o.khi = s_hi[r];
+    o.m = s_gm[r];
+    o.sc = smx_scale(o.cm, max(o.cs, 8u));
+    return o;
+  };
+  auto e_of = [&](const Row& o, uint32_t x, uint32_t t, uint32_t& e0, uint32_t& e1) {
+    const uint32_t d0 = (uint32_t)(o.m - (int32_t)(int16_t)x) & 0xFFFFu, d1 = (uint32_t)(o.m - ((int32_t)x >> 16)) & 0xFFFFu;
+    const uint32_t k0 = t * KS + word_key, k1 = k0 + 8u;
+    if (o.cs >= 8u) {
+      e0 = smx_e(d0, o.sc, tab);
+      e1 = smx_e(d1, o.sc, tab);
+    } else {
+      e0 = smx_e_wide(d0, o.cm, o.cs, tab);
+      e1 = smx_e_wide(d1, o.cm, o.cs, tab);
+    }
+    if (k0 < o.klo || k0 >= o.khi) e0 = 0;
+    if (k1 < o.klo || k1 >= o.khi) e1 = 0;
+  };
+  // pass 2: e of blocks [a, z) in place (or only the sums)
+  auto e_pass = [&](uint32_t a, uint32_t z, bool keep) {
+#pragma unroll 1
+    for (uint32_t r0_ = 0; r0_ < nr; r0_ += RSTEP) {
+      const uint32_t r = r0_ + rh;
       unsigned long long sum = 0;
-      for (uint32_t i = rl; i < (e - a) * (kT / 2u); i += rstep) {
-        const uint32_t x = row[i], key = a * kT + 2u * i;
-        uint32_t e0 = 0, e1 = 0;
-        const uint32_t d0 = (uint32_t)(m - (int32_t)(int16_t)x), d1 = (uint32_t)(m - ((int32_t)x >> 16));
-        if (key >= klo && key < khi) e0 = cs >= 8u ? smx_e(d0, sc, tab) : smx_e_wide(d0, cm, cs, tab);
-        if (key + 1u >= klo && key + 1u < khi) e1 = cs >= 8u ? smx_e(d1, sc, tab) : smx_e_wide(d1, cm, cs, tab);
-        sum += e0 + e1;
-        if (keep) row[i] = e_pack(e0) | (e_pack(e1) << 16);
+      if (r < nr) {
+        const Row o = row_of(r);
+        uint32_t* p = S + r * PITCH + rl;
+#pragma unroll 2
+        for (uint32_t j = a; j < z; j++, p += rcap * PITCH) {
+          uint32_t e0, e1;
+          e_of(o, *p, first + j * kWarps, e0, e1);
+          sum += e0 + e1;
+          if (keep) *p = e_pack(e0) | (e_pack(e1) << 16);
+        }
       }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0 && sum) atomicAdd(&s_s[r], sum);
+      for (int o = PW / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (rl == 0 && r < nr) s_ws[warp][r] += sum;
     }
   };
-  // pass 3: P of the window in place, from e (one window) or from the scores
-  auto p_pass = [&](uint32_t a, uint32_t e, bool from_e) {
-    for (uint32_t r = rw; r < nr; r += wgr) {
-      uint32_t* row = (uint32_t*)(S + r * pitch);
-      const uint32_t cm = s_cm[r], cs = s_cs[r], fp = s_fp[r], R = s_R[r], klo = s_lo[r], khi = s_hi[r];
-      const int32_t m = s_gm[r];
-      const SmxScale sc = smx_scale(cm, max(cs, 8u));
-      for (uint32_t i = rl; i < (e - a) * (kT / 2u); i += rstep) {
-        const uint32_t x = row[i], key = a * kT + 2u * i;
-        const bool v0 = key >= klo && key < khi, v1 = key + 1u >= klo && key + 1u < khi;
-        uint32_t e0 = e_unpack(x & 0xFFFFu), e1 = e_unpack(x >> 16);
-        if (!from_e) {
-          const uint32_t d0 = (uint32_t)(m - (int32_t)(int16_t)x), d1 = (uint32_t)(m - ((int32_t)x >> 16));
-          e0 = cs >= 8u ? smx_e(d0 & 0xFFFFu, sc, tab) : smx_e_wide(d0 & 0xFFFFu, cm, cs, tab);
-          e1 = cs >= 8u ? smx_e(d1 & 0xFFFFu, sc, tab) : smx_e_wide(d1 & 0xFFFFu, cm, cs, tab);
-        }
-        row[i] = (v0 ? smx_p(e0, R, fp) : 0u) | ((v1 ? smx_p(e1, R, fp) : 0u) << 16);
-      }
+  if (!again) {
+    e_pass(0, own, true);
+  } else {
+#pragma unroll 1
+    for (uint32_t a = 0; a < own; a += WIN) {
+      const uint32_t z = min(a + WIN, own);
+#pragma unroll 1
+      for (uint32_t j = a; j < z; j++) scores(first + j * kWarps, j - a);
+      e_pass(a, z, false);
+      __syncwarp();
     }
-  };
-  for (uint32_t a = t0; a < t1; a += A.win) {
-    const uint32_t e = min(a + A.win, t1);
-    if (nwin > 1) {
-      consumer_sync();  // the window before is read
-      for (uint32_t t = a; t < e; t++) scores(t, a);
-      consumer_sync();
-    }
-    e_pass(a, e, nwin == 1);
   }
-  cluster_meet();
+  __syncthreads();
   if (tid < kRows) {
     unsigned long long sum = 0;
-    if (X > 1)
+    for (uint32_t i = 0; i < kWarps; i++) sum += s_ws[i][tid];
+    s_s[tid] = sum;
+  }
+  if (X > 1) cluster_meet();
+  if (tid < kRows) {
+    unsigned long long sum = s_s[tid];
+    if (X > 1) {
+      sum = 0;
       for (uint32_t i = 0; i < X; i++) sum += cluster_ld64(cluster_addr(&s_s[tid], i));
-    else
-      sum = s_s[tid];
+    }
     s_R[tid] = smx_r(sum);
   }
-  consumer_sync();
+  __syncthreads();
 
-  const uint32_t dg = warp % DG, kg = warp / DG;
-  uint32_t acc[NT][3][4];
-#pragma unroll
-  for (uint32_t j = 0; j < NT; j++)
-#pragma unroll
-    for (int k = 0; k < 3; k++)
-#pragma unroll
-      for (int x = 0; x < 4; x++) acc[j][k][x] = 0;
-  for (uint32_t a = t0; a < t1; a += A.win) {
-    const uint32_t e = min(a + A.win, t1);
-    if (nwin > 1) {
-      consumer_sync();
-      for (uint32_t t = a; t < e; t++) scores(t, a);
-      consumer_sync();
+  // pass 3: P of a block in place, then its P.V
+  auto p_block = [&](uint32_t t, uint32_t slot) {
+#pragma unroll 1
+    for (uint32_t r = rh; r < nr; r += RSTEP) {
+      uint32_t* const p = S + (slot * rcap + r) * PITCH + rl;
+      const uint32_t x = *p, fp = s_fp[r], R = s_R[r];
+      uint32_t e0 = e_unpack(x & 0xFFFFu), e1 = e_unpack(x >> 16);
+      if (again) e_of(row_of(r), x, t, e0, e1);
+      if (fp >= 8u && fp <= 15u) {  // the high word of e R 2^(f_p - 8) + 2^31
+        const uint32_t Rp = R << (fp - 8u);
+        e0 = (uint32_t)(((uint64_t)e0 * Rp + (1ull << 31)) >> 32);
+        e1 = (uint32_t)(((uint64_t)e1 * Rp + (1ull << 31)) >> 32);
+        *p = pack_s16(e0, e1);
+      } else {
+        *p = smx_p(e0, R, fp) | smx_p(e1, R, fp) << 16;
+      }
     }
-    p_pass(a, e, nwin == 1);
-    consumer_sync();
-    for (uint32_t t = a; t < e; t++) {
-      const uint32_t s = gi % NST;
-      // every warp takes and leaves every tile, its own 32-key blocks or not: a slot is
-      // not filled again before all have seen it, so no wait falls a phase behind
-      if (ok) ok = wait_for(&full[s], (gi / NST) & 1u, A.err, 304);
-      __syncwarp();
-      gi++;
+    __syncwarp();
+  };
+  uint32_t acc[Sh::MT][4];
 #pragma unroll
-      for (uint32_t half = 0; half < 2; half++) {
-        const uint32_t u = 2u * (t - a) + half;
-        if (u % KG != kg) continue;
-        const uint8_t* vr = ring + s * STB + (32u * half + 4u * qt) * RB + (DW == 32 ? 32u * dg + 4u * qn : 2u * qn);
-        uint32_t vh[2][4], vl[2][4];
+  for (uint32_t j = 0; j < Sh::MT; j++)
 #pragma unroll
-        for (int p = 0; p < 2; p++) {
+    for (int x = 0; x < 4; x++) acc[j][x] = 0;
+  // rows of 64 bytes: odd quarters take each pair of keys in the other order, so that
+  // two quarters meet no bank twice
+  const bool turn = RB == 64 && (qt & 1u);
+  const uint32_t lowsel = turn ? 0x2064u : 0x6420u, highsel = turn ? 0x3175u : 0x7531u;
+  auto values = [&](uint32_t slot) {
+    const uint8_t* const st = stage_in(304);
+    const uint32_t* const pr = S + (slot * rcap + qn) * PITCH + 2u * qt;
+#pragma unroll(HD <= 64 ? KS / 32 : 1)
+    for (uint32_t k32 = 0; k32 < KS / 32; k32++) {
+      uint32_t p0[2], p1[2], p2[2] = {0, 0};
+#pragma unroll
+      for (uint32_t h = 0; h < 2; h++) {
+        uint2 v = make_uint2(0, 0);
+        if (qn < nr) v = *(const uint2*)(pr + 16u * k32 + 8u * h);
+        if (BITS == 16) {
+          p0[h] = __byte_perm(v.x, v.y, lowsel);
+          p1[h] = __byte_perm(v.x, v.y, highsel);
+        } else {  // P << shift: 23 bits, three planes against the codes
+          const uint8_t* const sp = st + KS * RB + 32u * k32 + 16u * h + 2u * qt;
+          const uint32_t sa = *(const uint16_t*)sp, sb = *(const uint16_t*)(sp + 8);
+          const uint32_t ya = (v.x & 0xFFFFu) << (sa & 31u), yb = (v.x >> 16) << (sb & 31u);
+          const uint32_t yc = (v.y & 0xFFFFu) << ((sa >> 8) & 31u), yd = (v.y >> 16) << ((sb >> 8) & 31u);
+          const uint32_t y0 = turn ? yc : ya, y1 = turn ? yd : yb, y2 = turn ? ya : yc, y3 = turn ? yb : yd;
+          const uint32_t f = __byte_perm(y0, y1, 0x5140), z = __byte_perm(y2, y3, 0x5140);
+          p0[h] = __byte_perm(f, z, 0x5410);
+          p1[h] = __byte_perm(f, z, 0x7632);
+          p2[h] = __byte_perm(__byte_perm(y0, y1, 0x0062), __byte_perm(y2, y3, 0x0062), 0x5410);
+        }
+      }
+      // this lane's four keys of 16 in the words' order: base, base + 8, and their neighbours
+      const uint32_t base = 32u * k32 + 2u * qt + (turn ? 1u : 0u);
+      const int32_t step = turn ? -(int32_t)RB : (int32_t)RB;
+#pragma unroll
+      for (uint32_t ch = 0; ch < Sh::CH; ch++) {
+        uint32_t th[2][4], tl[2][4];
+#pragma unroll
+        for (uint32_t h = 0; h < 2; h++) {
+          const uint8_t* const v0 = st + (base + 16u * h) * RB + (HD >= 32 ? 32u * ch + 4u * qn : 2u * qn);
           uint32_t x[4], y[4];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint8_t* q = vr + (16u * p + i) * RB;
-            if (DW == 32) {
-              // quarters alternate between the planes, as the scores' keys do
-              if (BITS == 16) {
+          for (uint32_t i = 0; i < 4; i++) {
+            const uint8_t* const q = v0 + (i & 1u) * 8u * RB + (int32_t)(i >> 1) * step;
+            if constexpr (HD >= 32) {
+              if (BITS == 16) {  // quarters alternate between the planes: two meet no bank twice
                 const uint32_t f0 = *(const uint32_t*)(q + ((qt & 1u) ? HD : 0)), f1 = *(const uint32_t*)(q + ((qt & 1u) ? 0 : HD));
                 x[i] = (qt & 1u) ? f1 : f0;
                 y[i] = (qt & 1u) ? f0 : f1;
@@ -791,103 +834,109 @@ __global__ void __launch_bounds__(288, HD <= 128 ? 2 : 1) paged_attn_split_kerne
               if (BITS == 16) y[i] = *(const uint16_t*)(q + HD);
             }
           }
-          transpose4(x[0], x[1], x[2], x[3], vh[p]);
-          if (BITS == 16) transpose4(y[0], y[1], y[2], y[3], vl[p]);
-        }
-        const int16_t* pr = S + u * 32u + 4u * qt;
-        uint32_t p0[4], p1[4], p2[4];
-        uint32_t shw[2] = {0, 0};
-        if (BITS == 8) {
-          const uint8_t* sv = ring + s * STB + kT * RB + 32u * half + 4u * qt;
-          shw[0] = *(const uint32_t*)sv;
-          shw[1] = *(const uint32_t*)(sv + 16);
+          transpose4(x[0], x[1], x[2], x[3], th[h]);
+          if (BITS == 16) transpose4(y[0], y[1], y[2], y[3], tl[h]);
         }
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
-          const uint32_t row = qn + 8u * (x & 1);
-          uint2 v = make_uint2(0, 0);
-          if (row < nr) v = *(const uint2*)(pr + row * pitch + 16u * (x >> 1));
+        for (uint32_t jj = 0; jj < (HD >= 32 ? 2 : 1); jj++) {
+          uint32_t (&o)[4] = acc[HD >= 32 ? 2u * ch + jj : 0u];
+          const uint32_t ah[4] = {th[0][2 * jj], th[0][2 * jj + 1], th[1][2 * jj], th[1][2 * jj + 1]};
+          uint32_t a0[4] = {0, 0, 0, 0}, a1[4] = {0, 0, 0, 0}, a2[4] = {0, 0, 0, 0};
           if (BITS == 16) {
-            p0[x] = __byte_perm(v.x, v.y, 0x6420);
-            p1[x] = __byte_perm(v.x, v.y, 0x7531);
-          } else {  // P << shift: 23 bits, three planes against the codes
-            const uint32_t sw = shw[x >> 1];
-            const uint32_t y0 = (v.x & 0xFFFFu) << (sw & 31u), y1 = (v.x >> 16) << ((sw >> 8) & 31u);
-            const uint32_t y2 = (v.y & 0xFFFFu) << ((sw >> 16) & 31u), y3 = (v.y >> 16) << ((sw >> 24) & 31u);
-            const uint32_t f = __byte_perm(y0, y1, 0x5140), h = __byte_perm(y2, y3, 0x5140);
-            p0[x] = __byte_perm(f, h, 0x5410);
-            p1[x] = __byte_perm(f, h, 0x7632);
-            p2[x] = __byte_perm(__byte_perm(y0, y1, 0x0062), __byte_perm(y2, y3, 0x0062), 0x5410);
-          }
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < NT; j++) {
-          if (BITS == 16) {
-            mma_uu(acc[j][0], p0, vl[0][j], vl[1][j]);
-            mma_us(acc[j][1], p0, vh[0][j], vh[1][j]);
-            mma_uu(acc[j][1], p1, vl[0][j], vl[1][j]);
-            mma_us(acc[j][2], p1, vh[0][j], vh[1][j]);
+            const uint32_t al[4] = {tl[0][2 * jj], tl[0][2 * jj + 1], tl[1][2 * jj], tl[1][2 * jj + 1]};
+            mma_uu(a0, al, p0[0], p0[1]);
+            mma_su(a1, ah, p0[0], p0[1]);
+            mma_uu(a1, al, p1[0], p1[1]);
+            mma_su(a2, ah, p1[0], p1[1]);
           } else {
-            mma_us(acc[j][0], p0, vh[0][j], vh[1][j]);
-            mma_us(acc[j][1], p1, vh[0][j], vh[1][j]);
-            mma_us(acc[j][2], p2, vh[0][j], vh[1][j]);
+            mma_su(a0, ah, p0[0], p0[1]);
+            mma_su(a1, ah, p1[0], p1[1]);
+            mma_su(a2, ah, p2[0], p2[1]);
           }
+#pragma unroll
+          for (int x = 0; x < 4; x++) o[x] += a0[x] + (a1[x] << 8) + (a2[x] << 16);
         }
       }
-      __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&empty[s]);
+    }
+    stage_out();
+  };
+#pragma unroll 1
+  for (uint32_t a = 0; a < own; a += WIN) {
+    const uint32_t z = min(a + WIN, own);
+    if (again)
+#pragma unroll 1
+      for (uint32_t j = a; j < z; j++) scores(first + j * kWarps, j - a);
+#pragma unroll 1
+    for (uint32_t j = a; j < z; j++) {
+      p_block(first + j * kWarps, j - a);
+      values(j - a);
     }
   }
-  // the key groups' sums (modulo 2^32: any order), then the cluster's
-  if (t1 > t0) {
+  // the warps' sums (modulo 2^32: any order) through their stages, which are read and
+  // hold kRows HD words at least; then the cluster's
+  uint32_t* const part = (uint32_t*)ring;  // [row][HD]
 #pragma unroll
-    for (uint32_t j = 0; j < NT; j++)
-#pragma unroll
-      for (int x = 0; x < 4; x++) {
-        const uint32_t row = qn + 8u * (x >> 1), col = 2u * qt + (x & 1);
-        const uint32_t dim = DW == 32 ? 32u * dg + 4u * col + j : 2u * col + j;
-        const uint32_t v = acc[j][0][x] + (acc[j][1][x] << 8) + (acc[j][2][x] << 16);
-        if (row < nr) atomicAdd(&s_O[row * HD + dim], v);
-      }
+  for (uint32_t j = 0; j < Sh::MT; j++) {
+    // sums 0, 1: dimension 32 ch + 4 qn + 2 jj (HD 16: 2 qn) of rows ra, rb; 2, 3: the next
+    const uint32_t dim = HD >= 32 ? 32u * (j >> 1) + 4u * qn + 2u * (j & 1u) : 2u * qn;
+    if (ra < nr) *(uint2*)(part + ra * HD + dim) = make_uint2(acc[j][0], acc[j][2]);
+    if (rb < nr) *(uint2*)(part + rb * HD + dim) = make_uint2(acc[j][1], acc[j][3]);
   }
-  cluster_meet();
-  for (uint32_t i = rank * 256u + tid; i < nr * HD; i += X * 256u) {
-    uint32_t v = 0;
-    if (X > 1)
-      for (uint32_t k = 0; k < X; k++) v += cluster_ld32(cluster_addr(&s_O[i], k));
-    else
-      v = s_O[i];
+  __syncthreads();
+  auto put = [&](uint32_t i, uint32_t v) {
     const uint32_t rr = r0 + i / HD;
     A.d.o[(uint64_t)(sq.lo + rr / G) * A.d.ldo + (uint64_t)(g * G + rr % G) * HD + i % HD] = (int16_t)out16(v);
+  };
+  for (uint32_t i = tid; i < nr * HD; i += 256u) {
+    uint32_t v = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kWarps; k++) v += *(const uint32_t*)(pa_sm + k * NST * STB + 4u * i);
+    if (X > 1) s_O[i] = v;
+    else put(i, v);
   }
-  if (X > 1) cluster_sync();  // no CTA leaves while another reads its sums
+  if (X > 1) {
+    cluster_meet();
+    for (uint32_t i = rank * 256u + tid; i < nr * HD; i += X * 256u) {
+      uint32_t v = 0;
+      for (uint32_t k = 0; k < X; k++) v += cluster_ld32(cluster_addr(&s_O[i], k));
+      put(i, v);
+    }
+    cluster_sync();  // no CTA leaves while another reads its sums
+  }
 }
 
 template <int HD, int BITS>
 int launch_split(SplitArgs A, uint32_t tiles, cudaStream_t st) {
   using Sh = SplitShape<HD, BITS>;
   const corm_paged_cache& c = A.d.c;
-  // two CTAs an SM up to 128 dimensions: about 112 KB each
-  const uint32_t budget = HD <= 128 ? 110u * 1024u : 220u * 1024u;
-  uint32_t stages = 48u * 1024u / Sh::STB;
-  A.stages = stages = stages < 3u ? 3u : (stages > 8u ? 8u : stages);
   const uint64_t blocks = (uint64_t)c.B * c.KV * tiles;
   const uint32_t cap = c.table_width * c.page, keys = A.d.max_keys < cap ? A.d.max_keys : cap;
-  uint32_t X = 1;
-  while (X < kMaxCluster && blocks * X < 296u && keys / (2u * X) >= 128u) X *= 2u;
-  A.X = X;
-  const uint32_t fixed = stages * Sh::STB + A.rcap * HD * 4u + 8192u;
-  const uint32_t room = (budget - fixed) / (A.rcap * 2u), most = (room - 16u) / kT;
   const uint32_t span = A.d.window && A.d.window < keys ? A.d.window + A.d.max_q : keys;
-  const uint32_t need = ((span < keys ? span : keys) / kT + 2u + X - 1u) / X;
-  A.win = need < 1u ? 1u : (need < most ? need : most);
-  const size_t smem = stages * Sh::STB + (size_t)A.rcap * split_pitch(A.win) * 2u + A.rcap * HD * 4u + 8192u;
+  const uint32_t kblocks = (span < keys ? span : keys) / Sh::KS + 2u;
+  // a cluster's CTAs: while all are resident at once and each warp has two blocks
+  uint32_t X = 1;
+  while (X < kMaxCluster && blocks * (X + 1u) <= 148u * Sh::OCC && kblocks >= 2u * kWarps * (X + 1u)) X++;
+  A.X = X;
+  const uint32_t need = ((kblocks + X - 1u) / X + kWarps - 1u) / kWarps;  // of a warp
+  const uint32_t fixed = 8192u + (X > 1 ? A.rcap * HD * 4u : 0u), block = kWarps * A.rcap * Sh::PITCH * 4u;
+  // as many CTAs an SM as the registers allow, if the scores fit beside two stages a warp
+  uint32_t occ = Sh::OCC, room = 0;
+  for (;; occ--) {
+    room = (occ == 3u ? 72u : (occ == 2u ? 110u : 222u)) * 1024u - fixed;
+    if (occ == 1u || (uint64_t)need * block + 2u * kWarps * Sh::STB <= room) break;
+  }
+  uint32_t stages = 1;
+  const uint32_t most = (room - kWarps * Sh::STB) / block;
+  A.win = need < most ? need : most;
+  while (stages < 4u && A.win * block + (stages + 1u) * kWarps * Sh::STB <= room) stages++;
+  A.stages = stages;
+  const size_t smem = kWarps * stages * Sh::STB + (size_t)A.win * block + fixed;
   auto kern = paged_attn_split_kernel<HD, BITS>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return corm::cuda_status("llm_paged_attn");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles * X, c.KV, c.B);
-  cfg.blockDim = dim3(288);
+  cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];

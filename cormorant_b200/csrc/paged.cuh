@@ -101,6 +101,12 @@ __device__ __forceinline__ int32_t out16(uint32_t acc) {
   const int32_t y = (int32_t)acc >> 8;
   return min(max(y, -32768), 32767);
 }
+// two values saturated to 16 bits in a word (lo in the low half)
+__device__ __forceinline__ uint32_t pack_s16(uint32_t lo, uint32_t hi) {
+  uint32_t r;
+  asm("cvt.pack.sat.s16.s32 %0, %1, %2;" : "=r"(r) : "r"(hi), "r"(lo));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack16(int32_t lo, int32_t hi) {  // both already in int16
   return ((uint32_t)hi << 16) | ((uint32_t)lo & 0xFFFFu);
 }

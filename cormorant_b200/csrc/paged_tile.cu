@@ -78,11 +78,6 @@ __device__ __forceinline__ uint32_t shr_clamp(uint32_t x, uint32_t s) {  // 0 fr
   return r;
 }
 // two values saturated to 16 bits in a word (lo in the low half)
-__device__ __forceinline__ uint32_t pack_s16(uint32_t lo, uint32_t hi) {
-  uint32_t r;
-  asm("cvt.pack.sat.s16.s32 %0, %1, %2;" : "=r"(r) : "r"(hi), "r"(lo));
-  return r;
-}
 __device__ __forceinline__ uint32_t pack_u16(uint32_t lo, uint32_t hi) {
   uint32_t r;
   asm("cvt.pack.sat.u16.s32 %0, %1, %2;" : "=r"(r) : "r"(hi), "r"(lo));
