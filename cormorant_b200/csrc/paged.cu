@@ -423,14 +423,20 @@ struct SplitShape {
   static constexpr uint32_t CH = HD < 32 ? 1 : HD / 32;       // chunks of 32 (HD 16: 16) dimensions
   static constexpr uint32_t MT = HD / 16;                     // 16-dimension tiles of the output
   static constexpr uint32_t PW = KS / 2;                      // words of a row's scores in a block
-  static constexpr uint32_t PITCH = PW + 8;                   // a row's words: 8 mod 16, so four rows' reads meet no bank twice
   static constexpr uint32_t OCC = HD <= 64 ? 3 : (HD == 128 ? 2 : 1);  // CTAs an SM that the registers allow
 };
+
+// word i of row r's scores in a block: groups of 8 words trade places by the row, so that
+// four rows' reads meet no bank twice
+template <uint32_t PW>
+__device__ __forceinline__ uint32_t score_word(uint32_t r, uint32_t i) {
+  return r * PW + (i ^ (PW == 32 ? 8u * (r & 3u) : 8u * ((r >> 1) & 1u)));
+}
 
 template <int HD, int BITS>
 __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_split_kernel(const __grid_constant__ SplitArgs A) {
   using Sh = SplitShape<HD, BITS>;
-  constexpr uint32_t RB = Sh::RB, KS = Sh::KS, STB = Sh::STB, NKS = Sh::NKS, PW = Sh::PW, PITCH = Sh::PITCH;
+  constexpr uint32_t RB = Sh::RB, KS = Sh::KS, STB = Sh::STB, NKS = Sh::NKS, PW = Sh::PW;
   extern __shared__ __align__(128) uint8_t pa_sm[];
   __shared__ uint64_t full[kWarps][4], cbar;
   __shared__ int32_t s_wmax[kWarps][kRows], s_m[kRows], s_gm[kRows];
@@ -441,8 +447,8 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   const uint32_t X = A.X, tile = blockIdx.x / X, rank = blockIdx.x % X, g = blockIdx.y, b = blockIdx.z, G = A.G;
   const uint32_t NST = A.stages, rcap = A.rcap, WIN = A.win;
   uint8_t* const ring = pa_sm + warp * NST * STB;                                          // this warp's stages
-  uint32_t* const S = (uint32_t*)(pa_sm + kWarps * NST * STB) + warp * WIN * rcap * PITCH;  // and scores: [block][row][PITCH]
-  uint16_t* const tab = (uint16_t*)(pa_sm + kWarps * (NST * STB + WIN * rcap * PITCH * 4u));
+  uint32_t* const S = (uint32_t*)(pa_sm + kWarps * NST * STB) + warp * WIN * rcap * PW;  // and scores: [block][row][PW]
+  uint16_t* const tab = (uint16_t*)(pa_sm + kWarps * (NST * STB + WIN * rcap * PW * 4u));
   uint32_t* const s_O = (uint32_t*)(tab + 4096);
   uint64_t* const bars = full[warp];
   if (lane == 0)
@@ -570,19 +576,23 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   uint32_t mxa = 0x80008000u, mxb = 0x80008000u;
   auto scores = [&](uint32_t t, uint32_t slot) {
     const uint8_t* const st = stage_in(302);
-    uint32_t* const d = S + slot * rcap * PITCH;
+    uint32_t* const d = S + slot * rcap * PW;
     const bool whole = t * KS >= lo_last && (t + 1u) * KS <= hi_first;
 #pragma unroll
     for (uint32_t k16 = 0; k16 < KS / 16; k16++) {
       const uint8_t* const row = st + (16u * k16 + qn) * RB;
-      uint32_t hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
+      uint32_t hh[4], mid[4], ll[4];
       auto step = [&](uint32_t ks, const uint32_t (&h)[4], const uint32_t (&l)[4]) {
-        mma_ss(hh, h, bh[ks][0], bh[ks][1]);
-        mma_su(mid, h, bl[ks][0], bl[ks][1]);
-        if (BITS == 16) {
-          mma_us(mid, l, bh[ks][0], bh[ks][1]);
-          mma_uu(ll, l, bl[ks][0], bl[ks][1]);
+        if (ks == 0) {
+          mma_ss_first(hh, h, bh[ks][0], bh[ks][1]);
+          mma_su_first(mid, h, bl[ks][0], bl[ks][1]);
+          if (BITS == 16) mma_uu_first(ll, l, bl[ks][0], bl[ks][1]);
+        } else {
+          mma_ss(hh, h, bh[ks][0], bh[ks][1]);
+          mma_su(mid, h, bl[ks][0], bl[ks][1]);
+          if (BITS == 16) mma_uu(ll, l, bl[ks][0], bl[ks][1]);
         }
+        if (BITS == 16) mma_us(mid, l, bh[ks][0], bh[ks][1]);
       };
       if constexpr (HD >= 64) {
 #pragma unroll
@@ -623,8 +633,8 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
         for (int x = 0; x < 4; x++) y[x] = (uint32_t)((int32_t)(((hh[x] << 8) + mid[x]) << (x < 2 ? s0 : s1)) >> 8);
       }
       uint32_t wa = pack_s16(y[0], y[2]), wb = pack_s16(y[1], y[3]);
-      if (ra < nr) d[ra * PITCH + 8u * k16 + qn] = wa;
-      if (rb < nr) d[rb * PITCH + 8u * k16 + qn] = wb;
+      if (ra < nr) d[score_word<PW>(ra, 8u * k16 + qn)] = wa;
+      if (rb < nr) d[score_word<PW>(rb, 8u * k16 + qn)] = wb;
       if (!whole) {
         const uint32_t k0 = t * KS + 16u * k16 + qn, k1 = k0 + 8u;
         const uint32_t la = s_lo[ra], ha = s_hi[ra], lb = s_lo[rb], hb = s_hi[rb];
@@ -678,31 +688,35 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   const uint32_t rl = lane % PW, rh = lane / PW;
   constexpr uint32_t RSTEP = 32 / PW;
   const uint32_t word_key = 16u * (rl >> 3) + (rl & 7u);  // the word's first key in its block; the second is 8 on
-  // e of a word's two scores, 0 where the row does not see the key
+  // e of a word's two scores, 0 where the row does not see the key.  With 9 <= Cs the
+  // product of d 2^16 and Cm 2^8, shifted down, is floor(d Cm / 2^(Cs - 1)) = 2 y and a
+  // bit: the table's byte offset is it mod 2^13 without the bit, the octave it / 2^13
   struct Row {
-    uint32_t cm, cs, klo, khi;
-    int32_t m;
-    SmxScale sc;
+    uint32_t cm, cs, klo, khi, m0, cm8, sh;
   };
   auto row_of = [&](uint32_t r) {
     Row o;
     o.cm = s_cm[r], o.cs = s_cs[r], o.klo = s_lo[r], o.khi = s_hi[r];
-    o.m = s_gm[r];
-    o.sc = smx_scale(o.cm, max(o.cs, 8u));
+    o.m0 = (uint32_t)s_gm[r] << 16;
+    o.cm8 = o.cs >= 40u ? 0u : (o.cm & 0xFFFFFFu) << 8;
+    o.sh = min(o.cs, 40u) - 9u;
     return o;
   };
   auto e_of = [&](const Row& o, uint32_t x, uint32_t t, uint32_t& e0, uint32_t& e1) {
-    const uint32_t d0 = (uint32_t)(o.m - (int32_t)(int16_t)x) & 0xFFFFu, d1 = (uint32_t)(o.m - ((int32_t)x >> 16)) & 0xFFFFu;
-    const uint32_t k0 = t * KS + word_key, k1 = k0 + 8u;
-    if (o.cs >= 8u) {
-      e0 = smx_e(d0, o.sc, tab);
-      e1 = smx_e(d1, o.sc, tab);
+    const uint32_t d0 = o.m0 - (x << 16), d1 = o.m0 - (x & 0xFFFF0000u);
+    if (o.cs >= 9u) {
+      const uint32_t t0 = __umulhi(d0, o.cm8) >> o.sh, t1 = __umulhi(d1, o.cm8) >> o.sh;
+      e0 = shr_clamp((uint32_t)*(const uint16_t*)((const uint8_t*)tab + (t0 & 0x1FFEu)) + 1u, t0 >> 13);
+      e1 = shr_clamp((uint32_t)*(const uint16_t*)((const uint8_t*)tab + (t1 & 0x1FFEu)) + 1u, t1 >> 13);
     } else {
-      e0 = smx_e_wide(d0, o.cm, o.cs, tab);
-      e1 = smx_e_wide(d1, o.cm, o.cs, tab);
+      e0 = smx_e_wide(d0 >> 16, o.cm, o.cs, tab);
+      e1 = smx_e_wide(d1 >> 16, o.cm, o.cs, tab);
     }
-    if (k0 < o.klo || k0 >= o.khi) e0 = 0;
-    if (k1 < o.klo || k1 >= o.khi) e1 = 0;
+    if (t * KS < lo_last || (t + 1u) * KS > hi_first) {  // (alike over the warp)
+      const uint32_t k0 = t * KS + word_key, k1 = k0 + 8u;
+      if (k0 < o.klo || k0 >= o.khi) e0 = 0;
+      if (k1 < o.klo || k1 >= o.khi) e1 = 0;
+    }
   };
   // pass 2: e of blocks [a, z) in place (or only the sums)
   auto e_pass = [&](uint32_t a, uint32_t z, bool keep) {
@@ -712,13 +726,13 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
       unsigned long long sum = 0;
       if (r < nr) {
         const Row o = row_of(r);
-        uint32_t* p = S + r * PITCH + rl;
+        uint32_t* p = S + score_word<PW>(r, rl);
 #pragma unroll 2
-        for (uint32_t j = a; j < z; j++, p += rcap * PITCH) {
+        for (uint32_t j = a; j < z; j++, p += rcap * PW) {
           uint32_t e0, e1;
           e_of(o, *p, first + j * kWarps, e0, e1);
           sum += e0 + e1;
-          if (keep) *p = e_pack(e0) | (e_pack(e1) << 16);
+          if (keep) *p = pack_u16(e0, e1);
         }
       }
 #pragma unroll
@@ -755,21 +769,27 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   }
   __syncthreads();
 
-  // pass 3: P of a block in place, then its P.V
-  auto p_block = [&](uint32_t t, uint32_t slot) {
+  // pass 3: P of blocks [a, z) in place, then P.V
+  auto p_pass = [&](uint32_t a, uint32_t z) {
 #pragma unroll 1
     for (uint32_t r = rh; r < nr; r += RSTEP) {
-      uint32_t* const p = S + (slot * rcap + r) * PITCH + rl;
-      const uint32_t x = *p, fp = s_fp[r], R = s_R[r];
-      uint32_t e0 = e_unpack(x & 0xFFFFu), e1 = e_unpack(x >> 16);
-      if (again) e_of(row_of(r), x, t, e0, e1);
-      if (fp >= 8u && fp <= 15u) {  // the high word of e R 2^(f_p - 8) + 2^31
-        const uint32_t Rp = R << (fp - 8u);
-        e0 = (uint32_t)(((uint64_t)e0 * Rp + (1ull << 31)) >> 32);
-        e1 = (uint32_t)(((uint64_t)e1 * Rp + (1ull << 31)) >> 32);
-        *p = pack_s16(e0, e1);
-      } else {
-        *p = smx_p(e0, R, fp) | smx_p(e1, R, fp) << 16;
+      uint32_t* p = S + score_word<PW>(r, rl);
+      const uint32_t fp = s_fp[r], R = s_R[r];
+      const bool fast = fp >= 8u && fp <= 15u;  // P is the high word of e R 2^(f_p - 8) + 2^31
+      const uint32_t Rp = fast ? R << (fp - 8u) : R;
+      const Row o = row_of(r);
+#pragma unroll 2
+      for (uint32_t j = a; j < z; j++, p += rcap * PW) {
+        const uint32_t x = *p, u0 = x & 0xFFFFu, u1 = x >> 16;
+        uint32_t e0 = u0 + ((u0 + 1u) >> 16), e1 = u1 + ((u1 + 1u) >> 16);
+        if (again) e_of(o, x, first + j * kWarps, e0, e1);
+        if (fast) {
+          e0 = (uint32_t)(((uint64_t)e0 * Rp + (1ull << 31)) >> 32);
+          e1 = (uint32_t)(((uint64_t)e1 * Rp + (1ull << 31)) >> 32);
+          *p = pack_s16(e0, e1);
+        } else {
+          *p = smx_p(e0, R, fp) | smx_p(e1, R, fp) << 16;
+        }
       }
     }
     __syncwarp();
@@ -785,14 +805,14 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   const uint32_t lowsel = turn ? 0x2064u : 0x6420u, highsel = turn ? 0x3175u : 0x7531u;
   auto values = [&](uint32_t slot) {
     const uint8_t* const st = stage_in(304);
-    const uint32_t* const pr = S + (slot * rcap + qn) * PITCH + 2u * qt;
+    const uint32_t* const pr = S + slot * rcap * PW;
 #pragma unroll(HD <= 64 ? KS / 32 : 1)
     for (uint32_t k32 = 0; k32 < KS / 32; k32++) {
       uint32_t p0[2], p1[2], p2[2] = {0, 0};
 #pragma unroll
       for (uint32_t h = 0; h < 2; h++) {
         uint2 v = make_uint2(0, 0);
-        if (qn < nr) v = *(const uint2*)(pr + 16u * k32 + 8u * h);
+        if (qn < nr) v = *(const uint2*)(pr + score_word<PW>(qn, 16u * k32 + 8u * h + 2u * qt));
         if (BITS == 16) {
           p0[h] = __byte_perm(v.x, v.y, lowsel);
           p1[h] = __byte_perm(v.x, v.y, highsel);
@@ -841,20 +861,20 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
         for (uint32_t jj = 0; jj < (HD >= 32 ? 2 : 1); jj++) {
           uint32_t (&o)[4] = acc[HD >= 32 ? 2u * ch + jj : 0u];
           const uint32_t ah[4] = {th[0][2 * jj], th[0][2 * jj + 1], th[1][2 * jj], th[1][2 * jj + 1]};
-          uint32_t a0[4] = {0, 0, 0, 0}, a1[4] = {0, 0, 0, 0}, a2[4] = {0, 0, 0, 0};
+          uint32_t a1[4], a2[4];
           if (BITS == 16) {
             const uint32_t al[4] = {tl[0][2 * jj], tl[0][2 * jj + 1], tl[1][2 * jj], tl[1][2 * jj + 1]};
-            mma_uu(a0, al, p0[0], p0[1]);
-            mma_su(a1, ah, p0[0], p0[1]);
+            mma_uu(o, al, p0[0], p0[1]);
+            mma_su_first(a1, ah, p0[0], p0[1]);
             mma_uu(a1, al, p1[0], p1[1]);
-            mma_su(a2, ah, p1[0], p1[1]);
+            mma_su_first(a2, ah, p1[0], p1[1]);
           } else {
-            mma_su(a0, ah, p0[0], p0[1]);
-            mma_su(a1, ah, p1[0], p1[1]);
-            mma_su(a2, ah, p2[0], p2[1]);
+            mma_su(o, ah, p0[0], p0[1]);
+            mma_su_first(a1, ah, p1[0], p1[1]);
+            mma_su_first(a2, ah, p2[0], p2[1]);
           }
 #pragma unroll
-          for (int x = 0; x < 4; x++) o[x] += a0[x] + (a1[x] << 8) + (a2[x] << 16);
+          for (int x = 0; x < 4; x++) o[x] += (a1[x] << 8) + (a2[x] << 16);
         }
       }
     }
@@ -866,11 +886,9 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
     if (again)
 #pragma unroll 1
       for (uint32_t j = a; j < z; j++) scores(first + j * kWarps, j - a);
+    p_pass(a, z);
 #pragma unroll 1
-    for (uint32_t j = a; j < z; j++) {
-      p_block(first + j * kWarps, j - a);
-      values(j - a);
-    }
+    for (uint32_t j = a; j < z; j++) values(j - a);
   }
   // the warps' sums (modulo 2^32: any order) through their stages, which are read and
   // hold kRows HD words at least; then the cluster's
@@ -913,18 +931,19 @@ int launch_split(SplitArgs A, uint32_t tiles, cudaStream_t st) {
   const uint32_t cap = c.table_width * c.page, keys = A.d.max_keys < cap ? A.d.max_keys : cap;
   const uint32_t span = A.d.window && A.d.window < keys ? A.d.window + A.d.max_q : keys;
   const uint32_t kblocks = (span < keys ? span : keys) / Sh::KS + 2u;
-  // a cluster's CTAs: while all are resident at once and each warp has two blocks
-  uint32_t X = 1;
-  while (X < kMaxCluster && blocks * (X + 1u) <= 148u * Sh::OCC && kblocks >= 2u * kWarps * (X + 1u)) X++;
-  A.X = X;
-  const uint32_t need = ((kblocks + X - 1u) / X + kWarps - 1u) / kWarps;  // of a warp
-  const uint32_t fixed = 8192u + (X > 1 ? A.rcap * HD * 4u : 0u), block = kWarps * A.rcap * Sh::PITCH * 4u;
-  // as many CTAs an SM as the registers allow, if the scores fit beside two stages a warp
-  uint32_t occ = Sh::OCC, room = 0;
+  // the CTAs an SM that the registers allow, or fewer: so many that the scores fit beside
+  // a stage a warp (two, where the registers bound); and as many CTAs a cluster as are
+  // all resident at once and leave each warp two blocks
+  uint32_t X, occ = Sh::OCC, room, need, fixed;
+  const uint32_t block = kWarps * A.rcap * Sh::PW * 4u;
   for (;; occ--) {
-    room = (occ == 3u ? 72u : (occ == 2u ? 110u : 222u)) * 1024u - fixed;
-    if (occ == 1u || (uint64_t)need * block + 2u * kWarps * Sh::STB <= room) break;
+    for (X = 1; X < kMaxCluster && blocks * (X + 1u) <= 148u * occ && kblocks >= 2u * kWarps * (X + 1u);) X++;
+    fixed = 8192u + (X > 1 ? A.rcap * HD * 4u : 0u);
+    need = ((kblocks + X - 1u) / X + kWarps - 1u) / kWarps;  // of a warp
+    room = (occ == 3u ? 73u : (occ == 2u ? 110u : 222u)) * 1024u - fixed;
+    if (occ == 1u || (uint64_t)need * block + (occ == 3u ? 1u : 2u) * kWarps * Sh::STB <= room) break;
   }
+  A.X = X;
   uint32_t stages = 1;
   const uint32_t most = (room - kWarps * Sh::STB) / block;
   A.win = need < most ? need : most;

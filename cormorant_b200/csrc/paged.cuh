@@ -38,31 +38,12 @@ __device__ __forceinline__ SeqRows seq_rows(const corm_paged_cache& c, uint32_t 
 // ---------------------------------------------------------------- the softmax unit's integers
 // e of a score d below the row's maximum: y = (d Cm) >> Cs, TAB[y mod 4096] >>
 // (y / 4096).  The table is held less one in 16 bits (TAB is 32774 .. 65536).
-struct SmxScale {
-  uint32_t cm8;  // Cm << 8
-  uint32_t sh;   // Cs - 8
-};
-// 8 <= Cs: (d << 16)(Cm << 8) >> 32 = (d Cm) >> 8 fits 32 bits (d < 2^16, Cm < 2^24),
-// and from Cs = 40 on y is 0
-__device__ __forceinline__ SmxScale smx_scale(uint32_t cm, uint32_t cs) {
-  SmxScale s;
-  s.cm8 = cs >= 40u ? 0u : (cm & 0xFFFFFFu) << 8;
-  s.sh = cs >= 40u ? 0u : cs - 8u;
-  return s;
-}
-__device__ __forceinline__ uint32_t smx_e(uint32_t d, SmxScale s, const uint16_t* tab) {
-  const uint32_t y = __umulhi(d << 16, s.cm8) >> s.sh;
-  const uint32_t o = y >> 12;
-  const uint32_t t = (uint32_t)tab[y & 4095u] + 1u;
-  return o > 16u ? 0u : t >> o;
-}
-// Cs < 8: y may pass 32 bits
+// any Cs (y may pass 32 bits below 8)
 __device__ __forceinline__ uint32_t smx_e_wide(uint32_t d, uint32_t cm, uint32_t cs, const uint16_t* tab) {
   const uint64_t y = ((uint64_t)d * (cm & 0xFFFFFFu)) >> cs;
   return (y >> 12) > 16u ? 0u : ((uint32_t)tab[y & 4095u] + 1u) >> (uint32_t)(y >> 12);
 }
 // e in 16 bits: TAB[0] = 65536 is the only value past 65535, and no entry is 65535
-__device__ __forceinline__ uint32_t e_pack(uint32_t e) { return min(e, 65535u); }
 __device__ __forceinline__ uint32_t e_unpack(uint32_t h) { return h + (h == 65535u ? 1u : 0u); }
 
 // P = min((e R + 2^(39 - f_p)) >> (40 - f_p), 32767); e R < 2^41
@@ -107,6 +88,16 @@ __device__ __forceinline__ uint32_t pack_s16(uint32_t lo, uint32_t hi) {
   asm("cvt.pack.sat.s16.s32 %0, %1, %2;" : "=r"(r) : "r"(hi), "r"(lo));
   return r;
 }
+__device__ __forceinline__ uint32_t shr_clamp(uint32_t x, uint32_t s) {  // 0 from 32 up
+  uint32_t r;
+  asm("shr.u32 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(s));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_u16(uint32_t lo, uint32_t hi) {
+  uint32_t r;
+  asm("cvt.pack.sat.u16.s32 %0, %1, %2;" : "=r"(r) : "r"(hi), "r"(lo));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack16(int32_t lo, int32_t hi) {  // both already in int16
   return ((uint32_t)hi << 16) | ((uint32_t)lo & 0xFFFFu);
 }
@@ -119,6 +110,13 @@ __device__ __forceinline__ uint32_t pack16(int32_t lo, int32_t hi) {  // both al
                  ".s32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"                                             \
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])                                                      \
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));                                      \
+  }                                                                                                                    \
+  /* C = A B */                                                                                                        \
+  __device__ __forceinline__ void NAME##_first(uint32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   \
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." TA "." TB                                                    \
+                 ".s32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%10,%10,%10,%10};"                                         \
+                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])                                                      \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));                              \
   }
 CORM_MMA_I8(mma_ss, "s8", "s8")
 CORM_MMA_I8(mma_su, "s8", "u8")

@@ -72,17 +72,6 @@ struct TileArgs {
 };
 
 __device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(RT) : "memory"); }
-__device__ __forceinline__ uint32_t shr_clamp(uint32_t x, uint32_t s) {  // 0 from 32 up
-  uint32_t r;
-  asm("shr.u32 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(s));
-  return r;
-}
-// two values saturated to 16 bits in a word (lo in the low half)
-__device__ __forceinline__ uint32_t pack_u16(uint32_t lo, uint32_t hi) {
-  uint32_t r;
-  asm("cvt.pack.sat.u16.s32 %0, %1, %2;" : "=r"(r) : "r"(hi), "r"(lo));
-  return r;
-}
 // A row's softmax registers and maximum as e of a packed score pair wants them.
 // t = floor(d Cm / 2^(Cs - 2)) = 4 y and two bits: the table's byte offset is t mod
 // 2^14 without them, the octave t / 2^14.
