@@ -393,8 +393,8 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__
 // the three passes.
 //
 // The eight warps work apart: a warp has every eighth block of keys (32 or 64),
-// copies them itself into stages of its own (one bulk copy per page piece, the
-// next under way while it computes; the V rows arrive under the softmax), and
+// copies them itself into stages of its own (16 bytes a lane, the next under way
+// while it computes; the V rows arrive under the softmax), and
 // nothing but the maxima, the sums and the output meets.  Warp-level MMAs with the
 // keys, then the output's dimensions, as the 16 rows of an MMA and the query rows as
 // its 8 columns: a decoded token's group of heads is far below the 128 rows of a
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   using Sh = SplitShape<HD, BITS>;
   constexpr uint32_t RB = Sh::RB, KS = Sh::KS, STB = Sh::STB, NKS = Sh::NKS, PW = Sh::PW;
   extern __shared__ __align__(128) uint8_t pa_sm[];
-  __shared__ uint64_t full[kWarps][4], cbar;
+  __shared__ uint64_t cbar;
   __shared__ int32_t s_wmax[kWarps][kRows], s_m[kRows], s_gm[kRows];
   __shared__ unsigned long long s_ws[kWarps][kRows], s_s[kRows];
   __shared__ uint32_t s_R[kRows], s_lo[kRows], s_hi[kRows], s_cm[kRows], s_cs[kRows], s_fp[kRows];
@@ -450,12 +450,10 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   uint32_t* const S = (uint32_t*)(pa_sm + kWarps * NST * STB) + warp * WIN * rcap * PW;  // and scores: [block][row][PW]
   uint16_t* const tab = (uint16_t*)(pa_sm + kWarps * (NST * STB + WIN * rcap * PW * 4u));
   uint32_t* const s_O = (uint32_t*)(tab + 4096);
-  uint64_t* const bars = full[warp];
-  if (lane == 0)
-    for (uint32_t i = 0; i < NST; i++) sm100::mbar_init(&bars[i], 1);
-  if (tid == 0) sm100::mbar_init(&cbar, X);
-  sm100::fence_mbar_init();
-  __syncwarp();
+  if (tid == 0) {
+    sm100::mbar_init(&cbar, X);
+    sm100::fence_mbar_init();
+  }
   corm_pdl_wait();
   corm_pdl_trigger();
   const SeqRows sq = seq_rows(c, b, c.rows);
@@ -478,48 +476,61 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   const uint32_t sub = min(c.page, KS), pieces = KS / sub, psh = 31u - __clz(c.page);
   const int32_t* const tb = c.table + (uint64_t)b * c.table_width;
   const uint32_t total = again ? 4u * own : 2u * own;
-  uint32_t eq = 0, ej = 0, ea = 0, ep = 0;  // the next copy's number, block, window and pass
-  bool ev = false;                          // of V
-  auto page_of = [&]() -> int32_t {         // the page of this lane's piece of the next copy
+  uint32_t eq = 0, ej = 0, ea = 0, ep = 0, es = 0;  // the next copy's number, block, window, pass and stage
+  bool ev = false;                                  // of V
+  auto page_of = [&]() -> int32_t {                 // the page of piece `lane` of the next copy, below 0: none
     const uint32_t key = (first + ej * kWarps) * KS + lane * sub;
-    return eq < total && lane < pieces && key < hi ? tb[key >> psh] : -1;
+    int32_t id = -1;
+    if (eq < total && lane < pieces && key < hi) id = tb[key >> psh];
+    return (uint32_t)id < c.pages ? id : -1;
   };
   int32_t id = page_of();
-  uint32_t es = 0;
+  // one group of asynchronous copies, 16 bytes a lane (empty after the last block);
+  // pieces without a page are zeros
   auto emit = [&]() {
-    const uint32_t key = (first + ej * kWarps) * KS + lane * sub;
-    const bool in = lane < pieces && key < hi, good = in && (uint32_t)id < c.pages;
-    uint8_t* const st = ring + es * STB;
-    if (in && !good) {  // a page of zeros
-      uint8_t* const dst = st + lane * sub * RB;
-      for (uint32_t i = 0; i < sub * RB; i += 16u) *(int4*)(dst + i) = make_int4(0, 0, 0, 0);
-      if (BITS == 8)
-        for (uint32_t i = 0; i < sub; i += 16u) *(int4*)(st + KS * RB + lane * sub + i) = make_int4(0, 0, 0, 0);
-      sm100::fence_proxy_async_smem();
+    if (eq < total) {
+      uint8_t* const st = ring + es * STB;
+      const uint8_t* const rows = ev ? (const uint8_t*)c.vc : (const uint8_t*)c.kc;
+      const uint32_t in0 = ((first + ej * kWarps) * KS) & (c.page - 1u);  // a block in a page: its first row
+      if (pieces == 1u) {
+        const int32_t pg = __shfl_sync(0xffffffffu, id, 0);
+        const uint32_t n = pg < 0 ? 0u : 16u;
+        const uint64_t line = ((uint64_t)(uint32_t)max(pg, 0) * c.KV + g) * c.page + in0;
+        const uint8_t* const src = rows + line * RB + lane * 16u;
+#pragma unroll
+        for (uint32_t i = 0; i < KS * RB / 512u; i++) cp_async16(st + lane * 16u + i * 512u, src + i * 512u, n);
+        if (BITS == 8 && lane < KS / 16u) cp_async16(st + KS * RB + lane * 16u, (ev ? c.vs : c.ks) + line + lane * 16u, n);
+      } else {
+#pragma unroll 1
+        for (uint32_t i = lane * 16u; i < KS * RB; i += 512u) {
+          const uint32_t row = i / RB;
+          const int32_t pg = __shfl_sync(0xffffffffu, id, row / sub);
+          const uint64_t line = ((uint64_t)(uint32_t)max(pg, 0) * c.KV + g) * c.page + row % sub;
+          cp_async16(st + i, rows + line * RB + i % RB, pg < 0 ? 0u : 16u);
+        }
+        if (BITS == 8) {
+          const int32_t pg = __shfl_sync(0xffffffffu, id, (lane * 16u / sub) & 31u);
+          const uint64_t line = ((uint64_t)(uint32_t)max(pg, 0) * c.KV + g) * c.page + lane * 16u % sub;
+          if (lane < KS / 16u) cp_async16(st + KS * RB + lane * 16u, (ev ? c.vs : c.ks) + line, pg < 0 ? 0u : 16u);
+        }
+      }
+      if (++es == NST) es = 0;
+      eq++;
+      ej++;
+      if (!again) {
+        if (ej == own) ej = 0, ev = true;
+      } else if (ep < 2u) {
+        if (ej == own) ej = 0, ep++;
+      } else if (ej == min(ea + WIN, own)) {
+        if (ev) ea += WIN;
+        ev = !ev;
+        ej = ea;
+      }
+      id = page_of();
     }
-    const uint32_t cnt = __popc(__ballot_sync(0xffffffffu, good));
-    if (lane == 0) sm100::mbar_expect_tx(&bars[es], cnt * sub * (RB + (BITS == 8 ? 1u : 0u)));
-    __syncwarp();
-    if (good) {
-      const uint64_t line = ((uint64_t)(uint32_t)id * c.KV + g) * c.page + (key & (c.page - 1u));
-      bulk_g2s(st + lane * sub * RB, (ev ? c.vc : c.kc) + line * RB, sub * RB, &bars[es]);
-      if (BITS == 8) bulk_g2s(st + KS * RB + lane * sub, (ev ? c.vs : c.ks) + line, sub, &bars[es]);
-    }
-    if (++es == NST) es = 0;
-    eq++;
-    ej++;
-    if (!again) {
-      if (ej == own) ej = 0, ev = true;
-    } else if (ep < 2u) {
-      if (ej == own) ej = 0, ep++;
-    } else if (ej == min(ea + WIN, own)) {
-      if (ev) ea += WIN;
-      ev = !ev;
-      ej = ea;
-    }
-    id = page_of();
+    cp_async_commit();
   };
-  for (uint32_t i = 0; i < min(NST, total); i++) emit();
+  for (uint32_t i = 0; i < NST; i++) emit();
 
   // ---------------- the rows
   if (tid < kRows) {
@@ -560,22 +571,24 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
 
   const uint32_t lo_last = s_lo[nr - 1u], hi_first = s_hi[0];  // every row sees [lo_last, hi_first)
   const uint32_t ra = 2u * qt, rb = ra + 1u;                   // the rows of this lane's columns
-  uint32_t cs_ = 0, cp_ = 0;                                   // the next stage and its parity
+  uint32_t cst = 0;                                            // the next stage
   bool ok = true;
-  auto stage_in = [&](int code) {
-    if (ok) ok = wait_for(&bars[cs_], cp_, A.err, code);
+  auto stage_in = [&]() {  // all but the last NST - 1 groups are here
+    if (NST == 1u) cp_async_wait<0>();
+    else if (NST == 2u) cp_async_wait<1>();
+    else cp_async_wait<3>();
     __syncwarp();
-    return ring + cs_ * STB;
+    return ring + cst * STB;
   };
   auto stage_out = [&]() {
     __syncwarp();
-    if (++cs_ == NST) cs_ = 0, cp_ ^= 1u;
-    if (eq < total) emit();
+    if (++cst == NST) cst = 0;
+    emit();
   };
   // the scores of block t into the window's slot; the running maxima of the keys the rows ra and rb see
   uint32_t mxa = 0x80008000u, mxb = 0x80008000u;
   auto scores = [&](uint32_t t, uint32_t slot) {
-    const uint8_t* const st = stage_in(302);
+    const uint8_t* const st = stage_in();
     uint32_t* const d = S + slot * rcap * PW;
     const bool whole = t * KS >= lo_last && (t + 1u) * KS <= hi_first;
 #pragma unroll
@@ -702,9 +715,9 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
     o.sh = min(o.cs, 40u) - 9u;
     return o;
   };
-  auto e_of = [&](const Row& o, uint32_t x, uint32_t t, uint32_t& e0, uint32_t& e1) {
+  auto e_of = [&](auto narrow, const Row& o, uint32_t x, uint32_t t, uint32_t& e0, uint32_t& e1) {
     const uint32_t d0 = o.m0 - (x << 16), d1 = o.m0 - (x & 0xFFFF0000u);
-    if (o.cs >= 9u) {
+    if constexpr (decltype(narrow)::value) {
       const uint32_t t0 = __umulhi(d0, o.cm8) >> o.sh, t1 = __umulhi(d1, o.cm8) >> o.sh;
       e0 = shr_clamp((uint32_t)*(const uint16_t*)((const uint8_t*)tab + (t0 & 0x1FFEu)) + 1u, t0 >> 13);
       e1 = shr_clamp((uint32_t)*(const uint16_t*)((const uint8_t*)tab + (t1 & 0x1FFEu)) + 1u, t1 >> 13);
@@ -714,30 +727,33 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
     }
     if (t * KS < lo_last || (t + 1u) * KS > hi_first) {  // (alike over the warp)
       const uint32_t k0 = t * KS + word_key, k1 = k0 + 8u;
-      if (k0 < o.klo || k0 >= o.khi) e0 = 0;
-      if (k1 < o.klo || k1 >= o.khi) e1 = 0;
+      e0 = k0 >= o.klo && k0 < o.khi ? e0 : 0u;
+      e1 = k1 >= o.klo && k1 < o.khi ? e1 : 0u;
     }
   };
   // pass 2: e of blocks [a, z) in place (or only the sums)
   auto e_pass = [&](uint32_t a, uint32_t z, bool keep) {
 #pragma unroll 1
-    for (uint32_t r0_ = 0; r0_ < nr; r0_ += RSTEP) {
-      const uint32_t r = r0_ + rh;
+    for (uint32_t q = 0; q < nr; q += RSTEP) {
+      const uint32_t r = min(q + rh, nr - 1u);
+      const bool mine = q + rh < nr;
+      const Row o = row_of(r);
       unsigned long long sum = 0;
-      if (r < nr) {
-        const Row o = row_of(r);
+      auto go = [&](auto narrow) {
         uint32_t* p = S + score_word<PW>(r, rl);
 #pragma unroll 2
         for (uint32_t j = a; j < z; j++, p += rcap * PW) {
           uint32_t e0, e1;
-          e_of(o, *p, first + j * kWarps, e0, e1);
+          e_of(narrow, o, *p, first + j * kWarps, e0, e1);
           sum += e0 + e1;
-          if (keep) *p = pack_u16(e0, e1);
+          if (keep && mine) *p = pack_u16(e0, e1);
         }
-      }
+      };
+      if (__all_sync(0xffffffffu, o.cs >= 9u)) go(std::true_type());
+      else go(std::false_type());
 #pragma unroll
       for (int o = PW / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (rl == 0 && r < nr) s_ws[warp][r] += sum;
+      if (rl == 0 && mine) s_ws[warp][r] += sum;
     }
   };
   if (!again) {
@@ -769,26 +785,36 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   }
   __syncthreads();
 
-  // pass 3: P of blocks [a, z) in place, then P.V
+  // pass 3: P of blocks [a, z) in place (in windows from the scores), then P.V
   auto p_pass = [&](uint32_t a, uint32_t z) {
 #pragma unroll 1
     for (uint32_t r = rh; r < nr; r += RSTEP) {
       uint32_t* p = S + score_word<PW>(r, rl);
       const uint32_t fp = s_fp[r], R = s_R[r];
-      const bool fast = fp >= 8u && fp <= 15u;  // P is the high word of e R 2^(f_p - 8) + 2^31
-      const uint32_t Rp = fast ? R << (fp - 8u) : R;
-      const Row o = row_of(r);
-#pragma unroll 2
-      for (uint32_t j = a; j < z; j++, p += rcap * PW) {
-        const uint32_t x = *p, u0 = x & 0xFFFFu, u1 = x >> 16;
-        uint32_t e0 = u0 + ((u0 + 1u) >> 16), e1 = u1 + ((u1 + 1u) >> 16);
-        if (again) e_of(o, x, first + j * kWarps, e0, e1);
-        if (fast) {
-          e0 = (uint32_t)(((uint64_t)e0 * Rp + (1ull << 31)) >> 32);
-          e1 = (uint32_t)(((uint64_t)e1 * Rp + (1ull << 31)) >> 32);
-          *p = pack_s16(e0, e1);
-        } else {
-          *p = smx_p(e0, R, fp) | smx_p(e1, R, fp) << 16;
+      if (again) {
+        const Row o = row_of(r);
+        uint32_t* v = p;
+#pragma unroll 1
+        for (uint32_t j = a; j < z; j++, v += rcap * PW) {
+          uint32_t e0, e1;
+          if (o.cs >= 9u) e_of(std::true_type(), o, *v, first + j * kWarps, e0, e1);
+          else e_of(std::false_type(), o, *v, first + j * kWarps, e0, e1);
+          *v = pack_u16(e0, e1);
+        }
+      }
+      if (fp >= 8u && fp <= 15u) {  // the high word of e R 2^(f_p - 8) + 2^31
+        const uint32_t Rp = R << (fp - 8u);
+#pragma unroll 4
+        for (uint32_t j = a; j < z; j++, p += rcap * PW) {
+          const uint32_t x = *p, u0 = x & 0xFFFFu, u1 = x >> 16;
+          const uint32_t e0 = u0 + ((u0 + 1u) >> 16), e1 = u1 + ((u1 + 1u) >> 16);
+          *p = pack_s16((uint32_t)(((uint64_t)e0 * Rp + (1ull << 31)) >> 32), (uint32_t)(((uint64_t)e1 * Rp + (1ull << 31)) >> 32));
+        }
+      } else {
+#pragma unroll 1
+        for (uint32_t j = a; j < z; j++, p += rcap * PW) {
+          const uint32_t x = *p;
+          *p = smx_p(e_unpack(x & 0xFFFFu), R, fp) | smx_p(e_unpack(x >> 16), R, fp) << 16;
         }
       }
     }
@@ -804,7 +830,7 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   const bool turn = RB == 64 && (qt & 1u);
   const uint32_t lowsel = turn ? 0x2064u : 0x6420u, highsel = turn ? 0x3175u : 0x7531u;
   auto values = [&](uint32_t slot) {
-    const uint8_t* const st = stage_in(304);
+    const uint8_t* const st = stage_in();
     const uint32_t* const pr = S + slot * rcap * PW;
 #pragma unroll(HD <= 64 ? KS / 32 : 1)
     for (uint32_t k32 = 0; k32 < KS / 32; k32++) {
@@ -947,7 +973,7 @@ int launch_split(SplitArgs A, uint32_t tiles, cudaStream_t st) {
   uint32_t stages = 1;
   const uint32_t most = (room - kWarps * Sh::STB) / block;
   A.win = need < most ? need : most;
-  while (stages < 4u && A.win * block + (stages + 1u) * kWarps * Sh::STB <= room) stages++;
+  while (stages < 4u && A.win * block + 2u * stages * kWarps * Sh::STB <= room) stages *= 2u;  // 1, 2 or 4
   A.stages = stages;
   const size_t smem = kWarps * stages * Sh::STB + (size_t)A.win * block + fixed;
   auto kern = paged_attn_split_kernel<HD, BITS>;

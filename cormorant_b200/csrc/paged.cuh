@@ -150,13 +150,14 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* er
   return true;
 }
 
-// ---------------------------------------------------------------- bulk copies and clusters
-__device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   sm100::smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
-               : "memory");
+// ---------------------------------------------------------------- copies and clusters
+// 16 bytes, the first n of them from memory (n = 0: zeros)
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, uint32_t n) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sm100::smem_u32(dst)), "l"(src), "r"(n) : "memory");
 }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
