@@ -398,10 +398,9 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__
 // nothing but the maxima, the sums and the output meets.  Warp-level MMAs with the
 // keys, then the output's dimensions, as the 16 rows of an MMA and the query rows as
 // its 8 columns: a decoded token's group of heads is far below the 128 rows of a
-// tcgen05 tile, and the copies are to bound the kernel.  The contraction over HD
-// takes the dimensions in the order in which a lane's 16-byte pieces hold them (q
-// alike), the one over the keys in the order in which the scores' words hold them
-// (word i of 16 keys: keys i and i + 8); V's bytes are transposed 4 x 4 in registers.
+// tcgen05 tile, and the copies are to bound the kernel.  The contraction over the
+// keys takes them in the order in which the scores' words hold them (word i of 16
+// keys: keys i and i + 8); V's rows are transposed on the way to the registers.
 constexpr uint32_t kRows = 8;     // rows of a tile
 constexpr uint32_t kWarps = 8;
 constexpr uint32_t kMaxCluster = 8;
@@ -420,12 +419,21 @@ struct SplitShape {
   static constexpr uint32_t KS = RB <= 64 ? 64 : 32;          // keys of a block (a stage)
   static constexpr uint32_t STB = KS * RB + (BITS == 8 ? 128u : 0u);  // a stage (its shifts last)
   static constexpr uint32_t NKS = HD < 32 ? 1 : HD / 32;      // MMA steps of a score
-  static constexpr uint32_t CH = HD < 32 ? 1 : HD / 32;       // chunks of 32 (HD 16: 16) dimensions
   static constexpr uint32_t MT = HD / 16;                     // 16-dimension tiles of the output
   static constexpr uint32_t PW = KS / 2;                      // words of a row's scores in a block
   static constexpr uint32_t OCC = HD <= 64 ? 3 : (HD == 128 ? 2 : 1);  // CTAs an SM that the registers allow
 };
 
+// A stage's rows, 16-byte pieces in another order by the row (byte offsets ^ this), so
+// that eight keys' pieces of one place, keys 0 .. 7 or 0 .. 3 and 8 .. 11, meet no bank
+// twice; linear in the row's bits
+template <uint32_t RB>
+__host__ __device__ constexpr uint32_t stage_swizzle(uint32_t row) {
+  return RB == 16 ? 0u
+                  : (RB == 32 ? 16u * (((row >> 2) ^ (row >> 3)) & 1u)
+                              : (RB == 64 ? 16u * (((row >> 1) & 3u) ^ (2u * ((row >> 3) & 1u)))
+                                          : 16u * ((row & 7u) ^ (4u * ((row >> 3) & 1u)))));
+}
 // word i of row r's scores in a block: groups of 8 words trade places by the row, so that
 // four rows' reads meet no bank twice
 template <uint32_t PW>
@@ -497,8 +505,10 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
         const uint32_t n = pg < 0 ? 0u : 16u;
         const uint64_t line = ((uint64_t)(uint32_t)max(pg, 0) * c.KV + g) * c.page + in0;
         const uint8_t* const src = rows + line * RB + lane * 16u;
+        const uint32_t to = (lane * 16u) ^ stage_swizzle<RB>(lane * 16u / RB);
 #pragma unroll
-        for (uint32_t i = 0; i < KS * RB / 512u; i++) cp_async16(st + lane * 16u + i * 512u, src + i * 512u, n);
+        for (uint32_t i = 0; i < KS * RB / 512u; i++)
+          cp_async16(st + (to ^ stage_swizzle<RB>(i * 512u / RB)) + i * 512u, src + i * 512u, n);
         if (BITS == 8 && lane < KS / 16u) cp_async16(st + KS * RB + lane * 16u, (ev ? c.vs : c.ks) + line + lane * 16u, n);
       } else {
 #pragma unroll 1
@@ -506,7 +516,7 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
           const uint32_t row = i / RB;
           const int32_t pg = __shfl_sync(0xffffffffu, id, row / sub);
           const uint64_t line = ((uint64_t)(uint32_t)max(pg, 0) * c.KV + g) * c.page + row % sub;
-          cp_async16(st + i, rows + line * RB + i % RB, pg < 0 ? 0u : 16u);
+          cp_async16(st + (i ^ stage_swizzle<RB>(row)), rows + line * RB + i % RB, pg < 0 ? 0u : 16u);
         }
         if (BITS == 8) {
           const int32_t pg = __shfl_sync(0xffffffffu, id, (lane * 16u / sub) & 31u);
@@ -550,9 +560,7 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   for (uint32_t ks = 0; ks < NKS; ks++)
 #pragma unroll
     for (uint32_t half = 0; half < 2; half++) {
-      // word v of the lane's pieces: dimensions 64 (v / 4) + 16 t + 4 (v % 4) (rows of 64 up)
-      const uint32_t v = 2u * ks + half;
-      const uint32_t dim = HD >= 64 ? 64u * (v >> 2) + 16u * qt + 4u * (v & 3u) : (HD == 32 ? 8u * qt + 4u * half : 4u * qt);
+      const uint32_t dim = 32u * ks + 16u * half + 4u * qt;
       bh[ks][half] = bl[ks][half] = 0;
       if (qn < nr && (HD > 16 || half == 0)) {
         const uint32_t rr = r0 + qn;
@@ -585,17 +593,31 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
     if (++cst == NST) cst = 0;
     emit();
   };
+  // a lane's row of an MMA's 16 x 32 operand: key (lane mod 16), the piece of 16 bytes lane / 16
+  const uint32_t krow = lane & 15u, kx = (HD >= 32 ? 16u * (lane >> 4) : 0u) ^ stage_swizzle<RB>(lane & 15u);
+  // of a transposed one's (32 keys as the scores' words hold them): key vrow
+  const uint32_t vr16 = 2u * ((lane >> 2) & 3u) + ((lane >> 1) & 1u) + 8u * (lane & 1u);
+  const uint32_t vrow = 16u * (lane >> 4) + vr16, vx = stage_swizzle<RB>(vr16);
   // the scores of block t into the window's slot; the running maxima of the keys the rows ra and rb see
   uint32_t mxa = 0x80008000u, mxb = 0x80008000u;
   auto scores = [&](uint32_t t, uint32_t slot) {
     const uint8_t* const st = stage_in();
+    const uint32_t st_a = sm100::smem_u32(st) + krow * RB;
     uint32_t* const d = S + slot * rcap * PW;
     const bool whole = t * KS >= lo_last && (t + 1u) * KS <= hi_first;
 #pragma unroll
     for (uint32_t k16 = 0; k16 < KS / 16; k16++) {
-      const uint8_t* const row = st + (16u * k16 + qn) * RB;
-      uint32_t hh[4], mid[4], ll[4];
-      auto step = [&](uint32_t ks, const uint32_t (&h)[4], const uint32_t (&l)[4]) {
+      const uint32_t row = st_a + 16u * k16 * RB;
+      uint32_t hh[4], mid[4], ll[4], h[4] = {0, 0, 0, 0}, l[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (uint32_t ks = 0; ks < NKS; ks++) {
+        if constexpr (HD >= 32) {
+          ldmatrix_x4(h, row + ((32u * ks) ^ kx));
+          if (BITS == 16) ldmatrix_x4(l, row + ((HD + 32u * ks) ^ kx));
+        } else {
+          ldmatrix_x2(h, row + kx);
+          if (BITS == 16) ldmatrix_x2(l, row + (HD ^ kx));
+        }
         if (ks == 0) {
           mma_ss_first(hh, h, bh[ks][0], bh[ks][1]);
           mma_su_first(mid, h, bl[ks][0], bl[ks][1]);
@@ -606,33 +628,6 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
           if (BITS == 16) mma_uu(ll, l, bl[ks][0], bl[ks][1]);
         }
         if (BITS == 16) mma_us(mid, l, bh[ks][0], bh[ks][1]);
-      };
-      if constexpr (HD >= 64) {
-#pragma unroll
-        for (uint32_t k = 0; k < HD / 64; k++) {
-          const uint8_t* const p = row + 64u * k + 16u * qt;
-          const uint4 h0 = *(const uint4*)p, h1 = *(const uint4*)(p + 8u * RB);
-          uint4 l0 = make_uint4(0, 0, 0, 0), l1 = l0;
-          if (BITS == 16) l0 = *(const uint4*)(p + HD), l1 = *(const uint4*)(p + 8u * RB + HD);
-          const uint32_t fh[2][4] = {{h0.x, h1.x, h0.y, h1.y}, {h0.z, h1.z, h0.w, h1.w}};
-          const uint32_t fl[2][4] = {{l0.x, l1.x, l0.y, l1.y}, {l0.z, l1.z, l0.w, l1.w}};
-          step(2u * k, fh[0], fl[0]);
-          step(2u * k + 1u, fh[1], fl[1]);
-        }
-      } else {
-        uint32_t h[4] = {0, 0, 0, 0}, l[4] = {0, 0, 0, 0};
-        if constexpr (HD == 32) {
-          const uint2 a0 = *(const uint2*)(row + 8u * qt), a1 = *(const uint2*)(row + 8u * RB + 8u * qt);
-          h[0] = a0.x, h[1] = a1.x, h[2] = a0.y, h[3] = a1.y;
-          if (BITS == 16) {
-            const uint2 c0 = *(const uint2*)(row + HD + 8u * qt), c1 = *(const uint2*)(row + 8u * RB + HD + 8u * qt);
-            l[0] = c0.x, l[1] = c1.x, l[2] = c0.y, l[3] = c1.y;
-          }
-        } else {
-          h[0] = *(const uint32_t*)(row + 4u * qt), h[1] = *(const uint32_t*)(row + 8u * RB + 4u * qt);
-          if (BITS == 16) l[0] = *(const uint32_t*)(row + HD + 4u * qt), l[1] = *(const uint32_t*)(row + 8u * RB + HD + 4u * qt);
-        }
-        step(0, h, l);
       }
       // columns ra and rb of keys qn (sums 0, 1) and qn + 8 (2, 3)
       uint32_t y[4];
@@ -820,18 +815,20 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
     }
     __syncwarp();
   };
-  uint32_t acc[Sh::MT][4];
+  // the output's sums of weight 1, 2^8 and 2^16 apart, or (many dimensions) in one
+  constexpr bool APART = HD <= 32;
+  uint32_t acc[Sh::MT][4], acc1[APART ? Sh::MT : 1][4], acc2[APART ? Sh::MT : 1][4];
 #pragma unroll
   for (uint32_t j = 0; j < Sh::MT; j++)
 #pragma unroll
-    for (int x = 0; x < 4; x++) acc[j][x] = 0;
-  // rows of 64 bytes: odd quarters take each pair of keys in the other order, so that
-  // two quarters meet no bank twice
-  const bool turn = RB == 64 && (qt & 1u);
-  const uint32_t lowsel = turn ? 0x2064u : 0x6420u, highsel = turn ? 0x3175u : 0x7531u;
+    for (int x = 0; x < 4; x++) {
+      acc[j][x] = 0;
+      if (APART) acc1[j][x] = acc2[j][x] = 0;
+    }
   auto values = [&](uint32_t slot) {
     const uint8_t* const st = stage_in();
     const uint32_t* const pr = S + slot * rcap * PW;
+    const uint32_t st_a = sm100::smem_u32(st) + vrow * RB;
 #pragma unroll(HD <= 64 ? KS / 32 : 1)
     for (uint32_t k32 = 0; k32 < KS / 32; k32++) {
       uint32_t p0[2], p1[2], p2[2] = {0, 0};
@@ -840,67 +837,49 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
         uint2 v = make_uint2(0, 0);
         if (qn < nr) v = *(const uint2*)(pr + score_word<PW>(qn, 16u * k32 + 8u * h + 2u * qt));
         if (BITS == 16) {
-          p0[h] = __byte_perm(v.x, v.y, lowsel);
-          p1[h] = __byte_perm(v.x, v.y, highsel);
+          p0[h] = __byte_perm(v.x, v.y, 0x6420);
+          p1[h] = __byte_perm(v.x, v.y, 0x7531);
         } else {  // P << shift: 23 bits, three planes against the codes
           const uint8_t* const sp = st + KS * RB + 32u * k32 + 16u * h + 2u * qt;
           const uint32_t sa = *(const uint16_t*)sp, sb = *(const uint16_t*)(sp + 8);
-          const uint32_t ya = (v.x & 0xFFFFu) << (sa & 31u), yb = (v.x >> 16) << (sb & 31u);
-          const uint32_t yc = (v.y & 0xFFFFu) << ((sa >> 8) & 31u), yd = (v.y >> 16) << ((sb >> 8) & 31u);
-          const uint32_t y0 = turn ? yc : ya, y1 = turn ? yd : yb, y2 = turn ? ya : yc, y3 = turn ? yb : yd;
+          const uint32_t y0 = (v.x & 0xFFFFu) << (sa & 31u), y1 = (v.x >> 16) << (sb & 31u);
+          const uint32_t y2 = (v.y & 0xFFFFu) << ((sa >> 8) & 31u), y3 = (v.y >> 16) << ((sb >> 8) & 31u);
           const uint32_t f = __byte_perm(y0, y1, 0x5140), z = __byte_perm(y2, y3, 0x5140);
           p0[h] = __byte_perm(f, z, 0x5410);
           p1[h] = __byte_perm(f, z, 0x7632);
           p2[h] = __byte_perm(__byte_perm(y0, y1, 0x0062), __byte_perm(y2, y3, 0x0062), 0x5410);
         }
       }
-      // this lane's four keys of 16 in the words' order: base, base + 8, and their neighbours
-      const uint32_t base = 32u * k32 + 2u * qt + (turn ? 1u : 0u);
-      const int32_t step = turn ? -(int32_t)RB : (int32_t)RB;
 #pragma unroll
-      for (uint32_t ch = 0; ch < Sh::CH; ch++) {
-        uint32_t th[2][4], tl[2][4];
-#pragma unroll
-        for (uint32_t h = 0; h < 2; h++) {
-          const uint8_t* const v0 = st + (base + 16u * h) * RB + (HD >= 32 ? 32u * ch + 4u * qn : 2u * qn);
-          uint32_t x[4], y[4];
-#pragma unroll
-          for (uint32_t i = 0; i < 4; i++) {
-            const uint8_t* const q = v0 + (i & 1u) * 8u * RB + (int32_t)(i >> 1) * step;
-            if constexpr (HD >= 32) {
-              if (BITS == 16) {  // quarters alternate between the planes: two meet no bank twice
-                const uint32_t f0 = *(const uint32_t*)(q + ((qt & 1u) ? HD : 0)), f1 = *(const uint32_t*)(q + ((qt & 1u) ? 0 : HD));
-                x[i] = (qt & 1u) ? f1 : f0;
-                y[i] = (qt & 1u) ? f0 : f1;
-              } else {
-                x[i] = *(const uint32_t*)q;
-              }
-            } else {
-              x[i] = *(const uint16_t*)q;
-              if (BITS == 16) y[i] = *(const uint16_t*)(q + HD);
-            }
+      for (uint32_t j = 0; j < Sh::MT; j++) {
+        uint32_t ah[4], al[4];
+        ldmatrix_t8(ah, st_a + 32u * k32 * RB + ((16u * j) ^ vx));
+        if (BITS == 16) ldmatrix_t8(al, st_a + 32u * k32 * RB + ((HD + 16u * j) ^ vx));
+        if constexpr (APART) {
+          if (BITS == 16) {
+            mma_uu(acc[j], al, p0[0], p0[1]);
+            mma_su(acc1[j], ah, p0[0], p0[1]);
+            mma_uu(acc1[j], al, p1[0], p1[1]);
+            mma_su(acc2[j], ah, p1[0], p1[1]);
+          } else {
+            mma_su(acc[j], ah, p0[0], p0[1]);
+            mma_su(acc1[j], ah, p1[0], p1[1]);
+            mma_su(acc2[j], ah, p2[0], p2[1]);
           }
-          transpose4(x[0], x[1], x[2], x[3], th[h]);
-          if (BITS == 16) transpose4(y[0], y[1], y[2], y[3], tl[h]);
-        }
-#pragma unroll
-        for (uint32_t jj = 0; jj < (HD >= 32 ? 2 : 1); jj++) {
-          uint32_t (&o)[4] = acc[HD >= 32 ? 2u * ch + jj : 0u];
-          const uint32_t ah[4] = {th[0][2 * jj], th[0][2 * jj + 1], th[1][2 * jj], th[1][2 * jj + 1]};
+        } else {
           uint32_t a1[4], a2[4];
           if (BITS == 16) {
-            const uint32_t al[4] = {tl[0][2 * jj], tl[0][2 * jj + 1], tl[1][2 * jj], tl[1][2 * jj + 1]};
-            mma_uu(o, al, p0[0], p0[1]);
+            mma_uu(acc[j], al, p0[0], p0[1]);
             mma_su_first(a1, ah, p0[0], p0[1]);
             mma_uu(a1, al, p1[0], p1[1]);
             mma_su_first(a2, ah, p1[0], p1[1]);
           } else {
-            mma_su(o, ah, p0[0], p0[1]);
+            mma_su(acc[j], ah, p0[0], p0[1]);
             mma_su_first(a1, ah, p1[0], p1[1]);
             mma_su_first(a2, ah, p2[0], p2[1]);
           }
 #pragma unroll
-          for (int x = 0; x < 4; x++) o[x] += (a1[x] << 8) + (a2[x] << 16);
+          for (int x = 0; x < 4; x++) acc[j][x] += (a1[x] << 8) + (a2[x] << 16);
         }
       }
     }
@@ -921,10 +900,12 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   uint32_t* const part = (uint32_t*)ring;  // [row][HD]
 #pragma unroll
   for (uint32_t j = 0; j < Sh::MT; j++) {
-    // sums 0, 1: dimension 32 ch + 4 qn + 2 jj (HD 16: 2 qn) of rows ra, rb; 2, 3: the next
-    const uint32_t dim = HD >= 32 ? 32u * (j >> 1) + 4u * qn + 2u * (j & 1u) : 2u * qn;
-    if (ra < nr) *(uint2*)(part + ra * HD + dim) = make_uint2(acc[j][0], acc[j][2]);
-    if (rb < nr) *(uint2*)(part + rb * HD + dim) = make_uint2(acc[j][1], acc[j][3]);
+    // sums 0, 1: dimension 16 j + qn of rows ra, rb; 2, 3: 8 dimensions on
+    if (APART)
+#pragma unroll
+      for (int x = 0; x < 4; x++) acc[j][x] += (acc1[j][x] << 8) + (acc2[j][x] << 16);
+    if (ra < nr) part[ra * HD + 16u * j + qn] = acc[j][0], part[ra * HD + 16u * j + qn + 8u] = acc[j][2];
+    if (rb < nr) part[rb * HD + 16u * j + qn] = acc[j][1], part[rb * HD + 16u * j + qn + 8u] = acc[j][3];
   }
   __syncthreads();
   auto put = [&](uint32_t i, uint32_t v) {

@@ -67,16 +67,6 @@ __device__ __forceinline__ uint32_t smx_r(unsigned long long S) {
   return r;
 }
 
-// four 4-byte rows -> four words of one byte column each
-__device__ __forceinline__ void transpose4(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t (&o)[4]) {
-  const uint32_t a = __byte_perm(w0, w1, 0x5140), b = __byte_perm(w2, w3, 0x5140);
-  const uint32_t c = __byte_perm(w0, w1, 0x7362), d = __byte_perm(w2, w3, 0x7362);
-  o[0] = __byte_perm(a, b, 0x5410);
-  o[1] = __byte_perm(a, b, 0x7632);
-  o[2] = __byte_perm(c, d, 0x5410);
-  o[3] = __byte_perm(c, d, 0x7632);
-}
-
 // an exact sum modulo 2^32 as the kernels round it: floor / 2^8, saturated
 __device__ __forceinline__ int32_t out16(uint32_t acc) {
   const int32_t y = (int32_t)acc >> 8;
@@ -123,6 +113,26 @@ CORM_MMA_I8(mma_su, "s8", "u8")
 CORM_MMA_I8(mma_us, "u8", "s8")
 CORM_MMA_I8(mma_uu, "u8", "u8")
 #undef CORM_MMA_I8
+
+// 8-bit operand fragments from shared memory, a row of 16 bytes a lane: a 16 x 32 (or
+// 16 x 16) A operand as it lies, and one of 32 rows whose columns become A's rows (two
+// 16 x 16 byte matrices transposed: lane l gets column l / 4, then l / 4 + 8, of rows
+// 4 (l mod 4) .. + 3, then of those 16 on)
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x2(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_t8(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
 
 // ---------------------------------------------------------------- waits
 // Bounded like sm100::mbar_wait; each look may suspend the warp for up to 20 us, so
