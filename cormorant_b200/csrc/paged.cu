@@ -3,6 +3,7 @@
 // of few rows a sequence.
 #include "paged.cuh"
 
+#include <atomic>
 #include <type_traits>
 
 #include "gemm_i8x4.h"
@@ -404,13 +405,12 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__
 constexpr uint32_t kRows = 8;     // rows of a tile
 constexpr uint32_t kWarps = 8;
 constexpr uint32_t kMaxCluster = 8;
-constexpr uint32_t kSplitRows = 32;  // rows of a sequence and KV head up to which this form runs
 
 struct SplitArgs {
   corm_llm_paged_attn_desc d;
   const int32_t* tab;
   int* err;
-  uint32_t G, X, stages, win, rcap;  // stages of a warp; win: blocks of a warp's window; rcap: rows held
+  uint32_t G, Ginv, X, stages, win, rcap;  // Ginv: ceil(2^16 / G); stages of a warp; win: blocks of a warp's window; rcap: rows held
 };
 
 template <int HD, int BITS>
@@ -447,17 +447,25 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   constexpr uint32_t RB = Sh::RB, KS = Sh::KS, STB = Sh::STB, NKS = Sh::NKS, PW = Sh::PW;
   extern __shared__ __align__(128) uint8_t pa_sm[];
   __shared__ uint64_t cbar;
-  __shared__ int32_t s_wmax[kWarps][kRows], s_m[kRows], s_gm[kRows];
+  __shared__ int32_t s_wmax[kWarps][kRows], s_m[kRows];
   __shared__ unsigned long long s_ws[kWarps][kRows], s_s[kRows];
-  __shared__ uint32_t s_R[kRows], s_lo[kRows], s_hi[kRows], s_cm[kRows], s_cs[kRows], s_fp[kRows];
+  __shared__ uint32_t s_lo[kRows], s_hi[kRows], s_cm[kRows], s_cs[kRows], s_fp[kRows];
   const corm_paged_cache& c = A.d.c;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-  const uint32_t X = A.X, tile = blockIdx.x / X, rank = blockIdx.x % X, g = blockIdx.y, b = blockIdx.z, G = A.G;
+  const uint32_t X = A.X, g = blockIdx.y, b = blockIdx.z, G = A.G;
+  const uint32_t tile = X == 1u ? blockIdx.x : blockIdx.x / X, rank = X == 1u ? 0u : blockIdx.x % X;
   const uint32_t NST = A.stages, rcap = A.rcap, WIN = A.win;
   uint8_t* const ring = pa_sm + warp * NST * STB;                                          // this warp's stages
   uint32_t* const S = (uint32_t*)(pa_sm + kWarps * NST * STB) + warp * WIN * rcap * PW;  // and scores: [block][row][PW]
   uint16_t* const tab = (uint16_t*)(pa_sm + kWarps * (NST * STB + WIN * rcap * PW * 4u));
   uint32_t* const s_O = (uint32_t*)(tab + 4096);
+  // before the wait for the kernel in front: the table, which no kernel writes
+#pragma unroll
+  for (uint32_t i = 0; i < 4; i++) {
+    const int4 v = ((const int4*)A.tab)[tid + 256u * i];
+    ((uint2*)tab)[tid + 256u * i] = make_uint2(pack16(v.x - 1, v.y - 1), pack16(v.z - 1, v.w - 1));
+  }
+  if (tid < kWarps * kRows) ((unsigned long long*)s_ws)[tid] = 0;
   if (tid == 0) {
     sm100::mbar_init(&cbar, X);
     sm100::fence_mbar_init();
@@ -468,7 +476,10 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   const uint32_t n = min(sq.n, A.d.max_q), r0 = tile * kRows;
   if ((uint64_t)r0 >= (uint64_t)n * G) return;  // the cluster's CTAs alike
   const uint32_t nr = min(kRows, n * G - r0);
-  const uint32_t i0 = r0 / G, i1 = (r0 + nr - 1u) / G;
+  // row r0 + d (d < 8) is token i0 + t, head o of the group: t = (o0 + d) / G, exact by Ginv
+  const uint32_t i0 = tile ? r0 / G : 0u, o0 = r0 - i0 * G;
+  auto token = [&](uint32_t d) { return ((o0 + d) * A.Ginv) >> 16; };
+  const uint32_t i1 = i0 + token(nr - 1u);
   // the keys some row of the tile sees: [lo, hi), in blocks from lo rounded down
   const uint32_t hi = min(sq.pos + i1 + 1u, sq.cap);
   const uint32_t w = A.d.window;
@@ -479,29 +490,54 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   const uint32_t own = first < end ? (end - first + kWarps - 1u) / kWarps : 0u;  // blocks first, first + 8, ...
   const bool again = own > WIN;  // more than a window (a warp's own affair)
 
+  const uint32_t qn = lane >> 2, qt = lane & 3u;
+  uint2 qw[NKS][2];  // q of row qn: four dimensions of each operand word
+  {
+    const uint32_t d = min(qn, nr - 1u), t = token(d);
+    const int16_t* const q = A.d.q + (uint64_t)(sq.lo + i0 + t) * A.d.ldq + (uint64_t)(g * G + o0 + d - t * G) * HD + 4u * qt;
+    const bool q8 = (((uintptr_t)A.d.q | (A.d.ldq * 2u)) & 7u) == 0;
+#pragma unroll
+    for (uint32_t ks = 0; ks < NKS; ks++)
+#pragma unroll
+      for (uint32_t half = 0; half < 2; half++) {
+        qw[ks][half] = make_uint2(0, 0);
+        if (qn < nr && (HD > 16 || half == 0)) {
+          const int16_t* const p = q + 32u * ks + 16u * half;
+          qw[ks][half] = q8 ? *(const uint2*)p : make_uint2(pack16(p[0], p[1]), pack16(p[2], p[3]));
+        }
+      }
+  }
   // ---------------- the copies: K's blocks, then V's; in windows K's blocks for each of
   // the first two passes, then each window's K and V
-  const uint32_t sub = min(c.page, KS), pieces = KS / sub, psh = 31u - __clz(c.page);
+  const uint32_t sub = min(c.page, KS), psh = 31u - __clz(c.page), ssh = 31u - __clz(sub);
+  const uint32_t pieces = KS >> ssh, pcs = 31u - __clz(pieces);  // pieces of a block
   const int32_t* const tb = c.table + (uint64_t)b * c.table_width;
   const uint32_t total = again ? 4u * own : 2u * own;
-  uint32_t eq = 0, ej = 0, ea = 0, ep = 0, es = 0;  // the next copy's number, block, window, pass and stage
+  uint32_t eq = 0, ej = 0, ea = 0, ep = 0, es = 0;  // the next copy's number, block, window and pass and stage
   bool ev = false;                                  // of V
-  auto page_of = [&]() -> int32_t {                 // the page of piece `lane` of the next copy, below 0: none
-    const uint32_t key = (first + ej * kWarps) * KS + lane * sub;
+  const uint32_t held = 32u >> pcs;                 // blocks whose pages the lanes hold, a piece each: from block ib on
+  uint32_t ib = 0;
+  auto pages_from = [&](uint32_t j) -> int32_t {  // below 0: no page
+    const uint32_t bj = j + (lane >> pcs), key = (first + bj * kWarps) * KS + ((lane & (pieces - 1u)) << ssh);
     int32_t id = -1;
-    if (eq < total && lane < pieces && key < hi) id = tb[key >> psh];
+    if (bj < own && key < hi) id = tb[key >> psh];
     return (uint32_t)id < c.pages ? id : -1;
   };
-  int32_t id = page_of();
+  int32_t ids = pages_from(0);
   // one group of asynchronous copies, 16 bytes a lane (empty after the last block);
   // pieces without a page are zeros
   auto emit = [&]() {
     if (eq < total) {
+      if (ej - ib >= held) {
+        ib = ej & ~(held - 1u);
+        ids = pages_from(ib);
+      }
+      const uint32_t at = (ej - ib) * pieces;
       uint8_t* const st = ring + es * STB;
       const uint8_t* const rows = ev ? (const uint8_t*)c.vc : (const uint8_t*)c.kc;
       const uint32_t in0 = ((first + ej * kWarps) * KS) & (c.page - 1u);  // a block in a page: its first row
       if (pieces == 1u) {
-        const int32_t pg = __shfl_sync(0xffffffffu, id, 0);
+        const int32_t pg = __shfl_sync(0xffffffffu, ids, at);
         const uint32_t n = pg < 0 ? 0u : 16u;
         const uint64_t line = ((uint64_t)(uint32_t)max(pg, 0) * c.KV + g) * c.page + in0;
         const uint8_t* const src = rows + line * RB + lane * 16u;
@@ -514,13 +550,13 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
 #pragma unroll 1
         for (uint32_t i = lane * 16u; i < KS * RB; i += 512u) {
           const uint32_t row = i / RB;
-          const int32_t pg = __shfl_sync(0xffffffffu, id, row / sub);
-          const uint64_t line = ((uint64_t)(uint32_t)max(pg, 0) * c.KV + g) * c.page + row % sub;
+          const int32_t pg = __shfl_sync(0xffffffffu, ids, at + (row >> ssh));
+          const uint64_t line = ((uint64_t)(uint32_t)max(pg, 0) * c.KV + g) * c.page + (row & (sub - 1u));
           cp_async16(st + (i ^ stage_swizzle<RB>(row)), rows + line * RB + i % RB, pg < 0 ? 0u : 16u);
         }
         if (BITS == 8) {
-          const int32_t pg = __shfl_sync(0xffffffffu, id, (lane * 16u / sub) & 31u);
-          const uint64_t line = ((uint64_t)(uint32_t)max(pg, 0) * c.KV + g) * c.page + lane * 16u % sub;
+          const int32_t pg = __shfl_sync(0xffffffffu, ids, (at + (lane * 16u >> ssh)) & 31u);
+          const uint64_t line = ((uint64_t)(uint32_t)max(pg, 0) * c.KV + g) * c.page + (lane * 16u & (sub - 1u));
           if (lane < KS / 16u) cp_async16(st + KS * RB + lane * 16u, (ev ? c.vs : c.ks) + line, pg < 0 ? 0u : 16u);
         }
       }
@@ -536,7 +572,6 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
         ev = !ev;
         ej = ea;
       }
-      id = page_of();
     }
     cp_async_commit();
   };
@@ -544,8 +579,8 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
 
   // ---------------- the rows
   if (tid < kRows) {
-    const uint32_t rr = r0 + min(tid, nr - 1u), i = rr / G, h = g * G + rr % G;
-    const uint32_t p = sq.pos + i;
+    const uint32_t d = min(tid, nr - 1u), t = token(d), h = g * G + o0 + d - t * G;
+    const uint32_t p = sq.pos + i0 + t;
     s_hi[tid] = min(p + 1u, sq.cap);
     s_lo[tid] = (w && p + 1u > w) ? p + 1u - w : 0u;
     s_cm[tid] = A.d.smx[2u * h];
@@ -553,27 +588,14 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
     s_cs[tid] = cfg & 63u;
     s_fp[tid] = (cfg >> 8) & 31u;
   }
-  if (tid < kWarps * kRows) ((unsigned long long*)s_ws)[tid] = 0;
-  const uint32_t qn = lane >> 2, qt = lane & 3u;
-  uint32_t bh[NKS][2], bl[NKS][2];  // q's planes: row qn
+  uint32_t bh[NKS][2], bl[NKS][2];  // q's planes
 #pragma unroll
   for (uint32_t ks = 0; ks < NKS; ks++)
 #pragma unroll
     for (uint32_t half = 0; half < 2; half++) {
-      const uint32_t dim = 32u * ks + 16u * half + 4u * qt;
-      bh[ks][half] = bl[ks][half] = 0;
-      if (qn < nr && (HD > 16 || half == 0)) {
-        const uint32_t rr = r0 + qn;
-        const int16_t* q = A.d.q + (uint64_t)(sq.lo + rr / G) * A.d.ldq + (uint64_t)(g * G + rr % G) * HD + dim;
-        const uint32_t x0 = pack16(q[0], q[1]), x1 = pack16(q[2], q[3]);
-        bh[ks][half] = __byte_perm(x0, x1, 0x7531);
-        bl[ks][half] = __byte_perm(x0, x1, 0x6420);
-      }
+      bh[ks][half] = __byte_perm(qw[ks][half].x, qw[ks][half].y, 0x7531);
+      bl[ks][half] = __byte_perm(qw[ks][half].x, qw[ks][half].y, 0x6420);
     }
-  for (uint32_t i = tid; i < 1024u; i += 256u) {
-    const int4 v = ((const int4*)A.tab)[i];
-    ((uint2*)tab)[i] = make_uint2(pack16(v.x - 1, v.y - 1), pack16(v.z - 1, v.w - 1));
-  }
   if (X > 1) cluster_sync();
   else __syncthreads();
 
@@ -678,20 +700,27 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
     s_wmax[warp][rb] = max((int32_t)(int16_t)(mxb & 0xFFFFu), (int32_t)mxb >> 16);
   }
   __syncthreads();
-  if (tid < kRows) {
-    int32_t m = s_wmax[0][tid];
-    for (uint32_t i = 1; i < kWarps; i++) m = max(m, s_wmax[i][tid]);
-    s_m[tid] = m;
+  if (X > 1) {
+    if (tid < kRows) {
+      int32_t m = s_wmax[0][tid];
+#pragma unroll
+      for (uint32_t i = 1; i < kWarps; i++) m = max(m, s_wmax[i][tid]);
+      s_m[tid] = m;
+    }
+    cluster_meet();
   }
-  if (X > 1) cluster_meet();
-  if (tid < kRows) {
-    int32_t m = s_m[tid];
-    if (X > 1)
-      for (uint32_t i = 0; i < X; i++) m = max(m, (int32_t)cluster_ld32(cluster_addr(&s_m[tid], i)));
-    s_gm[tid] = m;
-  }
-  __syncthreads();
-
+  // the row's maximum over the CTA's warps, or the cluster's CTAs
+  auto row_max = [&](uint32_t r) {
+    int32_t m = INT32_MIN;
+    if (X == 1) {
+#pragma unroll
+      for (uint32_t i = 0; i < kWarps; i++) m = max(m, s_wmax[i][r]);
+    } else {
+      for (uint32_t i = 0; i < X; i++) m = max(m, (int32_t)cluster_ld32(cluster_addr(&s_m[r], i)));
+    }
+    return m;
+  };
+  const int32_t mx = row_max(lane & 7u);
   // a word (two keys) a lane, PW lanes a row, the rows in turn
   const uint32_t rl = lane % PW, rh = lane / PW;
   constexpr uint32_t RSTEP = 32 / PW;
@@ -702,10 +731,10 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   struct Row {
     uint32_t cm, cs, klo, khi, m0, cm8, sh;
   };
-  auto row_of = [&](uint32_t r) {
+  auto row_of = [&](uint32_t r, uint32_t m0) {  // m0: the maximum at 2^16
     Row o;
     o.cm = s_cm[r], o.cs = s_cs[r], o.klo = s_lo[r], o.khi = s_hi[r];
-    o.m0 = (uint32_t)s_gm[r] << 16;
+    o.m0 = m0;
     o.cm8 = o.cs >= 40u ? 0u : (o.cm & 0xFFFFFFu) << 8;
     o.sh = min(o.cs, 40u) - 9u;
     return o;
@@ -732,11 +761,11 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
     for (uint32_t q = 0; q < nr; q += RSTEP) {
       const uint32_t r = min(q + rh, nr - 1u);
       const bool mine = q + rh < nr;
-      const Row o = row_of(r);
-      unsigned long long sum = 0;
+      const Row o = row_of(r, (uint32_t)__shfl_sync(0xffffffffu, mx, r) << 16);
+      uint32_t sum = 0;  // (of a window: below 2^32 over the row)
       auto go = [&](auto narrow) {
         uint32_t* p = S + score_word<PW>(r, rl);
-#pragma unroll 2
+#pragma unroll 4
         for (uint32_t j = a; j < z; j++, p += rcap * PW) {
           uint32_t e0, e1;
           e_of(narrow, o, *p, first + j * kWarps, e0, e1);
@@ -764,30 +793,37 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
     }
   }
   __syncthreads();
-  if (tid < kRows) {
-    unsigned long long sum = 0;
-    for (uint32_t i = 0; i < kWarps; i++) sum += s_ws[i][tid];
-    s_s[tid] = sum;
-  }
-  if (X > 1) cluster_meet();
-  if (tid < kRows) {
-    unsigned long long sum = s_s[tid];
-    if (X > 1) {
-      sum = 0;
-      for (uint32_t i = 0; i < X; i++) sum += cluster_ld64(cluster_addr(&s_s[tid], i));
+  if (X > 1) {
+    if (tid < kRows) {
+      unsigned long long sum = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < kWarps; i++) sum += s_ws[i][tid];
+      s_s[tid] = sum;
     }
-    s_R[tid] = smx_r(sum);
+    cluster_meet();
   }
-  __syncthreads();
+  auto row_r = [&](uint32_t r) {
+    unsigned long long sum = 0;
+    if (X == 1) {
+#pragma unroll
+      for (uint32_t i = 0; i < kWarps; i++) sum += s_ws[i][r];
+    } else {
+      for (uint32_t i = 0; i < X; i++) sum += cluster_ld64(cluster_addr(&s_s[r], i));
+    }
+    return smx_r(sum);
+  };
+  const uint32_t Rs = row_r(lane & 7u);
 
   // pass 3: P of blocks [a, z) in place (in windows from the scores), then P.V
   auto p_pass = [&](uint32_t a, uint32_t z) {
 #pragma unroll 1
-    for (uint32_t r = rh; r < nr; r += RSTEP) {
+    for (uint32_t q = 0; q < nr; q += RSTEP) {
+      const uint32_t r = min(q + rh, kRows - 1u), R = __shfl_sync(0xffffffffu, Rs, r), m0 = (uint32_t)__shfl_sync(0xffffffffu, mx, r) << 16;
+      if (r >= nr) continue;
       uint32_t* p = S + score_word<PW>(r, rl);
-      const uint32_t fp = s_fp[r], R = s_R[r];
+      const uint32_t fp = s_fp[r];
       if (again) {
-        const Row o = row_of(r);
+        const Row o = row_of(r, m0);
         uint32_t* v = p;
 #pragma unroll 1
         for (uint32_t j = a; j < z; j++, v += rcap * PW) {
@@ -909,8 +945,8 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   }
   __syncthreads();
   auto put = [&](uint32_t i, uint32_t v) {
-    const uint32_t rr = r0 + i / HD;
-    A.d.o[(uint64_t)(sq.lo + rr / G) * A.d.ldo + (uint64_t)(g * G + rr % G) * HD + i % HD] = (int16_t)out16(v);
+    const uint32_t d = i / HD, t = token(d);
+    A.d.o[(uint64_t)(sq.lo + i0 + t) * A.d.ldo + (uint64_t)(g * G + o0 + d - t * G) * HD + i % HD] = (int16_t)out16(v);
   };
   for (uint32_t i = tid; i < nr * HD; i += 256u) {
     uint32_t v = 0;
@@ -930,6 +966,38 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
   }
 }
 
+// dynamic shared memory of a CTA, occ of them an SM
+constexpr uint32_t split_smem(uint32_t occ) { return (occ == 3u ? 73u : (occ == 2u ? 111u : 222u)) * 1024u; }
+
+// how many clusters of X CTAs, d an SM, the current device holds at once (asked for once)
+template <int HD, int BITS>
+uint32_t resident_clusters(uint32_t X, uint32_t d) {
+  static std::atomic<int> known[16][kMaxCluster + 1][4];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 16)
+    if (const int n = known[dev][X][d].load(std::memory_order_relaxed)) return (uint32_t)n - 1u;
+  auto kern = paged_attn_split_kernel<HD, BITS>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(X * 1024u);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = split_smem(d);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = X;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  if (dev < 16) known[dev][X][d].store(n + 1, std::memory_order_relaxed);
+  return (uint32_t)n;
+}
+
 template <int HD, int BITS>
 int launch_split(SplitArgs A, uint32_t tiles, cudaStream_t st) {
   using Sh = SplitShape<HD, BITS>;
@@ -939,21 +1007,32 @@ int launch_split(SplitArgs A, uint32_t tiles, cudaStream_t st) {
   const uint32_t span = A.d.window && A.d.window < keys ? A.d.window + A.d.max_q : keys;
   const uint32_t kblocks = (span < keys ? span : keys) / Sh::KS + 2u;
   // the CTAs an SM that the registers allow, or fewer: so many that the scores fit beside
-  // a stage a warp (two, where the registers bound); and as many CTAs a cluster as are
-  // all resident at once and leave each warp two blocks
+  // a stage a warp, but no more than are used.  A cluster lies within a GPC, so X CTAs of
+  // it are at once resident for all `blocks` when the device holds so many clusters at
+  // some d CTAs an SM.  d CTAs share an SM's issue slots but hide one another's waits: the
+  // least (d + 1) / X is taken that leaves a warp two blocks (8 sequences x 5 heads of 21k
+  // to 32k keys: X = 3 77 us, 4 64, 5 56, 6 43, and 59 for 8, which is not resident at
+  // once; 4 x 5 heads at 16 bits: 104, 80, 68, 46, 8 43)
   uint32_t X, occ = Sh::OCC, room, need, fixed;
   const uint32_t block = kWarps * A.rcap * Sh::PW * 4u;
   for (;; occ--) {
-    for (X = 1; X < kMaxCluster && blocks * (X + 1u) <= 148u * occ && kblocks >= 2u * kWarps * (X + 1u);) X++;
+    uint64_t bd = (blocks + 147u) / 148u;
+    X = 1;
+    for (uint32_t x = 2; x <= kMaxCluster && kblocks >= 2u * kWarps * x; x++) {
+      uint32_t d = 1;
+      while (d <= occ && resident_clusters<HD, BITS>(x, d) < blocks) d++;
+      if (d <= occ && (d + 1u) * X < (bd + 1u) * x) X = x, bd = d;
+    }
     fixed = 8192u + (X > 1 ? A.rcap * HD * 4u : 0u);
     need = ((kblocks + X - 1u) / X + kWarps - 1u) / kWarps;  // of a warp
-    room = (occ == 3u ? 73u : (occ == 2u ? 110u : 222u)) * 1024u - fixed;
-    if (occ == 1u || (uint64_t)need * block + (occ == 3u ? 1u : 2u) * kWarps * Sh::STB <= room) break;
+    room = split_smem(occ) - fixed;
+    if (occ == 1u || ((uint64_t)need * block + kWarps * Sh::STB <= room && (occ == 2u || bd > 2u))) break;
   }
   A.X = X;
+  A.Ginv = (65536u + A.G - 1u) / A.G;
   uint32_t stages = 1;
   const uint32_t most = (room - kWarps * Sh::STB) / block;
-  A.win = need < most ? need : most;
+  A.win = min(min(need, most), 512u);  // (a row's sum of e over a window fits 32 bits)
   while (stages < 4u && A.win * block + 2u * stages * kWarps * Sh::STB <= room) stages *= 2u;  // 1, 2 or 4
   A.stages = stages;
   const size_t smem = kWarps * stages * Sh::STB + (size_t)A.win * block + fixed;
@@ -1100,7 +1179,17 @@ extern "C" int corm_llm_paged_attn(const corm_llm_paged_attn_desc* d, corm_strea
   const uint64_t tiles = (rows + kRows - 1u) / kRows;
   if (tiles > (1ull << 27)) return corm::fail(CORM_ELIMIT, "corm_llm_paged_attn: max_q %u", d->max_q);
   cudaStream_t st = (cudaStream_t)stream;
-  if (rows > kSplitRows && paged::tile_takes(A.d)) return paged::launch_tiles(A.d, A.tab, A.err, st);
+  // this form or 128-row tiles: up to 32 rows a sequence and KV head this one (8 rows cost
+  // it the time that 128 cost the other).  Beyond, where its CTAs leave SMs idle (8 groups
+  // of 600 keys: 128 rows 14 us against 37), and up to 64 rows where they are at once
+  // resident (32 groups of 600: 64 rows 16 us against 31) or the other's scores do not fit
+  // (128 groups of 4000: 64 rows 223 us against 229, 40 rows 151 against 243; of 600, 64
+  // rows: 52 against 45)
+  const uint32_t cap = c.table_width * c.page, span = A.d.window ? A.d.window + A.d.max_q : cap;
+  const uint32_t keys = min(A.d.max_keys, min(cap, span < A.d.window ? cap : span));
+  const uint64_t ctas = tiles * c.B * c.KV;
+  const bool few = rows <= 32u || (rows <= 64u && (keys > 640u || ctas <= 444u)) || (rows <= 128u && ctas <= 148u);
+  if (!few && paged::tile_takes(A.d)) return paged::launch_tiles(A.d, A.tab, A.err, st);
   switch (c.HD * 2u + (c.bits == 8u)) {
     case 32: return launch_split<16, 16>(A, (uint32_t)tiles, st);
     case 33: return launch_split<16, 8>(A, (uint32_t)tiles, st);

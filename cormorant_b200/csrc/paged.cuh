@@ -96,14 +96,14 @@ __device__ __forceinline__ uint32_t pack16(int32_t lo, int32_t hi) {  // both al
 // (warp-level; used where a tile has 16 rows at most)
 #define CORM_MMA_I8(NAME, TA, TB)                                                                                      \
   __device__ __forceinline__ void NAME(uint32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {           \
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." TA "." TB                                                    \
+    asm("mma.sync.aligned.m16n8k32.row.col.s32." TA "." TB                                                    \
                  ".s32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"                                             \
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])                                                      \
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));                                      \
   }                                                                                                                    \
   /* C = A B */                                                                                                        \
   __device__ __forceinline__ void NAME##_first(uint32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   \
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." TA "." TB                                                    \
+    asm("mma.sync.aligned.m16n8k32.row.col.s32." TA "." TB                                                    \
                  ".s32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%10,%10,%10,%10};"                                         \
                  : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])                                                      \
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));                              \
