@@ -39,15 +39,17 @@ namespace {
 using namespace paged;
 
 // ---------------------------------------------------------------- preparation
-// A group of HD / 8 lanes per (row, head slot), a lane holding the 8 elements of
-// four pairs; a thread keeps its slot over all its rows (the grid's step is a
-// multiple of the slots), so its entries are decoded once.  Norm: the squares'
-// sum by shuffles over the group, the divisor by the unit's table and Newton
+// A warp per row, or per part of a row's heads where there are few rows: HD / 8 lanes
+// a head, a lane holding the 8 elements of four pairs, the heads in turns of 256 / HD
+// (the rotated ones, then v's).  A row's sequence, page, cosines and sines are looked
+// up once for all its heads, and a lane's entries once for all its rows.  Norm: the
+// squares' sum by shuffles over the head, the divisor by the unit's table and Newton
 // step, 64-bit throughout (D < 2^63, |x Rm| < 2^48, |P1 G| < 2^56).
+constexpr uint32_t kTurns = 8;  // turns of a part: their entries' forms are a byte each of one word
 struct PrepArgs {
   corm_llm_paged_prep_desc d;
   const uint32_t* rsq;
-  uint32_t vec;  // 8-byte loads and stores are aligned and whole
+  uint32_t turned, turns, per, parts;  // turns of the rotated heads, of all; a part's; parts of a row
 };
 
 // the row-ops unit's 1 / sqrt(D) ~ Rm 2^-sh for 1 <= D < 2^63
@@ -73,313 +75,424 @@ __device__ __noinline__ int32_t rot_any(int32_t x, int32_t cs, int32_t y, int32_
   return (int32_t)corm_sat16_128(corm_rne_shr128(((__int128)u << a) + ((__int128)v << b), c));
 }
 // no up-shift, a down-shift k <= 31 whose quotient is below 2^31 (sums stay below
-// 2^40: k >= 9, or an element that is not rotated): both roundings (floor for the
-// parity, then the result) are one funnel shift each.  half1 = 2^(k - 1) - 1 and
-// par = 1, both 0 for k = 0
-__device__ __forceinline__ int32_t rot_plain(int32_t x, int32_t cs, int32_t y, int32_t sn, uint32_t k, uint32_t half1,
+// 2^40: k >= 9, or an element that is not rotated).  To nearest, ties to even: with
+// half1 = 2^(k - 1) - 1 added first, the bit at 2^k is still the quotient's parity in a
+// tie, and where it is not, adding it carries nothing.  par = 1; both 0 for k = 0
+__device__ __forceinline__ int32_t rot_plain(int32_t x, int32_t cs, int32_t y, int32_t sn, uint32_t k, int64_t half1,
                                              uint32_t par) {
-  const int64_t v = (int64_t)x * cs + (int64_t)y * sn;
-  const uint32_t odd = __funnelshift_r((uint32_t)v, (uint32_t)(v >> 32), k) & par;
-  const int64_t u = v + (int64_t)(half1 + odd);
+  const int64_t v = (int64_t)x * cs + ((int64_t)y * sn + half1);
+  const int64_t u = v + (int64_t)(__funnelshift_r((uint32_t)v, (uint32_t)(v >> 32), k) & par);
   return (int32_t)__funnelshift_r((uint32_t)u, (uint32_t)(u >> 32), k);
+}
+
+// A row of the batch: its sequence (rows ascend: b goes forward), position and page
+struct RowAt {
+  bool in;        // a row of a sequence
+  uint64_t p;     // its position
+  uint64_t line;  // the page's first cached row of head 0, plus the row's place in a page
+  bool held;      // the position has a page
+};
+__device__ __forceinline__ uint32_t first_sequence(const corm_paged_cache& c, uint64_t row) {
+  uint32_t b = 0, hi = c.B;  // the last b with cu[b] <= row lies in [b, hi)
+  while (hi - b > 1u) {
+    const uint32_t mid = (b + hi) / 2u;
+    if ((int64_t)c.cu[mid] <= (int64_t)row) b = mid;
+    else hi = mid;
+  }
+  return b;
+}
+__device__ __forceinline__ RowAt row_at(const corm_paged_cache& c, uint64_t row, uint32_t& b) {
+  while (b + 1u < c.B && (int64_t)c.cu[b + 1] <= (int64_t)row) b++;
+  const SeqRows s = seq_rows(c, b, c.rows);
+  RowAt o;
+  o.in = row >= s.lo && row < s.lo + s.n;
+  o.p = (uint64_t)s.pos + (row - s.lo);
+  o.held = false;
+  o.line = 0;
+  if (o.in && o.p < s.cap) {
+    const uint32_t sh = 31u - __clz(c.page);
+    const int32_t pg = c.table[(uint64_t)b * c.table_width + (uint32_t)(o.p >> sh)];
+    o.held = (uint32_t)pg < c.pages;
+    if (o.held) o.line = (uint64_t)(uint32_t)pg * c.KV * c.page + ((uint32_t)o.p & (c.page - 1u));
+  }
+  return o;
 }
 
 template <int HD, bool VEC, bool NORM>
 __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constant__ PrepArgs A) {
+  constexpr uint32_t LPH = HD / 8, HPT = 32 / LPH;  // lanes a head, heads a turn
+  __shared__ int2 s_norm[NORM ? 2 : 1][NORM ? HD : 1];  // the norms' factors and down-shifts, q's and k's
   corm_pdl_wait();
   corm_pdl_trigger();
-  constexpr uint32_t LPH = HD / 8;     // lanes per head
-  constexpr uint32_t SPB = 256 / LPH;  // heads per block and pass
   const corm_llm_paged_prep_desc& d = A.d;
   const corm_paged_cache& c = d.c;
-  const uint32_t KV = c.KV, slots = d.H + 2u * KV;
-  const uint32_t lane = threadIdx.x % LPH;
-  const uint64_t item0 = (uint64_t)blockIdx.x * SPB + threadIdx.x / LPH, step = (uint64_t)gridDim.x * SPB;  // step % slots == 0
-  const uint32_t slot = (uint32_t)(item0 % slots);
-  const uint32_t row_step = (uint32_t)(step / slots);
-  const bool is_q = slot < d.H, is_v = slot >= d.H + KV;
-  const uint32_t head = is_q ? slot : (is_v ? slot - d.H - KV : slot - d.H);
-  const uint32_t rot = is_v ? 0u : d.rot, hr = rot / 2u;
-  // the dimensions of this lane's pairs: a rotated pair p at (p, p + rot / 2) or
-  // (2 p, 2 p + 1); the rest of the head in neighbouring pairs
-  uint32_t da[4], db[4];
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    const uint32_t p = 4u * lane + k;
-    const bool split = p < hr && !d.interleaved;
-    da[k] = split ? p : 2u * p;
-    db[k] = split ? p + hr : 2u * p + 1u;
-  }
-  const bool spl = 4u * lane < hr && !d.interleaved;  // VEC: alike for the lane's four pairs
-  // the usual entries: no up-shift and one down-shift for the lane's elements, whose
-  // quotients fit 32 bits; any others are read again where they are used
-  const uint8_t* ent = (const uint8_t*)(is_q ? d.pq : (is_v ? d.pv : d.pk));
-  const bool bc = d.flags & (is_q ? 1u : (is_v ? 4u : 2u)), direct = is_v && (d.flags & 8u);
-  auto shifts = [&](uint32_t dim) -> uint32_t {  // sh_a | sh_b << 8 | sh_c << 16
-    return direct ? 0u : *(const uint32_t*)(ent + 16ull * (bc ? 0u : head * HD + dim) + 8) & 0x3F3F3Fu;
-  };
-  const uint32_t k0 = shifts(da[0]), kd = k0 >> 16;
-  bool plain = (k0 & 0xFFFFu) == 0u && kd <= 31u && (kd >= 9u || 4u * lane >= hr);
-#pragma unroll
-  for (int k = 0; k < 4; k++) plain = plain && shifts(da[k]) == k0 && shifts(db[k]) == k0;
-  const uint32_t half1 = kd ? (1u << (kd & 31u)) / 2u - 1u : 0u, par = kd ? 1u : 0u;
-  const uint8_t* ne = (const uint8_t*)(is_q ? d.nq : (is_v ? nullptr : d.nk));
-  int32_t ga[4], gb[4];
-  uint32_t na = 0, nb = 0;  // the norm's down-shifts, a byte each
-  if (NORM && ne) {
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const uint8_t* ea = ne + 16u * da[k];
-      const uint8_t* eb = ne + 16u * db[k];
-      ga[k] = *(const int32_t*)ea;
-      gb[k] = *(const int32_t*)eb;
-      na |= (ea[10] & 63u) << (8 * k);
-      nb |= (eb[10] & 63u) << (8 * k);
-    }
-  }
-  const uint64_t eps = is_q ? d.eps_q : d.eps_k;
-  const int16_t* src = is_q ? d.q0 : (is_v ? d.v0 : d.k0);
-  const uint64_t ld = is_q ? d.ldq0 : (is_v ? d.ldv : d.ldk);
-  const unsigned mask = LPH == 32 ? 0xffffffffu : ((1u << LPH) - 1u) << ((threadIdx.x & 31u) / LPH * LPH);
+  const uint32_t KV = c.KV, lane = threadIdx.x % LPH, sub = (threadIdx.x & 31u) / LPH, hr = d.rot / 2u;
+  const uint32_t gw = blockIdx.x * 8u + (threadIdx.x >> 5), row_step = gridDim.x * 8u / A.parts, part = gw % A.parts;
+  uint64_t row = gw / A.parts;
   const int32_t total = c.cu[c.B];
   const uint64_t rows = min((uint64_t)c.rows, (uint64_t)max(total, 0));
-  // the sequence of the first row: the last b with cu[b] <= row (cu ascends), then
-  // forward as the rows do
-  uint32_t b = 0;
-  {
-    uint32_t hi = c.B;  // the answer lies in [b, hi)
-    const int64_t r = (int64_t)(item0 / slots);
-    while (hi - b > 1u) {
-      const uint32_t mid = (b + hi) / 2u;
-      if ((int64_t)c.cu[mid] <= r) b = mid;
-      else hi = mid;
+  if (NORM) {
+    for (uint32_t i = threadIdx.x; i < 2u * HD; i += 256u) {
+      const uint8_t* ne = (const uint8_t*)(i < HD ? d.nq : d.nk);
+      if (ne) s_norm[i / HD][i % HD] = make_int2(*(const int32_t*)(ne + 16u * (i % HD)), ne[16u * (i % HD) + 10u] & 63);
     }
+    __syncthreads();
   }
-  for (uint64_t row = item0 / slots; row < rows; row += row_step) {
-    while (b + 1u < c.B && (int64_t)c.cu[b + 1] <= (int64_t)row) b++;
-    const SeqRows s = seq_rows(c, b, c.rows);
-    if (row < s.lo || row >= s.lo + s.n) continue;  // a row of no sequence (alike over the group)
-    const uint64_t p = (uint64_t)s.pos + (row - s.lo);
-    const int16_t* x = src + row * ld + (uint64_t)head * HD;
-    int32_t va[4], vb[4];
+  if (row >= rows || row >= row_step) return;
+  const uint32_t it0 = part * A.per, it1 = min(it0 + A.per, A.turns);
+  // a turn's head: whether there is one for this lane, of what, which
+  struct Slot {
+    bool any, is_q, is_v;
+    uint32_t head;
+  };
+  auto slot_of = [&](uint32_t it) {
+    Slot s;
+    const bool v = it >= A.turned;
+    const uint32_t i = (v ? it - A.turned : it) * HPT + sub;
+    s.is_v = v;
+    s.any = i < (v ? KV : d.H + KV);
+    s.is_q = !v && i < d.H;
+    s.head = v || s.is_q ? i : i - d.H;
+    return s;
+  };
+  // the dimensions of this lane's pairs: a rotated pair p at (p, p + rot / 2) or
+  // (2 p, 2 p + 1); the rest of the head, and v's, in neighbouring pairs
+  auto dim_a = [&](uint32_t k, bool v) {
+    const uint32_t p = 4u * lane + k;
+    return p < hr && !d.interleaved && !v ? p : 2u * p;
+  };
+  auto dim_b = [&](uint32_t k, bool v) {
+    const uint32_t p = 4u * lane + k;
+    return p < hr && !d.interleaved && !v ? p + hr : 2u * p + 1u;
+  };
+  auto shifts = [&](const Slot& s, uint32_t dim) -> uint32_t {  // sh_a | sh_b << 8 | sh_c << 16
+    const uint8_t* ent = (const uint8_t*)(s.is_q ? d.pq : (s.is_v ? d.pv : d.pk));
+    const bool bc = d.flags & (s.is_q ? 1u : (s.is_v ? 4u : 2u));
+    return s.is_v && (d.flags & 8u) ? 0u : *(const uint32_t*)(ent + 16ull * (bc ? 0u : s.head * HD + dim) + 8) & 0x3F3F3Fu;
+  };
+  // the usual entries: no up-shift and one down-shift for the lane's elements, whose
+  // quotients fit 32 bits: the down-shift, a byte a turn; any others (255) are read
+  // again where they are used
+  uint64_t forms = 0;
+#pragma unroll 1
+  for (uint32_t it = it0; it < it1; it++) {
+    const Slot s = slot_of(it);
+    uint32_t kd = 255;
+    if (s.any) {
+      const uint32_t k0 = shifts(s, dim_a(0, s.is_v));
+      kd = k0 >> 16;
+      bool plain = (k0 & 0xFFFFu) == 0u && kd <= 31u && (kd >= 9u || s.is_v || 4u * lane >= hr);
+#pragma unroll
+      for (uint32_t k = 0; k < 4; k++) plain = plain && shifts(s, dim_a(k, s.is_v)) == k0 && shifts(s, dim_b(k, s.is_v)) == k0;
+      if (!plain) kd = 255;
+    }
+    forms |= (uint64_t)kd << (8u * (it - it0));
+  }
+  const bool spl = 4u * lane < hr && !d.interleaved;  // VEC: alike for the lane's four pairs
+  // the next row's heads, q's and k's counted as one (k's head i - H), this lane's place
+  // in them; the second four of its elements are `far` on (VEC)
+  const uint32_t place = VEC ? (spl ? 4u : 8u) * lane : 0u, far = spl ? hr : 4u, place_v = VEC ? 8u * lane : 0u;
+  const int16_t* nq = d.q0 + row * d.ldq0 + place;
+  const int16_t* nk = d.k0 + row * d.ldk + place - (uint64_t)d.H * HD;
+  const int16_t* nv = d.v0 + row * d.ldv + place_v;
+  int16_t* yq = d.q + row * d.ldq + place;
+  // the 8 elements of a turn: two words of 4, the pairs' firsts and seconds where `spl`
+  // (or not VEC), else as they lie
+  auto load = [&](uint32_t it) {
+    uint4 w = make_uint4(0, 0, 0, 0);
+    const bool v = it >= A.turned;
+    const uint32_t i = (v ? it - A.turned : it) * HPT + sub;
+    if (i >= (v ? KV : d.H + KV)) return w;
+    const int16_t* x = (v ? nv : (i < d.H ? nq : nk)) + (uint64_t)i * HD;
     if (VEC) {
-      uint2 w0, w1;
-      if (spl) {
-        w0 = *(const uint2*)(x + 4u * lane);
-        w1 = *(const uint2*)(x + 4u * lane + hr);
-      } else {
-        w0 = *(const uint2*)(x + 8u * lane);
-        w1 = *(const uint2*)(x + 8u * lane + 4u);
-      }
-      const int32_t v8[8] = {(int16_t)w0.x, (int32_t)w0.x >> 16, (int16_t)w0.y, (int32_t)w0.y >> 16,
-                             (int16_t)w1.x, (int32_t)w1.x >> 16, (int16_t)w1.y, (int32_t)w1.y >> 16};
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        va[k] = spl ? v8[k] : v8[2 * k];
-        vb[k] = spl ? v8[4 + k] : v8[2 * k + 1];
-      }
+      const uint2 a = *(const uint2*)x, b = *(const uint2*)(x + (v ? 4u : far));
+      w = make_uint4(a.x, a.y, b.x, b.y);
     } else {
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        va[k] = x[da[k]];
-        vb[k] = x[db[k]];
-      }
+      w = make_uint4(pack16(x[dim_a(0, v)], x[dim_a(1, v)]), pack16(x[dim_a(2, v)], x[dim_a(3, v)]),
+                     pack16(x[dim_b(0, v)], x[dim_b(1, v)]), pack16(x[dim_b(2, v)], x[dim_b(3, v)]));
     }
-    if (NORM && ne) {
-      uint64_t s2 = 0;
-#pragma unroll
-      for (int k = 0; k < 4; k++) s2 += (uint64_t)(uint32_t)(va[k] * va[k]) + (uint32_t)(vb[k] * vb[k]);
-#pragma unroll
-      for (uint32_t o = LPH / 2; o > 0; o >>= 1) s2 += __shfl_xor_sync(mask, s2, o);
-      uint64_t Rm;
-      int sh;
-      rsqrt64(max(s2 + eps, (uint64_t)1), Rm, sh, A.rsq);
-      sh -= 24;
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        va[k] = (int32_t)corm_sat16(corm_rne_shr64f((((int64_t)va[k] * (int64_t)Rm) >> sh) * ga[k], (int)(na >> (8 * k)) & 63));
-        vb[k] = (int32_t)corm_sat16(corm_rne_shr64f((((int64_t)vb[k] * (int64_t)Rm) >> sh) * gb[k], (int)(nb >> (8 * k)) & 63));
-      }
-    }
-    const int32_t* tr = d.rope + (uint64_t)min(p, (uint64_t)(d.rope_rows - 1u)) * d.rot;
+    return w;
+  };
+  uint32_t b = first_sequence(c, row);
+  uint4 w = load(it0);
+#pragma unroll 1
+  for (; row < rows; row += row_step, yq += row_step * d.ldq) {
+    const RowAt at = row_at(c, row, b);
+    const uint32_t rb = c.bits == 8u ? HD : 2 * HD;
+    int8_t* const kr = c.kc + at.line * rb;
+    int8_t* const vr = c.vc + at.line * rb;
     int32_t cs[4], sn[4];
-    if (VEC && 4u * lane < hr) {
-      const int4 c4 = __ldg((const int4*)(tr + 4u * lane)), s4 = __ldg((const int4*)(tr + hr + 4u * lane));
-      cs[0] = c4.x, cs[1] = c4.y, cs[2] = c4.z, cs[3] = c4.w;
-      sn[0] = s4.x, sn[1] = s4.y, sn[2] = s4.z, sn[3] = s4.w;
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const uint32_t pr = 4u * lane + k;
-        cs[k] = pr < hr ? __ldg(tr + pr) : 1;  // past the rotated part: x << sh_a alone
-        sn[k] = pr < hr ? __ldg(tr + hr + pr) : 0;
-      }
-    }
-    if (plain) {
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int32_t a = va[k], bb = vb[k];
-        va[k] = min(max(rot_plain(a, cs[k], -bb, sn[k], kd, half1, par), -32768), 32767);
-        vb[k] = min(max(rot_plain(bb, cs[k], a, sn[k], kd, half1, par), -32768), 32767);
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int32_t a = va[k], bb = vb[k];
-        va[k] = rot_any(a, cs[k], -bb, sn[k], shifts(da[k]));
-        vb[k] = rot_any(bb, cs[k], a, sn[k], shifts(db[k]));
-      }
-    }
-    if (is_q) {
-      int16_t* y = d.q + row * d.ldq + (uint64_t)head * HD;
-      if (VEC) {
-        if (spl) {
-          *(uint2*)(y + 4u * lane) = make_uint2(pack16(va[0], va[1]), pack16(va[2], va[3]));
-          *(uint2*)(y + 4u * lane + hr) = make_uint2(pack16(vb[0], vb[1]), pack16(vb[2], vb[3]));
-        } else {
-          *(uint2*)(y + 8u * lane) = make_uint2(pack16(va[0], vb[0]), pack16(va[1], vb[1]));
-          *(uint2*)(y + 8u * lane + 4u) = make_uint2(pack16(va[2], vb[2]), pack16(va[3], vb[3]));
-        }
+    {
+      const int32_t* tr = d.rope + (uint64_t)min(at.in ? at.p : (uint64_t)0, (uint64_t)(d.rope_rows - 1u)) * d.rot;
+      if (VEC && 4u * lane < hr) {
+        const int4 c4 = __ldg((const int4*)(tr + 4u * lane)), s4 = __ldg((const int4*)(tr + hr + 4u * lane));
+        cs[0] = c4.x, cs[1] = c4.y, cs[2] = c4.z, cs[3] = c4.w;
+        sn[0] = s4.x, sn[1] = s4.y, sn[2] = s4.z, sn[3] = s4.w;
       } else {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          y[da[k]] = (int16_t)va[k];
-          y[db[k]] = (int16_t)vb[k];
+          const uint32_t pr = 4u * lane + k;
+          cs[k] = pr < hr ? __ldg(tr + pr) : 1;  // past the rotated part: x << sh_a alone
+          sn[k] = pr < hr ? __ldg(tr + hr + pr) : 0;
         }
       }
-      continue;
     }
-    uint32_t shift = 0;
-    if (c.bits == 8u) {  // (every lane of the group, also where nothing is written)
-      uint32_t t = 0;
+#pragma unroll 1
+    for (uint32_t it = it0; it < it1; it++) {
+      const uint4 x = w;
+      // the next turn's elements, while this one's are worked on
+      if (it + 1u < it1) {
+        w = load(it + 1u);
+      } else if (row + row_step < rows) {
+        nq += row_step * d.ldq0;
+        nk += row_step * d.ldk;
+        nv += row_step * d.ldv;
+        w = load(it0);
+      }
+      if (!at.in) continue;  // a row of no sequence
+      const Slot s = slot_of(it);
+      const bool sp = VEC ? spl && !s.is_v : true;
+      int32_t va[4], vb[4];
+      {
+        const int32_t v8[8] = {(int16_t)x.x, (int32_t)x.x >> 16, (int16_t)x.y, (int32_t)x.y >> 16,
+                               (int16_t)x.z, (int32_t)x.z >> 16, (int16_t)x.w, (int32_t)x.w >> 16};
 #pragma unroll
-      for (int k = 0; k < 4; k++) t = max(t, max((uint32_t)(va[k] ^ (va[k] >> 31)), (uint32_t)(vb[k] ^ (vb[k] >> 31))));
+        for (int k = 0; k < 4; k++) {
+          va[k] = sp ? v8[k] : v8[2 * k];
+          vb[k] = sp ? v8[4 + k] : v8[2 * k + 1];
+        }
+      }
+      if (NORM && !s.is_v) {  // (alike over the warp; a head's lanes all have it or not)
+        uint64_t s2 = 0;
 #pragma unroll
-      for (uint32_t o = LPH / 2; o > 0; o >>= 1) t = max(t, __shfl_xor_sync(mask, t, o));
-      const int bits = 32 - __clz((int)t);
-      shift = bits > 7 ? (uint32_t)(bits - 7) : 0u;
-      // RNE by shift <= 8; only the upper end can round past the codes
+        for (int k = 0; k < 4; k++) s2 += (uint64_t)(uint32_t)(va[k] * va[k]) + (uint32_t)(vb[k] * vb[k]);
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
+        for (uint32_t o = LPH / 2; o > 0; o >>= 1) s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+        if (s.is_q ? d.nq : d.nk) {
+          uint64_t Rm;
+          int sh;
+          rsqrt64(max(s2 + (s.is_q ? d.eps_q : d.eps_k), (uint64_t)1), Rm, sh, A.rsq);
+          sh -= 24;
+          // |x| <= sqrt(D): x Rm 2^-sh is 2^24 at most, and the table's error
+          auto normed = [&](int32_t x, uint32_t dim) {
+            const int2 g = s_norm[s.is_q ? 0 : 1][NORM ? dim : 0];
+            return (int32_t)corm_sat16(corm_rne_shr64f((int64_t)(int32_t)(((int64_t)x * (int64_t)Rm) >> sh) * g.x, g.y));
+          };
+#pragma unroll
+          for (uint32_t k = 0; k < 4; k++) {
+            va[k] = normed(va[k], dim_a(k, false));
+            vb[k] = normed(vb[k], dim_b(k, false));
+          }
+        }
+      }
+      const uint32_t kd = (uint32_t)(forms >> (8u * (it - it0))) & 255u;
+      if (kd != 255u) {
+        const uint32_t half1 = kd ? (1u << kd) / 2u - 1u : 0u, par = kd ? 1u : 0u;
+        if (s.is_v) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            va[k] = (va[k] + (int32_t)(half1 + ((uint32_t)(va[k] >> kd) & par))) >> kd;
+            vb[k] = (vb[k] + (int32_t)(half1 + ((uint32_t)(vb[k] >> kd) & par))) >> kd;
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const int32_t a = va[k], bb = vb[k];
+            va[k] = rot_plain(a, cs[k], -bb, sn[k], kd, half1, par);
+            vb[k] = rot_plain(bb, cs[k], a, sn[k], kd, half1, par);
+          }
+        }
+      } else if (s.any) {
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+          const int32_t a = va[k], bb = vb[k];
+          va[k] = rot_any(a, s.is_v ? 1 : cs[k], -bb, s.is_v ? 0 : sn[k], shifts(s, dim_a(k, s.is_v)));
+          vb[k] = rot_any(bb, s.is_v ? 1 : cs[k], a, s.is_v ? 0 : sn[k], shifts(s, dim_b(k, s.is_v)));
+        }
+      }
+      // (saturates)
+      uint32_t w0 = pack_s16(va[0], va[1]), w1 = pack_s16(va[2], va[3]), w2 = pack_s16(vb[0], vb[1]), w3 = pack_s16(vb[2], vb[3]);
+      if (s.is_q) {
+        int16_t* y = yq + (uint64_t)s.head * HD;
+        if (VEC) {
+          *(uint2*)y = sp ? make_uint2(w0, w1) : make_uint2(__byte_perm(w0, w2, 0x5410), __byte_perm(w0, w2, 0x7632));
+          *(uint2*)(y + far) = sp ? make_uint2(w2, w3) : make_uint2(__byte_perm(w1, w3, 0x5410), __byte_perm(w1, w3, 0x7632));
+        } else {
+          const uint32_t ww[4] = {w0, w1, w2, w3};
+#pragma unroll
+          for (uint32_t k = 0; k < 4; k++) {
+            y[dim_a(k, false)] = (int16_t)(ww[k >> 1] >> (16u * (k & 1u)));
+            y[dim_b(k, false)] = (int16_t)(ww[2 + (k >> 1)] >> (16u * (k & 1u)));
+          }
+        }
+      }
+      uint32_t shift = 0;
+      if (c.bits == 8u) {  // (every lane: the head's largest element)
+        uint32_t t = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          va[k] = min(max(va[k], -32768), 32767);
+          vb[k] = min(max(vb[k], -32768), 32767);
+          t = max(t, max((uint32_t)(va[k] ^ (va[k] >> 31)), (uint32_t)(vb[k] ^ (vb[k] >> 31))));
+        }
+#pragma unroll
+        for (uint32_t o = LPH / 2; o > 0; o >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
+        const int bits = 32 - __clz((int)t);
+        shift = bits > 7 ? (uint32_t)(bits - 7) : 0u;
+      }
+      if (s.is_q || !s.any || !at.held) continue;
+      int8_t* y = (s.is_v ? vr : kr) + (uint64_t)s.head * (c.page * rb);
+      if (c.bits == 8u) {
+        // RNE by shift <= 8; only the upper end can round past the codes
         const int32_t h = (1 << shift) >> 1, r = h ? h - 1 : 0;
-        va[k] = min((va[k] + r + (h ? (va[k] >> shift) & 1 : 0)) >> shift, 127);
-        vb[k] = min((vb[k] + r + (h ? (vb[k] >> shift) & 1 : 0)) >> shift, 127);
-      }
-    }
-    if (p >= s.cap) continue;
-    const int32_t pg = c.table[(uint64_t)b * c.table_width + p / c.page];
-    if ((uint32_t)pg >= c.pages) continue;
-    const uint64_t line = ((uint64_t)pg * KV + head) * c.page + p % c.page;
-    int8_t* y = (is_v ? c.vc : c.kc) + line * (c.bits == 8u ? HD : 2 * HD);
-    if (VEC) {
-      uint32_t w[4];  // bytes of va, of vb: low (or code), then high
 #pragma unroll
-      for (int q = 0; q < 2; q++) {
-        const int32_t* v = q ? vb : va;
-        const uint32_t l0 = pack16(v[0], v[1]), l1 = pack16(v[2], v[3]);
-        w[q] = __byte_perm(l0, l1, 0x6420);
-        w[2 + q] = __byte_perm(l0, l1, 0x7531);
-      }
-#pragma unroll
-      for (int pl = 0; pl < 2; pl++) {  // low bytes (codes), high bytes
-        if (pl && c.bits == 8u) break;
-        int8_t* yp = y + (c.bits == 8u || pl ? 0 : HD);
-        if (spl) {
-          *(uint32_t*)(yp + 4u * lane) = w[2 * pl];
-          *(uint32_t*)(yp + 4u * lane + hr) = w[2 * pl + 1];
-        } else {
-          *(uint2*)(yp + 8u * lane) =
-              make_uint2(__byte_perm(w[2 * pl], w[2 * pl + 1], 0x5140), __byte_perm(w[2 * pl], w[2 * pl + 1], 0x7362));
+        for (int k = 0; k < 4; k++) {
+          va[k] = min((va[k] + r + (h ? (va[k] >> shift) & 1 : 0)) >> shift, 127);
+          vb[k] = min((vb[k] + r + (h ? (vb[k] >> shift) & 1 : 0)) >> shift, 127);
         }
+        if (lane == 0) (s.is_v ? c.vs : c.ks)[at.line + (uint64_t)s.head * c.page] = (uint8_t)shift;
+        w0 = pack_s16(va[0], va[1]), w1 = pack_s16(va[2], va[3]), w2 = pack_s16(vb[0], vb[1]), w3 = pack_s16(vb[2], vb[3]);
       }
-    } else {
+      if (VEC) {
+        // bytes of va, of vb: low (or code), then high
+        const uint32_t wb[4] = {__byte_perm(w0, w1, 0x6420), __byte_perm(w2, w3, 0x6420), __byte_perm(w0, w1, 0x7531),
+                                __byte_perm(w2, w3, 0x7531)};
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        if (c.bits == 8u) {
-          y[da[k]] = (int8_t)va[k];
-          y[db[k]] = (int8_t)vb[k];
-        } else {
-          y[da[k]] = (int8_t)(va[k] >> 8);
-          y[db[k]] = (int8_t)(vb[k] >> 8);
-          y[HD + da[k]] = (int8_t)va[k];
-          y[HD + db[k]] = (int8_t)vb[k];
+        for (int pl = 0; pl < 2; pl++) {  // low bytes (codes), high bytes
+          if (pl && c.bits == 8u) break;
+          int8_t* yp = y + (c.bits == 8u || pl ? 0 : HD);
+          if (sp) {
+            *(uint32_t*)(yp + 4u * lane) = wb[2 * pl];
+            *(uint32_t*)(yp + 4u * lane + hr) = wb[2 * pl + 1];
+          } else {
+            *(uint2*)(yp + 8u * lane) = make_uint2(__byte_perm(wb[2 * pl], wb[2 * pl + 1], 0x5140),
+                                                   __byte_perm(wb[2 * pl], wb[2 * pl + 1], 0x7362));
+          }
+        }
+      } else {
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+          const uint32_t da = dim_a(k, s.is_v), db = dim_b(k, s.is_v), m = 16u * (k & 1u);
+          const uint32_t a = (k < 2 ? w0 : w1) >> m, bb = (k < 2 ? w2 : w3) >> m;
+          if (c.bits == 8u) {
+            y[da] = (int8_t)a;
+            y[db] = (int8_t)bb;
+          } else {
+            y[da] = (int8_t)(a >> 8);
+            y[db] = (int8_t)(bb >> 8);
+            y[HD + da] = (int8_t)a;
+            y[HD + db] = (int8_t)bb;
+          }
         }
       }
     }
-    if (c.bits == 8u && lane == 0) (is_v ? c.vs : c.ks)[line] = (uint8_t)shift;
   }
 }
 
 // ---------------------------------------------------------------- read-back
-// A lane per 8 elements of (row, KV head, K or V): 8-byte loads of each plane,
-// one 16-byte store (8-byte stores where the output is not on 16 bytes).
+// A warp per row, or per part of its heads (K's, then V's) where there are few rows;
+// HD / 8 lanes a head, 8 elements a lane: 8-byte loads of each plane, four heads' under
+// way at once, one 16-byte store (words where the output is not on 16 bytes).
+struct ReadArgs {
+  corm_llm_paged_read_desc d;
+  uint32_t vec, heads, turns, per, parts;  // heads: K's and V's, or one of them
+};
 template <int HD>
-__global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__ corm_llm_paged_read_desc d, uint32_t vec) {
+__global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__ ReadArgs A) {
   corm_pdl_wait();
   corm_pdl_trigger();
-  constexpr uint32_t LPH = HD / 8;
+  constexpr uint32_t LPH = HD / 8, HPT = 32 / LPH, U = 4;
+  const corm_llm_paged_read_desc& d = A.d;
   const corm_paged_cache& c = d.c;
-  const uint32_t slots = 2u * c.KV;
+  const uint32_t lane = threadIdx.x % LPH, sub = (threadIdx.x & 31u) / LPH, nk = d.k ? c.KV : 0u;
+  const uint32_t gw = blockIdx.x * 8u + (threadIdx.x >> 5), row_step = gridDim.x * 8u / A.parts;
+  const uint32_t part = gw % A.parts, it0 = part * A.per, it1 = min(it0 + A.per, A.turns);
+  uint64_t row = gw / A.parts;
   const int32_t last = c.cu[c.B];
   const uint64_t rows = min((uint64_t)c.rows, (uint64_t)max(last, 0));
-  const uint64_t total = rows * slots * LPH;
-  uint32_t b = 0;
-  bool first = true;
-  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256u) {
-    const uint32_t lane = (uint32_t)(i % LPH);
-    const uint64_t it = i / LPH;
-    const uint64_t row = it / slots;
-    const uint32_t slot = (uint32_t)(it - row * slots);
-    if (first) {
-      uint32_t hi = c.B;
-      while (hi - b > 1u) {
-        const uint32_t mid = (b + hi) / 2u;
-        if ((int64_t)c.cu[mid] <= (int64_t)row) b = mid;
-        else hi = mid;
-      }
-      first = false;
-    }
-    while (b + 1u < c.B && (int64_t)c.cu[b + 1] <= (int64_t)row) b++;
-    const bool is_v = slot >= c.KV;
-    int16_t* out = is_v ? d.v : d.k;
-    if (!out) continue;
-    const SeqRows s = seq_rows(c, b, c.rows);
-    if (row < s.lo || row >= s.lo + s.n) continue;
-    const uint32_t g = is_v ? slot - c.KV : slot;
-    const uint64_t p = (uint64_t)s.pos + (row - s.lo);
-    const int32_t pg = p < s.cap ? c.table[(uint64_t)b * c.table_width + p / c.page] : -1;
-    uint32_t w[4] = {0, 0, 0, 0};
-    if ((uint32_t)pg < c.pages) {
-      const uint64_t line = ((uint64_t)pg * c.KV + g) * c.page + p % c.page;
-      const int8_t* y = (is_v ? c.vc : c.kc) + line * (c.bits == 8u ? HD : 2 * HD) + 8u * lane;
-      const uint2 h = *(const uint2*)y;
-      if (c.bits == 8u) {
-        const uint32_t sh = (is_v ? c.vs : c.ks)[line];
+  if (row >= rows || row >= row_step) return;
+  const bool b8 = c.bits == 8u;
+  const uint32_t rb = b8 ? HD : 2 * HD, hb = c.page * rb;  // bytes from head to head
+  uint32_t b = first_sequence(c, row);
+#pragma unroll 1
+  for (; row < rows; row += row_step) {
+    const RowAt at = row_at(c, row, b);
+    if (!at.in) continue;
+    const int8_t* const kr = c.kc + at.line * rb + 8u * lane;
+    const int8_t* const vr = c.vc + at.line * rb + 8u * lane;
+    int16_t* const ko = d.k + row * d.ldk + 8u * lane;
+    int16_t* const vo = d.v + row * d.ldv + 8u * lane;
+#pragma unroll 1
+    for (uint32_t t = it0; t < it1; t += U) {
+      uint2 h[U], l[U];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const uint32_t q = k < 2 ? h.x : h.y;
-          const int32_t v0 = (int8_t)(q >> (16 * (k & 1))), v1 = (int8_t)(q >> (16 * (k & 1) + 8));
-          w[k] = pack16(sh < 16u ? v0 << sh : 0, sh < 16u ? v1 << sh : 0);
+      for (uint32_t u = 0; u < U; u++) {
+        const uint32_t i = (t + u) * HPT + sub;
+        const bool is_v = i >= nk;
+        const uint32_t g = is_v ? i - nk : i;
+        h[u] = l[u] = make_uint2(0, 0);
+        if (at.held && t + u < it1 && i < A.heads) {
+          const int8_t* const y = (is_v ? vr : kr) + (uint64_t)g * hb;
+          h[u] = *(const uint2*)y;
+          if (b8) l[u].x = (is_v ? c.vs : c.ks)[at.line + (uint64_t)g * c.page];
+          else l[u] = *(const uint2*)(y + HD);
         }
-      } else {
-        const uint2 l = *(const uint2*)(y + HD);
-        w[0] = __byte_perm(l.x, h.x, 0x5140);
-        w[1] = __byte_perm(l.x, h.x, 0x7362);
-        w[2] = __byte_perm(l.y, h.y, 0x5140);
-        w[3] = __byte_perm(l.y, h.y, 0x7362);
       }
-    }
-    int16_t* o = out + row * (is_v ? d.ldv : d.ldk) + (uint64_t)g * HD + 8u * lane;
-    if (vec) {
-      *(uint4*)o = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        o[2 * k] = (int16_t)w[k];
-        o[2 * k + 1] = (int16_t)(w[k] >> 16);
+      for (uint32_t u = 0; u < U; u++) {
+        const uint32_t i = (t + u) * HPT + sub;
+        const bool is_v = i >= nk;
+        const uint32_t g = is_v ? i - nk : i;
+        if (t + u >= it1 || i >= A.heads) continue;
+        uint32_t w[4];
+        if (b8) {
+          const uint32_t sh = l[u].x;  // (a shift from 16 up leaves nothing)
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const uint32_t q = k < 2 ? h[u].x : h[u].y;
+            const uint32_t v0 = (uint32_t)(int32_t)(int8_t)(q >> (16 * (k & 1))), v1 = (uint32_t)(int32_t)(int8_t)(q >> (16 * (k & 1) + 8));
+            w[k] = sh < 16u ? __byte_perm(v0 << sh, v1 << sh, 0x5410) : 0u;
+          }
+        } else {
+          w[0] = __byte_perm(l[u].x, h[u].x, 0x5140);
+          w[1] = __byte_perm(l[u].x, h[u].x, 0x7362);
+          w[2] = __byte_perm(l[u].y, h[u].y, 0x5140);
+          w[3] = __byte_perm(l[u].y, h[u].y, 0x7362);
+        }
+        int16_t* const o = (is_v ? vo : ko) + (uint64_t)g * HD;
+        if (A.vec) {
+          *(uint4*)o = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            o[2 * k] = (int16_t)w[k];
+            o[2 * k + 1] = (int16_t)(w[k] >> 16);
+          }
+        }
       }
     }
   }
+}
+
+// The launch of a kernel with a warp per row and part: `turns` of work a row in parts of
+// at most `most` turns, smaller ones while the warps that are resident at once (`blocks_sm`
+// blocks of 8 an SM) have fewer than `each` / 2 parts each: the preparation, whose turns
+// are long, evens out its last round (4.5k rows of 12 turns: 76 us against 92); the
+// read-back, short beside a row's lookups, only fills the SMs (14 us against 22)
+struct RowGrid {
+  uint32_t per, parts, grid;
+};
+RowGrid row_grid(uint64_t rows, uint32_t turns, uint32_t most, uint32_t blocks_sm, uint32_t each) {
+  const uint64_t room = 148ull * 8u * blocks_sm;
+  RowGrid g;
+  g.parts = (turns + most - 1u) / most;
+  while (g.parts < turns && rows * g.parts * 2u < each * room) g.parts++;
+  g.per = (turns + g.parts - 1u) / g.parts;
+  g.parts = (turns + g.per - 1u) / g.per;
+  const uint64_t want = (rows * g.parts + 7u) / 8u, least = (g.parts + 7u) / 8u;  // (a row's parts at least)
+  const uint64_t grid = want < room / 8u ? want : room / 8u;
+  g.grid = (uint32_t)(grid < least ? least : grid);
+  return g;
 }
 
 // ---------------------------------------------------------------- attention, few rows
@@ -1087,30 +1200,25 @@ extern "C" int corm_llm_paged_prep(const corm_llm_paged_prep_desc* d, corm_strea
   A.d = *d;
   A.rsq = tb->ro_rsq;
   // 8-byte rows, 16-byte table rows, whole lanes of one kind of pair
-  A.vec = !(((uintptr_t)d->q0 | (uintptr_t)d->k0 | (uintptr_t)d->v0 | (uintptr_t)d->q) & 7u) &&
-          !((d->ldq0 | d->ldk | d->ldv | d->ldq) & 3u) && !((uintptr_t)d->rope & 15u) && d->rot % 8u == 0;
+  const bool vec = !(((uintptr_t)d->q0 | (uintptr_t)d->k0 | (uintptr_t)d->v0 | (uintptr_t)d->q) & 7u) &&
+                   !((d->ldq0 | d->ldk | d->ldv | d->ldq) & 3u) && !((uintptr_t)d->rope & 15u) && d->rot % 8u == 0;
   cudaStream_t st = (cudaStream_t)stream;
-  const uint32_t slots = d->H + 2u * c.KV, spb = 256u / (c.HD / 8u);
-  // a grid whose step is a whole number of rows: every thread keeps its head
-  uint32_t g = slots, r = spb;
-  while (r) {
-    const uint32_t t = g % r;
-    g = r;
-    r = t;
-  }
-  const uint64_t unit = slots / g;  // blocks
-  const uint64_t want = ((uint64_t)c.rows * slots + spb - 1) / spb, most = 148u * 16u;
-  uint64_t grid = ((want < most ? want : most) + unit - 1) / unit * unit;
-  auto launch = [&](auto kern) { corm_launch_pdl(kern, dim3((unsigned)grid), dim3(256), 0, st, A); };
+  const uint32_t hpt = 256u / c.HD;
+  A.turned = (d->H + c.KV + hpt - 1u) / hpt;
+  A.turns = A.turned + (c.KV + hpt - 1u) / hpt;
+  const RowGrid rg = row_grid(c.rows, A.turns, kTurns, 3, 8);
+  A.per = rg.per;
+  A.parts = rg.parts;
+  auto launch = [&](auto kern) { corm_launch_pdl(kern, dim3(rg.grid), dim3(256), 0, st, A); };
   {
     corm::ProfScope prof_("paged_prep_kernel", st);
     auto pick = [&](auto hd) {
       constexpr int W = decltype(hd)::value;
       if (d->nq || d->nk) {
-        if (A.vec) launch(paged_prep_kernel<W, true, true>);
+        if (vec) launch(paged_prep_kernel<W, true, true>);
         else launch(paged_prep_kernel<W, false, true>);
       } else {
-        if (A.vec) launch(paged_prep_kernel<W, true, false>);
+        if (vec) launch(paged_prep_kernel<W, true, false>);
         else launch(paged_prep_kernel<W, false, false>);
       }
     };
@@ -1134,11 +1242,17 @@ extern "C" int corm_llm_paged_read(const corm_llm_paged_read_desc* d, corm_strea
     return corm::fail(CORM_EINVAL, "corm_llm_paged_read: row strides below the row lengths");
   if (((uintptr_t)d->k | (uintptr_t)d->v) & 1u) return corm::fail(CORM_EINVAL, "corm_llm_paged_read: unaligned rows");
   if (int rc = corm::check_device()) return rc;
-  const uint32_t vec = !(((uintptr_t)d->k | (uintptr_t)d->v) & 15u) && !((d->k ? d->ldk : 0) & 7u) &&
-                       !((d->v ? d->ldv : 0) & 7u);
+  ReadArgs A;
+  A.d = *d;
+  A.vec = !(((uintptr_t)d->k | (uintptr_t)d->v) & 15u) && !((d->k ? d->ldk : 0) & 7u) && !((d->v ? d->ldv : 0) & 7u);
+  A.heads = (d->k ? c.KV : 0u) + (d->v ? c.KV : 0u);
   cudaStream_t st = (cudaStream_t)stream;
-  const unsigned grid = corm_blocks((size_t)c.rows * 2u * c.KV * (c.HD / 8u), 256, 148u * 16u);
-  auto launch = [&](auto kern) { corm_launch_pdl(kern, dim3(grid), dim3(256), 0, st, *d, vec); };
+  const uint32_t hpt = 256u / c.HD;
+  A.turns = (A.heads + hpt - 1u) / hpt;
+  const RowGrid rg = row_grid(c.rows, A.turns, A.turns, 6, 1);
+  A.per = rg.per;
+  A.parts = rg.parts;
+  auto launch = [&](auto kern) { corm_launch_pdl(kern, dim3(rg.grid), dim3(256), 0, st, A); };
   {
     corm::ProfScope prof_("paged_read_kernel", st);
     switch (c.HD) {
