@@ -103,6 +103,38 @@ def _param(name: str, words) -> N.TensorInfo:
     return _t(name, (len(words),), data=np.asarray(words, np.float64) / 256.0)
 
 
+def paged_rope(cos, sin) -> np.ndarray:
+    """float32 [positions][HD / 2] tables as PagedAttnNode takes them: int32
+    [positions][HD], cos then sin, at 2^23 (the values of ``rope_table_words``)."""
+    t = np.concatenate([np.asarray(cos, np.float32), np.asarray(sin, np.float32)], 1).astype(np.float64)
+    return np.rint(t * 2.0 ** RH.ROPE_BITS).astype(np.int32)
+
+
+def paged_layer(prefix: str, *, layer: int, rows: int, H: int, KV: int, HD: int, fq0, fk0, fv, fq, fkc, fvc, fp,
+                rope, q0: N.TensorInfo, k0: N.TensorInfo, v: N.TensorInfo, logit_scale: Optional[float] = None,
+                window: int = 0):
+    """One layer's attention over a paged cache as one node, at the exponents
+    ``prefill_layer`` takes, with the same parameter entries and softmax registers
+    (``rope``: ``paged_rope``): a row's words are that chain's.  Returns (nodes, pv)."""
+    fq0, fk0, fv, fq, fkc, fvc, fp = (np.asarray(a, np.int64) for a in (fq0, fk0, fv, fq, fkc, fvc, fp))
+    fkc, fvc = (np.repeat(f, HD) if f.size == KV else np.broadcast_to(f, (KV * HD,)) for f in (fkc, fvc))
+    wq, pq_bc = RH.pblock(0, 0, *RH.rope_params(fq0, H, HD, fq), H * HD)
+    wk, pk_bc = RH.pblock(0, 0, *RH.rope_params(fk0, KV, HD, fkc.reshape(KV, HD)[:, 0]), KV * HD)
+    ins = [q0, k0, v, _param(f"{prefix}.pq", wq), _param(f"{prefix}.pk", wk)]
+    v_direct, pv_bc = bool((np.broadcast_to(fv, (KV * HD,)) == fvc).all()), True
+    if not v_direct:
+        sa, sc = RH.vround_params(fv, fvc)
+        wv, pv_bc = RH.pblock(0, 0, sa, 0, sc, KV * HD)
+        ins.append(_param(f"{prefix}.pv_p", wv))
+    fs = score_exp(fq, fkc.reshape(KV, HD)[:, 0], KV)
+    sigma = 1.0 / math.sqrt(HD) if logit_scale is None else float(logit_scale)
+    smx = np.array([smx_regs(int(fs[h]), sigma, int(fp[h])) for h in range(H)], np.int32)
+    pv_exp = np.repeat(fp, HD) + fvc.reshape(KV, HD)[np.arange(H) // (H // KV)].reshape(-1) - 8
+    pv = _t(f"{prefix}.pv", (rows, H * HD), pv_exp)
+    return [N.PagedAttnNode(inputs=ins, output=pv, layer=layer, rows=rows, H=H, KV=KV, HD=HD, v_direct=v_direct,
+                            pq_bc=pq_bc, pk_bc=pk_bc, pv_bc=pv_bc, window=window, rope=rope, smx=smx)], pv
+
+
 def prefill_layer(prefix: str, *, T: int, H: int, KV: int, HD: int, C: int, fq0, fk0, fv, fq, fkc, fvc, fp,
                   cos, sin, q0: N.TensorInfo, k0: N.TensorInfo, v: N.TensorInfo, pos: N.TensorInfo,
                   n: Optional[N.TensorInfo], ck: N.TensorInfo, cv: N.TensorInfo, pv_exp=None,

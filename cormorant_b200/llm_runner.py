@@ -5,15 +5,21 @@ device between them (``corm_greedy_embed``: the first argmax of each
 sequence's logits and its embedding row as the next input) — the loop the
 reference's host runs between its LLM entries (the prefill entry, then a
 decode entry per token, with LlmDequant / argmax / LlmEmbed on the host).
+
+``PagedLlamaRunner`` serves sequences of any lengths instead: prompts, chunks of
+them and single tokens of several sequences in one pass over a paged KV cache
+(no counterpart in the reference, which runs one sequence at a time).
 """
 from __future__ import annotations
 
-from typing import List, Optional
+from typing import Dict, Hashable, List, Optional, Sequence
 
 import numpy as np
 import torch
 
 from . import ops
+from ._lib import CORM_EINVAL, CormError
+from .paged import PagedBatch, PagedCache, PagePool
 from .simulator import GpuSimulator
 
 
@@ -60,3 +66,107 @@ class LlamaRunner:
             lg = self.decode_step(lg, i, ids[i])
         self.last_logits = lg
         return [r for r in ids.cpu().numpy()]
+
+
+class PagedLlamaRunner:
+    """Passes of a ``workloads.LlamaModel`` over a paged KV cache of ``pages``
+    pages of ``page`` rows (``bits`` 16 or 8) a layer.  A sequence is any hashable
+    name; it comes into being with its first tokens and holds its pages until
+    ``release``.  Every pass takes the unit's softmax, a prompt's and a single
+    token's alike, so at 16 bits a token's words do not depend on how its sequence
+    was cut into passes nor on what ran beside it (with 8 bits nor do they: a row's
+    codes are its own)."""
+
+    def __init__(self, model, pages: int, page: int = 64, bits: int = 16, device=None, fuse: bool = True):
+        self.m, self.fuse = model, fuse
+        self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.caches = [PagedCache(pages, page, model.KV, model.HD, bits, device=self.device) for _ in range(model.L)]
+        self.pool = PagePool(pages, page)
+        self.length: Dict[Hashable, int] = {}
+        emb = np.rint(model.emb * 2.0 ** model.E["fr"]).astype(np.int32)
+        self.table = torch.from_numpy(emb).to(self.device)
+        self._sims: Dict[tuple, GpuSimulator] = {}
+        self._share: Optional[GpuSimulator] = None
+
+    def _sim(self, rows: int, head: bool) -> GpuSimulator:
+        key = (rows, head)
+        if key not in self._sims:
+            g = self.m.head_graph(rows) if head else self.m.paged_graph(rows)
+            self._sims[key] = s = GpuSimulator(g, device=self.device, fuse=self.fuse, share=self._share)
+            self._share = self._share or s
+        return self._sims[key]
+
+    @staticmethod
+    def _padded(rows: int) -> int:
+        """The rows a pass is built for: graphs of few row counts serve all."""
+        return rows if rows <= 16 else -(-rows // 64) * 64
+
+    def _pass(self, seqs: Sequence[Hashable], new: Sequence[int], h: torch.Tensor) -> torch.Tensor:
+        """The layers over h (int32, the new rows packed; whole padded rows), the
+        last row of every sequence through the head: its logits."""
+        m = self.m
+        at = [self.length.get(s, 0) for s in seqs]
+        if len(set(seqs)) != len(seqs) or not seqs or min(new) < 1:
+            raise CormError(CORM_EINVAL, "PagedLlamaRunner: distinct sequences with a token or more each expected")
+        for s, a, n in zip(seqs, at, new):
+            if a + n > m.C:
+                raise CormError(CORM_EINVAL, f"PagedLlamaRunner: sequence {s!r}: {a + n} positions, the model has {m.C}")
+        need = sum(max(-(-(a + n) // self.pool.page) - len(self.pool.held.get(s, [])), 0) for s, a, n in zip(seqs, at, new))
+        if need > len(self.pool.free):
+            raise MemoryError(f"PagedLlamaRunner: {need} pages wanted, {len(self.pool.free)} free (no sequence changed)")
+        tables = [self.pool.extend(s, a + n) for s, a, n in zip(seqs, at, new)]
+        batch = PagedBatch.of(tables, new, at, device=self.device)
+        sim = self._sim(self._padded(batch.rows), False)
+        sim.paged = (self.caches, batch)
+        out = sim._graph.output_tensors[0].onnx_name
+        try:
+            res, _ = sim.forward_raw({"h_step": h}, keep=[out])
+        finally:
+            sim.paged = None
+        B = len(seqs)
+        last = torch.empty(B * m.D + 4, dtype=torch.int32, device=self.device)
+        rows = res[out][:batch.rows * m.D].view(batch.rows, m.D)
+        torch.index_select(rows, 0, batch.cu[1:] - 1, out=last[:B * m.D].view(B, m.D))
+        head = self._sim(B, True)
+        out = head._graph.output_tensors[0].onnx_name
+        res, _ = head.forward_raw({"h_step": last}, keep=[out])
+        self.length.update({s: a + n for s, a, n in zip(seqs, at, new)})
+        return res[out]
+
+    def _rows(self, rows: int) -> torch.Tensor:
+        return torch.zeros(self._padded(rows) * self.m.D + 4, dtype=torch.int32, device=self.device)
+
+    def append(self, seqs: Sequence[Hashable], ids: Sequence[Sequence[int]]) -> torch.Tensor:
+        """One pass over new tokens of some sequences (prompts, chunks, single
+        tokens together): int16 logits [len(seqs)][vocab] of their last ones."""
+        new = [len(i) for i in ids]
+        if len(new) != len(seqs):
+            raise CormError(CORM_EINVAL, f"PagedLlamaRunner: {len(seqs)} sequences, tokens of {len(new)}")
+        flat = np.concatenate([np.asarray(i, np.int64).reshape(-1) for i in ids]) if new else np.zeros(0, np.int64)
+        if flat.size and (flat.min() < 0 or flat.max() >= self.m.vocab):
+            raise CormError(CORM_EINVAL, f"PagedLlamaRunner: token ids in [0, {self.m.vocab}) expected")
+        h, n = self._rows(flat.size), flat.size * self.m.D
+        torch.index_select(self.table, 0, torch.from_numpy(flat).to(self.device), out=h[:n].view(flat.size, self.m.D))
+        return self._pass(seqs, new, h)
+
+    def step(self, seqs: Sequence[Hashable], logits: torch.Tensor, ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """A greedy token for each of ``seqs`` after ``logits`` (their order),
+        chosen on the device (int32 ``ids`` if given); its logits."""
+        h = self._rows(len(seqs))
+        ops.greedy_embed(logits, self.table, h, ids, batch=len(seqs), vocab=self.m.vocab, dim=self.m.D)
+        return self._pass(seqs, [1] * len(seqs), h)
+
+    def generate(self, prompts: Dict[Hashable, Sequence[int]], steps: int) -> Dict[Hashable, List[int]]:
+        """The prompts in one pass, then ``steps`` greedy tokens of each."""
+        seqs = list(prompts)
+        lg = self.append(seqs, [prompts[s] for s in seqs])
+        ids = torch.empty((steps, len(seqs)), dtype=torch.int32, device=self.device)
+        for i in range(steps):
+            lg = self.step(seqs, lg, ids[i])
+        self.last_logits = lg
+        return dict(zip(seqs, ids.cpu().numpy().T.tolist()))
+
+    def release(self, seq: Hashable) -> None:
+        """Ends a sequence; its pages are free."""
+        self.pool.release(seq)
+        self.length.pop(seq, None)

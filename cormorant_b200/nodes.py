@@ -433,6 +433,32 @@ class LlmAttnMergeNode:
 
 
 @dataclass
+class PagedAttnNode:
+    """One layer's attention over a paged KV cache (no counterpart in the
+    reference, whose caches are contiguous): the rows of a batch of sequences,
+    packed, prepared (RoPE at each row's position, q rotated, k and the re-rounded
+    v into the pages) and attended causally with the unit's softmax.  inputs =
+    [q0, k0, v, pq, pk, (pvb)]; output [rows][H HD]; ``rope`` int32 [positions][HD]
+    (cos, then sin, at 2^23), ``smx`` int32 [H][2]; ``layer`` names the cache the
+    pass holds."""
+    inputs: List[TensorInfo]
+    output: TensorInfo
+    layer: int = 0
+    rows: int = 1
+    H: int = 1
+    KV: int = 1
+    HD: int = 16
+    v_direct: bool = False
+    pq_bc: bool = False
+    pk_bc: bool = False
+    pv_bc: bool = True
+    window: int = 0
+    rope: Optional[np.ndarray] = field(default=None, repr=False)
+    smx: Optional[np.ndarray] = field(default=None, repr=False)
+    onnx_node: object = None
+
+
+@dataclass
 class LlmSelectRowNode:
     """y = h[n - 1] with n clamped to [1, rows] — the last valid row of a
     padded prefill (llm_nodes.py:1663-1718); ``res32``: h / y int32 DMA

@@ -104,6 +104,7 @@ class GpuSimulator:
         self._groups = self._sibling_groups() if fuse else {}
         self._pairs = self._rowops_pairs() if fuse else {}
         self._mulacts = self._mulact_pairs() if fuse else {}
+        self.paged = None  # a pass over paged caches: (a PagedCache a layer, its PagedBatch)
 
     # ------------------------------------------------------------ tensors
     def _alloc(self, numel: int) -> torch.Tensor:
@@ -457,6 +458,8 @@ class GpuSimulator:
                 y = self._attn_merge(sn, get)
             elif kind == "LlmSelectRowNode":
                 y = self._select_row(sn, get)
+            elif kind == "PagedAttnNode":
+                y = self._paged_attn(sn, get)
             elif kind in ("LlmEmbedNode", "LlmDequantNode", "LlmToHostNode", "LlmResAddNode", "LlmRMSNormNode",
                           "LlmSiluMulNode", "LlmGeluMulNode"):
                 y = self._llm_host(sn, kind, get)
@@ -1232,6 +1235,27 @@ class GpuSimulator:
                                self._exps8(("fq", sn.output.onnx_name), np.asarray(sn.fq, np.int64)),
                                pos=pos, n=n, T=T, H=H, KV=KV, HD=HD, C_=C, Q=sn.Q, batch=B)
         return qx
+
+    def _paged_attn(self, sn, get):
+        """PagedAttnNode on the pass's caches and batch (``paged``: a cache a
+        layer, and the PagedBatch of its rows)."""
+        if self.paged is None:
+            raise ValueError("PagedAttnNode: the pass holds no paged cache (GpuSimulator.paged)")
+        caches, batch = self.paged
+        q0, k0, v = (get(t) for t in sn.inputs[:3])
+        pq, pk = get(sn.inputs[3]), get(sn.inputs[4])
+        pv = None if sn.v_direct else get(sn.inputs[5])
+
+        def table(key, data):  # int32, on the device once for all passes that share the weights
+            if key not in self._weights:
+                self._weights[key] = torch.from_numpy(np.ascontiguousarray(data, np.int32)).to(self.device)
+            return self._weights[key]
+        rope, smx = table(("paged.rope", id(sn.rope)), sn.rope), table(("paged.smx", sn.smx.tobytes()), sn.smx)
+        q, y = self._alloc(sn.output.numel), self._alloc(sn.output.numel)
+        ops.llm_paged_prep(caches[sn.layer], batch, q0, k0, v, q, H=sn.H, rope=rope, pq=pq, pk=pk, pv=pv,
+                           pq_bc=sn.pq_bc, pk_bc=sn.pk_bc, pv_bc=sn.pv_bc, v_direct=sn.v_direct)
+        ops.llm_paged_attn(caches[sn.layer], batch, q, y, H=sn.H, smx=smx, window=sn.window)
+        return y
 
     def _select_row(self, sn, get):
         """h[n - 1], n clamped to [1, rows] (llm_nodes.py:1713-1717), of every

@@ -421,6 +421,7 @@ class LlamaModel:
         inv = 1.0 / theta ** (np.arange(0, head_dim, 2, dtype=np.float64) / head_dim)
         ang = np.outer(np.arange(C, dtype=np.float64), inv)
         self.cos, self.sin = np.cos(ang).astype(np.float32), np.sin(ang).astype(np.float32)
+        self.rope = None
         self.emb = rng.normal(0.0, 0.02, (vocab, D))
         self.first = first
         self.ids = _per_unit(seed, first, batch, lambda r: r.integers(0, vocab, size=seq))
@@ -429,13 +430,23 @@ class LlamaModel:
         self.prefill_feeds = {"h0": self.emb[self.ids].reshape(batch * seq, D), "pos": np.array([0]),
                               "n": np.array([seq])}
 
-    def _graph(self, T: int, prefill: bool):
+    def paged_graph(self, rows: int):
+        """The layers over ``rows`` packed rows of any sequences and a paged KV
+        cache (PagedAttnNode): the int32 residual rows in and out."""
+        return self._graph(0, False, rows)
+
+    def head_graph(self, rows: int):
+        """The final RMSNorm and the LM head of ``rows`` residual rows."""
+        return self._graph(0, False, rows, head=True)
+
+    def _graph(self, T: int, prefill: bool, rows: int = None, head: bool = False):
         from . import attention as AT
         E, B, D, H, KV, HD, C = self.E, self.B, self.D, self.H, self.KV, self.HD, self.C
-        nq, nk, ffn, R = H * HD, KV * HD, self.ffn, B * T
+        paged = rows is not None
+        nq, nk, ffn, R = H * HD, KV * HD, self.ffn, rows if paged else B * T
         weights: List[N.TensorInfo] = []
         nodes: list = []
-        tag = "p" if prefill else "d"
+        tag = "g" if paged else ("p" if prefill else "d")
 
         def ten(name, shape, exp=None, **kw):
             return N.TensorInfo(f"{tag}.{name}", list(shape), exp=None if exp is None else np.asarray(exp, np.int64),
@@ -470,19 +481,25 @@ class LlamaModel:
         h = h0 = N.TensorInfo("h0" if prefill else "h_step", [R, D], exp=np.asarray(E["fr"], np.int64), dma="i32")
         pos = N.TensorInfo("pos", [1], host="i32")
         n_t = N.TensorInfo("n", [1], host="i32") if prefill else None
-        for li in range(self.L):
+        for li in range(0 if head else self.L):
             lw = self.w[li]
             x = rmsnorm(f"l{li}.x", h, E["fx"])
             q0 = linear(f"l{li}.q0", x, lw["q0"], E["fq0"])
             k0 = linear(f"l{li}.k0", x, lw["k0"], E["fk0"])
             v = linear(f"l{li}.v", x, lw["v"], E["fv"])
-            ck, cv = self.states[2 * li], self.states[2 * li + 1]
-            chain, pv = AT.prefill_layer(f"{tag}.l{li}.attn", T=T, H=H, KV=KV, HD=HD, C=C, fq0=np.full(nq, E["fq0"]),
-                                         fk0=np.full(nk, E["fk0"]), fv=np.full(nk, E["fv"]), fq=np.full(H, E["fq"]),
-                                         fkc=np.full(KV, E["fkc"]), fvc=np.full(KV, E["fvc"]),
-                                         fp=np.full(H, E["fp"]), cos=self.cos, sin=self.sin, q0=q0, k0=k0, v=v,
-                                         pos=pos, n=n_t, ck=ck, cv=cv, batch=B,
-                                         softmax="unit" if prefill else "host")
+            exps = dict(fq0=np.full(nq, E["fq0"]), fk0=np.full(nk, E["fk0"]), fv=np.full(nk, E["fv"]),
+                        fq=np.full(H, E["fq"]), fkc=np.full(KV, E["fkc"]), fvc=np.full(KV, E["fvc"]),
+                        fp=np.full(H, E["fp"]), q0=q0, k0=k0, v=v)
+            if paged:
+                if self.rope is None:  # one table for the layers of all paged graphs
+                    self.rope = AT.paged_rope(self.cos, self.sin)
+                chain, pv = AT.paged_layer(f"{tag}.l{li}.attn", layer=li, rows=R, H=H, KV=KV, HD=HD, rope=self.rope,
+                                           **exps)
+            else:
+                ck, cv = self.states[2 * li], self.states[2 * li + 1]
+                chain, pv = AT.prefill_layer(f"{tag}.l{li}.attn", T=T, H=H, KV=KV, HD=HD, C=C, pos=pos, n=n_t, ck=ck,
+                                             cv=cv, batch=B, softmax="unit" if prefill else "host", cos=self.cos,
+                                             sin=self.sin, **exps)
             for nd in chain:
                 for t in nd.inputs:
                     if t is not None and t.data is not None and all(t is not w for w in weights):
@@ -503,12 +520,13 @@ class LlamaModel:
             last = ten("h_last", (B, D), E["fr"], dma="i32")
             nodes.append(N.LlmSelectRowNode(inputs=[h, n_t], output=last, rows=T, n=D, res32=True, batch=B))
             h = last
-        xf = rmsnorm("xf", h, E["fx"], rows=B)
-        logits = linear("logits", xf, self.w_lm, E["fl"], rows=B)
-        ins = [h0, pos] + ([n_t] if prefill else [])
+        ins, out = [h0] if paged else [h0, pos] + ([n_t] if prefill else []), h
+        if head or not paged:
+            xf = rmsnorm("xf", h, E["fx"], rows=rows if paged else B)
+            out = linear("logits", xf, self.w_lm, E["fl"], rows=rows if paged else B)
         weights = list({w.onnx_name: w for w in weights}.values())
-        return N.Graph(nodes=nodes, weight_tensors=weights, input_tensors=ins, output_tensors=[logits],
-                       state_tensors=list(self.states))
+        return N.Graph(nodes=nodes, weight_tensors=weights, input_tensors=ins, output_tensors=[out],
+                       state_tensors=[] if paged else list(self.states))
 
     def macs_per_token(self, keys: int, prefill: bool = True) -> float:
         """Int16 MACs per token of a pass: the projections, the attention at

@@ -1,0 +1,193 @@
+"""A Llama model served over the paged KV cache (llm_runner.PagedLlamaRunner):
+prompts of unlike lengths, chunks and single tokens in one pass, sequences that
+come, end and leave their pages to others, against the contiguous prefill graph
+(with the same softmax unit) run over each sequence's whole tokens."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from cormorant_b200 import workloads as WL  # noqa: E402
+from cormorant_b200._lib import CormError  # noqa: E402
+from cormorant_b200.llm_runner import PagedLlamaRunner  # noqa: E402
+from oracle import paged as OP  # noqa: E402
+
+gpu = pytest.mark.gpu
+SMALL = dict(layers=1, hidden=64, heads=4, kv_heads=2, head_dim=16, ffn=128, vocab=50)
+
+
+@pytest.fixture
+def paged_cpu(cpu_ops, monkeypatch):
+    """The paged operators replayed on the oracle over CPU tensors, beside the
+    other kernels' job models."""
+    from cormorant_b200 import ops
+
+    def host(cache, batch):
+        a = [None if t is None else t.numpy() for t in (cache.kc, cache.vc, cache.ks, cache.vs, batch.table, batch.cu,
+                                                        batch.pos)]
+        return OP.Cache(*a, cache.HD, cache.bits)
+
+    def rows(t, n, w):
+        return t.numpy().reshape(-1)[:n * w].reshape(n, w)
+
+    def prep(cache, batch, q0, k0, v0, q, *, H, rope, pq, pk, pv=None, rot=None, interleaved=False, pq_bc=False,
+             pk_bc=False, pv_bc=False, v_direct=False, **kw):
+        assert not kw
+        R, nq, nk = batch.rows, H * cache.HD, cache.KV * cache.HD
+        out = np.zeros((R, nq), np.int64)
+
+        def ent(t, bc, n):
+            e = t.numpy()[:8 if bc else 8 * n]
+            return e.astype(np.int16)
+        OP.prep(host(cache, batch), rows(q0, R, nq).astype(np.int64), rows(k0, R, nk).astype(np.int64),
+                rows(v0, R, nk).astype(np.int64), out, H=H, rope=rope.numpy().reshape(-1, cache.HD).astype(np.int64),
+                rot=cache.HD, interleaved=False, pq=ent(pq, pq_bc, nq), pk=ent(pk, pk_bc, nk),
+                pv=None if v_direct else ent(pv, pv_bc, nk))
+        rows(q, R, nq)[...] = out
+
+    def attn(cache, batch, q, o, *, H, smx, window=0):
+        R, n = batch.rows, H * cache.HD
+        out = np.zeros((R, n), np.int64)
+        OP.attn(host(cache, batch), rows(q, R, n).astype(np.int64), out, H=H, smx=smx.numpy(), window=window)
+        rows(o, R, n)[...] = out
+    monkeypatch.setattr(ops, "llm_paged_prep", prep)
+    monkeypatch.setattr(ops, "llm_paged_attn", attn)
+
+
+def _words(logits, n, vocab):
+    return logits[:n * vocab].cpu().numpy().reshape(n, vocab)
+
+
+def _contiguous(dims, seq, tokens, device):
+    """The contiguous prefill's logits after the tokens, and its model."""
+    from cormorant_b200.simulator import GpuSimulator
+    m = WL.LlamaModel(batch=1, seq=seq, **dims)
+    sim = GpuSimulator(m.prefill_graph, device=device)
+    out = m.prefill_graph.output_tensors[0].onnx_name
+    got = []
+    for t in tokens:
+        h = np.zeros((seq, m.D))
+        h[:len(t)] = m.emb[np.asarray(t)]
+        feeds = {"h0": h, "pos": np.array([0]), "n": np.array([len(t)])}
+        raw = {x.onnx_name: (np.asarray(feeds[x.onnx_name]).astype(np.int64).reshape(-1) if x.host
+                             else sim._to_raw(x, feeds[x.onnx_name])) for x in m.prefill_graph.input_tensors}
+        res, _ = sim.forward_raw(raw, keep=[out], states=sim.states_to_device())
+        got.append(_words(res[out], 1, m.vocab)[0])
+    return np.stack(got)
+
+
+def _served(dims, device, lengths, steps, seq, page, bits=16, chunk=5):
+    """Two sequences from their prompts, a third joining in chunks while they
+    decode, then one ended and its pages taken by a fourth; every pass's logits
+    with the tokens that lead to them."""
+    m = WL.LlamaModel(batch=1, seq=seq, **dims)
+    rng = np.random.default_rng(1)
+    prompt = {s: rng.integers(0, m.vocab, n).tolist() for s, n in zip("abcd", lengths)}
+    pages = sum(-(-(lengths[i] + 3 * steps) // page) for i in range(3)) + 1
+    r = PagedLlamaRunner(m, pages=pages, page=page, bits=bits, device=device)
+    seen = []
+
+    def note(tokens, logits):
+        seen.extend(zip([list(t) for t in tokens], _words(logits, len(tokens), m.vocab)))
+    tok = {s: list(prompt[s]) for s in "ab"}
+    lg = r.append("ab", [tok["a"], tok["b"]])
+    note([tok["a"], tok["b"]], lg)
+    ids = torch.empty(2, dtype=torch.int32, device=r.device)
+    for _ in range(steps):
+        lg = r.step("ab", lg, ids)
+        for s, t in zip("ab", ids.tolist()):
+            tok[s].append(t)
+        note([tok["a"], tok["b"]], lg)
+    tok["c"] = []
+    while len(tok["c"]) < lengths[2]:  # a chunk of c beside a token of a and b
+        best = _words(lg, 2, m.vocab).argmax(1)
+        new = prompt["c"][len(tok["c"]):len(tok["c"]) + chunk]
+        for s, t in zip("ab", best.tolist()):
+            tok[s].append(t)
+        tok["c"] += new
+        lg = r.append("acb", [tok["a"][-1:], new, tok["b"][-1:]])
+        note([tok["a"], tok["c"], tok["b"]], lg)
+        lg = torch.from_numpy(_words(lg, 3, m.vocab)[[0, 2]].reshape(-1).copy()).to(r.device)
+    r.release("a")
+    free = len(r.pool.free)
+    lg = r.append("d", [prompt["d"]])
+    note([prompt["d"]], lg)
+    assert r.length == dict(b=len(tok["b"]), c=lengths[2], d=lengths[3]) and len(r.pool.free) < free
+    return m, seen
+
+
+def test_runner_host_logic_cpu(paged_cpu):
+    dims = dict(SMALL, seed=4)
+    _, seen = _served(dims, "cpu", (9, 3, 7, 12), 2, 32, 16)
+    want = _contiguous(dims, 32, [t for t, _ in seen], "cpu")
+    assert len(seen) >= 10
+    for (t, got), w in zip(seen, want):
+        assert np.array_equal(got, w), len(t)
+
+
+def test_runner_refuses(paged_cpu):
+    m = WL.LlamaModel(batch=1, seq=16, cache=32, seed=4, **SMALL)
+    r = PagedLlamaRunner(m, pages=2, page=16, device="cpu")
+    for seqs, ids in (("ab", [[1]]), ("aa", [[1], [2]]), ("a", [[]]), ("a", [[50]]), ("a", [[-1]]), ([], []),
+                      ("a", [[1] * 33])):
+        with pytest.raises(CormError):
+            r.append(seqs, ids)
+    with pytest.raises(MemoryError):
+        r.append("abc", [[1], [2], [3]])
+    assert not r.pool.held and not r.length and len(r.pool.free) == 2
+    r.append("ab", [[1] * 16, [2]])
+    with pytest.raises(MemoryError):
+        r.append("ba", [[1], [1]])  # a has no page for its 17th token; b is as it was
+    assert r.length == dict(a=16, b=1)
+    r.release("b")
+    r.append("a", [[1]])
+    assert r.length == dict(a=17)
+
+
+@gpu
+@pytest.mark.parametrize("dims,lengths,page", [
+    (dict(layers=2, hidden=64, heads=4, kv_heads=2, head_dim=16, ffn=128, vocab=300), (9, 3, 70, 40), 16),
+    (dict(layers=2, hidden=960, heads=15, kv_heads=5, head_dim=64, ffn=256, vocab=500), (33, 100, 61, 90), 64),
+    (dict(layers=1, hidden=512, heads=4, kv_heads=4, head_dim=128, ffn=256, vocab=300), (5, 130, 40, 60), 32)],
+    ids=["hd16", "hd64", "hd128"])
+def test_gpu_runner_is_the_contiguous_model(dims, lengths, page):
+    from cormorant_b200 import ops
+    dims = dict(dims, seed=6)
+    _, seen = _served(dims, None, lengths, 3, 160, page, chunk=33)
+    want = _contiguous(dims, 160, [t for t, _ in seen], None)
+    for (t, got), w in zip(seen, want):
+        assert np.array_equal(got, w), len(t)
+    assert ops.device_status() == 0
+
+
+@gpu
+def test_gpu_runner_8_bit_pages():
+    """8-bit pages: a token's words do not depend on the cut into passes."""
+    dims = dict(layers=2, hidden=256, heads=8, kv_heads=2, head_dim=32, ffn=256, vocab=200, seed=8)
+    m = WL.LlamaModel(batch=1, seq=64, **dims)
+    rng = np.random.default_rng(3)
+    ids = rng.integers(0, 200, 40).tolist()
+    got = []
+    for cuts in ([40], [1] * 40, [7, 30, 1, 2]):
+        r = PagedLlamaRunner(m, pages=6, page=16, bits=8)
+        at = 0
+        for i, c in enumerate(cuts):
+            if i == 1:  # company
+                r.append("x", [ids[:9]])
+            lg = r.append("a", [ids[at:at + c]])
+            at += c
+        got.append(_words(lg, 1, 200))
+    assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+
+
+@gpu
+def test_gpu_runner_generate():
+    """Greedy tokens of several prompts at once are those of each alone."""
+    dims = dict(layers=2, hidden=960, heads=15, kv_heads=5, head_dim=64, ffn=256, vocab=500, seed=2)
+    m = WL.LlamaModel(batch=1, seq=64, **dims)
+    rng = np.random.default_rng(5)
+    prompts = {s: rng.integers(0, 500, n).tolist() for s, n in (("p", 17), ("q", 1), ("r", 45))}
+    r = PagedLlamaRunner(m, pages=8, page=64)
+    both = r.generate(prompts, 5)
+    for s, p in prompts.items():
+        assert PagedLlamaRunner(m, pages=2, page=64).generate({s: p}, 5)[s] == both[s]
