@@ -1,8 +1,8 @@
 // corm_llm_paged_attn on 128-row tiles (prompts and chunks): tcgen05 kind::i8
 // on the cache's byte planes.
 //
-// Persistent: a CTA an SM takes items = (128-row tile, sequence, KV head), the rows that
-// see most first, a row being (token, head of the group), token-major; with few items a
+// Persistent: a CTA an SM takes items = (128-row tile, sequence, KV head), the ones that
+// see most keys first, a row being (token, head of the group), token-major; with few items a
 // cluster of CTAs shares an item's keys.  As in the 16-row kernel, the unit's e(d) is a
 // table of d = m - score, so nothing can be rescaled as a running maximum moves: three
 // phases over the scores, which stay in shared memory (int16, then e in place) where the
@@ -25,6 +25,7 @@
 // Every sum is modulo 2^32, the rule's own wrap.
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 
@@ -68,6 +69,7 @@ struct TileArgs {
   int* err;
   uint32_t G, X, stages, win;  // win: tiles of a window
   uint32_t tiles;              // row tiles of the longest sequence
+  uint32_t by_seq;             // items in the order of the sequences' lengths
   uint32_t k8, k16;            // 2^8 and 2^16, as operands (shifts would go to the busier pipe)
 };
 
@@ -147,11 +149,21 @@ struct Item {
   uint32_t t0, t1;                // key tiles
 };
 // Item i (tiles of the last rows first, as they see most); false: its tile has no rows.
-__device__ __forceinline__ bool item_at(const TileArgs& A, uint32_t i, uint32_t rank, Item& o) {
+__device__ __forceinline__ bool item_at(const TileArgs& A, uint32_t i, uint32_t rank, uint32_t order, Item& o) {
   const corm_paged_cache& c = A.d.c;
-  const uint32_t per_tile = c.B * c.KV, tile = A.tiles - 1u - i / per_tile, rem = i % per_tile, G = A.G, w = A.d.window;
-  o.b = rem / c.KV;
-  o.g = rem % c.KV;
+  const uint32_t G = A.G, w = A.d.window;
+  uint32_t tile;
+  if (A.by_seq) {
+    const uint32_t per = A.tiles * c.KV, rem = i % per;
+    o.b = __shfl_sync(0xffffffffu, order, i / per);
+    tile = A.tiles - 1u - rem / c.KV;
+    o.g = rem % c.KV;
+  } else {
+    const uint32_t per = c.B * c.KV, rem = i % per;
+    tile = A.tiles - 1u - i / per;
+    o.b = rem / c.KV;
+    o.g = rem % c.KV;
+  }
   const SeqRows s = seq_rows(c, o.b, c.rows);
   const uint32_t all = min(s.n, A.d.max_q) * G;  // < 2^31 (the host checks)
   o.r0 = tile * BMR;
@@ -167,6 +179,24 @@ __device__ __forceinline__ bool item_at(const TileArgs& A, uint32_t i, uint32_t 
   o.t0 = tile0 + min(rank * per, n);
   o.t1 = tile0 + min(rank * per + per, n);
   return true;
+}
+
+// Lane k's sequence is the one with the k-th most keys (B <= 32)
+__device__ __forceinline__ uint32_t order_of(const TileArgs& A, uint32_t lane) {
+  const corm_paged_cache& c = A.d.c;
+  uint32_t keys = 0;
+  if (lane < c.B) {
+    const SeqRows s = seq_rows(c, lane, c.rows);
+    keys = s.n ? min(s.pos + min(s.n, A.d.max_q), s.cap) : 0u;
+  }
+  uint32_t rank = 0, order = 0;
+  for (uint32_t i = 0; i < c.B; i++) {
+    const uint32_t k = __shfl_sync(0xffffffffu, keys, i);
+    rank += k > keys || (k == keys && i < lane);
+  }
+  for (uint32_t i = 0; i < c.B; i++)
+    if (__shfl_sync(0xffffffffu, rank, i) == lane) order = i;
+  return order;
 }
 
 // The grid has a CTA (cluster) an item; those that run take over the ones not yet
@@ -258,6 +288,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       sm100::prefetch_tmap(&map_v);
     }
     const uint32_t sub = min(c.page, BK), pieces = BK / sub, psh = 31u - __clz(c.page);
+    const uint32_t order = A.by_seq ? order_of(A, lane) : 0u;
     uint32_t gi = 0, asked = 0, answered = 0;
     bool ok = true;
     auto item_slot = [&]() {  // the slot's readers of ITEMS items ago are done
@@ -292,7 +323,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     // publishes the first item with rows from number `at` on, or the end
     auto find = [&](int32_t at, Item& o) {
-      while (at >= 0 && !item_at(A, (uint32_t)at, rank, o)) {
+      while (at >= 0 && !item_at(A, (uint32_t)at, rank, order, o)) {
         ask();
         at = taken();
       }
@@ -977,6 +1008,37 @@ bool make_row_map(CUtensorMap* map, const void* base, uint32_t rb, uint64_t line
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+constexpr uint32_t kTileSmem = 203u * 1024u;  // dynamic, of the 227 KB: the static arrays take 24
+
+// how many clusters of X CTAs the current device holds at once (asked for once)
+template <int HD, int BITS>
+uint32_t resident_clusters(uint32_t X) {
+  static std::atomic<int> known[16][9];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 16)
+    if (const int n = known[dev][X].load(std::memory_order_relaxed)) return (uint32_t)n - 1u;
+  auto kern = paged_attn_tile_kernel<HD, BITS>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(X * 1024u);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = kTileSmem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = X;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  if (dev < 16) known[dev][X].store(n + 1, std::memory_order_relaxed);
+  return (uint32_t)n;
+}
+
 template <int HD, int BITS>
 int launch(TileArgs A, uint32_t tiles, cudaStream_t st) {
   using Sh = Shape<HD, BITS>;
@@ -994,14 +1056,29 @@ int launch(TileArgs A, uint32_t tiles, cudaStream_t st) {
   const uint32_t ktiles = ((span < keys ? span : keys) + BK - 1u) / BK + 1u;
   const uint64_t blocks = (uint64_t)c.B * c.KV * tiles;
   if (blocks > (1ull << 27)) return corm::fail(CORM_ELIMIT, "corm_llm_paged_attn: max_q %u over %u sequences", A.d.max_q, c.B);
-  // two stages of at most 32 KB (a tile's copies are short beside its integer work);
-  // the rest of the 227 KB, less 24 KB of static arrays, for scores
+  // two stages of at most 32 KB (a tile's copies are short beside its integer work); the
+  // rest for scores
   A.stages = Sh::STAGE > 16384u ? 2u : 32768u / Sh::STAGE;
   const uint32_t tile_bytes = TILE_BYTES + (BITS == 8 ? 2u * BK : 0u);
-  const uint32_t most = (203u * 1024u - 1024u - A.stages * Sh::STAGE) / tile_bytes;
+  const uint32_t most = (kTileSmem - 1024u - A.stages * Sh::STAGE) / tile_bytes;
+  // Shares of an item's keys.  A cluster's items cost its tiles of keys and the time of
+  // about 3.5 more, a round of those at once resident or (unlike lengths overlap) a little
+  // less than the items by those; without clusters a CTA goes from item to item.  8k keys
+  // of 128 dimensions: 16 items 466 us with 1, 257 with 2, 144 with 4, 185 with 8; 36 items
+  // 484, 257, 287, 279; 144 items of unlike lengths 489, 364; one prompt of 8192 1267, 1441
   uint32_t X = 1;
-  while (X < 8u && blocks * 2u * X <= 148u && ktiles >= 4u * X) X *= 2u;
+  float best = 0.0f;
+  for (uint32_t x = 1; x <= 8u && (x == 1u || ktiles >= 4u * x); x *= 2u) {
+    const float at_once = x == 1u ? 148.0f : (float)resident_clusters<HD, BITS>(x);
+    if (at_once < 1.0f) continue;
+    const float rounds = (float)blocks / at_once, least = c.B == 1u ? 2.0f : 1.5f;
+    const float cost = (rounds <= 1.0f ? 1.0f : (0.9f * rounds > least ? 0.9f * rounds : least)) * ((float)ktiles / (float)x + 3.5f);
+    if (x == 1u || cost < best) X = x, best = cost;
+  }
   A.X = X;
+  // the rows that see most first: a prompt's last tiles, or, where most keys were there
+  // before the rows, the tiles of the sequences with most
+  A.by_seq = c.B <= 32u && keys / 2u >= A.d.max_q;
   const uint32_t need = (ktiles + X - 1u) / X;
   A.win = need < 2u ? 2u : (need < most ? need : most);  // (a cluster's sums take up to two tiles' memory)
   const size_t smem = 1024u + A.stages * Sh::STAGE + (size_t)A.win * tile_bytes;

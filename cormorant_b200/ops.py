@@ -328,33 +328,39 @@ def llm_decode_attn(qx, kc, vc, tab, ip, o, *, pos, B, KV, G, HD, rows, Q=16, wi
     check(lib().corm_llm_decode_attn(C.byref(d), st))
 
 
-def _ld(t, n, ld):
-    """A row stride: as given, or a 2-D tensor's own, or dense."""
-    return int(ld) if ld is not None else (t.stride(0) if t is not None and t.dim() == 2 and t.shape[0] > 1 else n)
-
-
-def _rows(t, dt, name, rows, n, ld, dev):
-    """A packed array's address: dtype, device and memory checked for rows of
-    n elements at row stride ld (a view of a wider array, too)."""
-    if t.dtype != dt or t.device != dev:
-        raise CormError(_lib.CORM_EINVAL, f"{name}: a {dt} tensor on {dev} expected, got {t.dtype} on {t.device}")
-    need = (rows - 1) * ld + n if rows else 0
-    if ld < n or t.numel() < need or not t.is_contiguous():
-        room = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+def _rows(t, name, rows, n, ld, dev):
+    """(address, row stride) of a packed int16 array: rows of n elements at
+    stride ld (None: a 2-D tensor's own, or dense), a view of a wider array, too;
+    type, device and memory checked."""
+    if t.dtype is not torch.int16 or t.get_device() != dev:
+        raise CormError(_lib.CORM_EINVAL, f"{name}: torch.int16 on device {dev} expected, got {t.dtype} on {t.device}")
+    shape = t.shape
+    if ld is None:
+        ld = n if len(shape) != 2 or shape[0] <= 1 else t.stride(0)
+    if ld < n or t.numel() < (rows - 1) * ld + n or not t.is_contiguous():
+        room, need = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset(), (rows - 1) * ld + n if rows else 0
         if ld < n or room < need or (t.numel() > 1 and t.stride(-1) != 1):
-            raise CormError(_lib.CORM_EINVAL, f"{name}: {rows} rows of {n} at stride {ld} expected, got {tuple(t.shape)}")
-    return t.data_ptr()
+            raise CormError(_lib.CORM_EINVAL, f"{name}: {rows} rows of {n} at stride {ld} expected, got {tuple(shape)}")
+    return t.data_ptr(), ld
 
 
 def _paged(cache, batch):
-    """The cache's descriptor for a batch, on the current device and stream."""
+    """The cache's descriptor for a batch, the current device and its stream."""
     c = cache.desc(batch)
-    if cache.device.type != "cuda":
+    if cache.index < 0:
         raise CormError(_lib.CORM_EINVAL, "the paged cache is not on a CUDA device (the library has no CPU path)")
     st = _ready()
-    if cache.device.index != _tls.dev:
+    if cache.index != _tls.dev:
         raise CormError(_lib.CORM_EINVAL, f"the paged cache is on {cache.device}, the current device is {_tls.dev}")
-    return c, st
+    return c, st, cache.index
+
+
+def _entries(t, n, name, dev):
+    if t is None:
+        return None
+    if t.get_device() != dev or not t.is_contiguous() or t.numel() * t.element_size() < 16 * n:
+        raise CormError(_lib.CORM_EINVAL, f"{name}: {n} 16-byte entries on device {dev} expected")
+    return t.data_ptr()
 
 
 def llm_paged_prep(cache, batch, q0, k0, v0, q, *, H, rope, pq, pk, pv=None, rot=None, interleaved=False, pq_bc=False,
@@ -365,27 +371,23 @@ def llm_paged_prep(cache, batch, q0, k0, v0, q, *, H, rope, pq, pk, pv=None, rot
     ``rot`` dimensions by ``rope`` int32 [positions][rot], q into ``q``, k and the
     re-rounded v0 into the cache's pages (``paged.PagedCache``, ``PagedBatch``).
     pq / pk / pv: 16-byte parameter entries (any dtype)."""
-    c, st = _paged(cache, batch)
-    dev, KV, HD, R = cache.device, cache.KV, cache.HD, batch.rows
+    c, st, dev = _paged(cache, batch)
+    HD, R = cache.HD, batch.rows
+    nh, nkv = H * HD, cache.KV * HD
     rot = HD if rot is None else int(rot)
-    ldq0, ldq = _ld(q0, H * HD, ldq0), _ld(q, H * HD, ldq)
-    ldk, ldv = _ld(k0, KV * HD, ldk), _ld(v0, KV * HD, ldv)
-
-    def entries(t, n, name):
-        if t is None:
-            return None
-        if t.device != dev or not t.is_contiguous() or t.numel() * t.element_size() < 16 * n:
-            raise CormError(_lib.CORM_EINVAL, f"{name}: {n} 16-byte entries on {dev} expected")
-        return t.data_ptr()
-    if rope.dtype != torch.int32 or rope.device != dev or not rope.is_contiguous() or rot < 1 or rope.numel() < rot:
-        raise CormError(_lib.CORM_EINVAL, f"rope: a contiguous int32 [positions][{rot}] table on {dev} expected")
+    if rope.dtype is not torch.int32 or rope.get_device() != dev or not rope.is_contiguous() or rot < 1 or \
+            rope.numel() < rot:
+        raise CormError(_lib.CORM_EINVAL, f"rope: a contiguous int32 [positions][{rot}] table on device {dev} expected")
+    pq0, ldq0 = _rows(q0, "q0", R, nh, ldq0, dev)
+    pk0, ldk = _rows(k0, "k0", R, nkv, ldk, dev)
+    pv0, ldv = _rows(v0, "v0", R, nkv, ldv, dev)
+    pqo, ldq = _rows(q, "q", R, nh, ldq, dev)
     d = _lib.PagedPrepDesc(
-        c, _rows(q0, torch.int16, "q0", R, H * HD, ldq0, dev), _rows(k0, torch.int16, "k0", R, KV * HD, ldk, dev),
-        _rows(v0, torch.int16, "v0", R, KV * HD, ldv, dev), _rows(q, torch.int16, "q", R, H * HD, ldq, dev),
-        rope.data_ptr(), entries(pq, 1 if pq_bc else H * HD, "pq"), entries(pk, 1 if pk_bc else KV * HD, "pk"),
-        None if v_direct else entries(pv, 1 if pv_bc else KV * HD, "pv"), entries(nq, HD, "nq"), entries(nk, HD, "nk"),
-        eps_q, eps_k, ldq0, ldk, ldv, ldq, H, rot, int(bool(interleaved)), rope.numel() // rot,
-        (1 if pq_bc else 0) | (2 if pk_bc else 0) | (4 if pv_bc else 0) | (8 if v_direct else 0))
+        c, pq0, pk0, pv0, pqo, rope.data_ptr(), _entries(pq, 1 if pq_bc else nh, "pq", dev),
+        _entries(pk, 1 if pk_bc else nkv, "pk", dev),
+        None if v_direct else _entries(pv, 1 if pv_bc else nkv, "pv", dev), _entries(nq, HD, "nq", dev),
+        _entries(nk, HD, "nk", dev), eps_q, eps_k, ldq0, ldk, ldv, ldq, H, rot, int(bool(interleaved)),
+        rope.numel() // rot, (1 if pq_bc else 0) | (2 if pk_bc else 0) | (4 if pv_bc else 0) | (8 if v_direct else 0))
     check(lib().corm_llm_paged_prep(C.byref(d), st))
 
 
@@ -393,25 +395,24 @@ def llm_paged_attn(cache, batch, q, o, *, H, smx, window=0, ldq=None, ldo=None):
     """corm_llm_paged_attn: the causal (windowed) grouped-head attention of the
     packed q rows over the cache's pages into o; ``smx`` int32 [H][2]: each head's
     softmax registers (Cm, Cs | f_p << 8)."""
-    c, st = _paged(cache, batch)
-    n, dev = H * cache.HD, cache.device
-    ldq, ldo = _ld(q, n, ldq), _ld(o, n, ldo)
-    if smx.dtype != torch.int32 or smx.device != dev or not smx.is_contiguous() or smx.numel() < 2 * H:
-        raise CormError(_lib.CORM_EINVAL, f"smx: a contiguous int32 [{H}][2] tensor on {dev} expected")
-    d = _lib.PagedAttnDesc(c, _rows(q, torch.int16, "q", batch.rows, n, ldq, dev),
-                           _rows(o, torch.int16, "o", batch.rows, n, ldo, dev), smx.data_ptr(), ldq, ldo, H,
-                           batch.max_q, batch.max_keys, window)
+    c, st, dev = _paged(cache, batch)
+    n, R = H * cache.HD, batch.rows
+    if smx.dtype is not torch.int32 or smx.get_device() != dev or not smx.is_contiguous() or smx.numel() < 2 * H:
+        raise CormError(_lib.CORM_EINVAL, f"smx: a contiguous int32 [{H}][2] tensor on device {dev} expected")
+    pq, ldq = _rows(q, "q", R, n, ldq, dev)
+    po, ldo = _rows(o, "o", R, n, ldo, dev)
+    d = _lib.PagedAttnDesc(c, pq, po, smx.data_ptr(), ldq, ldo, H, batch.max_q, batch.max_keys, window)
     check(lib().corm_llm_paged_attn(C.byref(d), st))
 
 
 def llm_paged_read(cache, batch, k, v, *, ldk=None, ldv=None):
     """corm_llm_paged_read: the cached words of the packed rows' positions into
     int16 rows k and v (either may be None)."""
-    c, st = _paged(cache, batch)
-    n, dev = cache.KV * cache.HD, cache.device
-    ldk, ldv = _ld(k, n, ldk), _ld(v, n, ldv)
-    d = _lib.PagedReadDesc(c, None if k is None else _rows(k, torch.int16, "k", batch.rows, n, ldk, dev),
-                           None if v is None else _rows(v, torch.int16, "v", batch.rows, n, ldv, dev), ldk, ldv)
+    c, st, dev = _paged(cache, batch)
+    n, R = cache.KV * cache.HD, batch.rows
+    pk, ldk = (None, n) if k is None else _rows(k, "k", R, n, ldk, dev)
+    pv, ldv = (None, n) if v is None else _rows(v, "v", R, n, ldv, dev)
+    d = _lib.PagedReadDesc(c, pk, pv, ldk, ldv)
     check(lib().corm_llm_paged_read(C.byref(d), st))
 
 

@@ -50,7 +50,7 @@ class PagedCache:
                 _bad(f"PagedCache: {numel} contiguous {dt} on one device expected, got {tuple(t.shape)} {t.dtype}")
         self.kc, self.vc = buffers[:2]
         self.ks, self.vs = buffers[2:] if bits == 8 else (None, None)
-        self.device = self.kc.device
+        self.device, self.index = self.kc.device, self.kc.get_device()
 
     def desc(self, batch: "PagedBatch") -> _lib.PagedCacheDesc:
         """The cache and the batch as the library takes them (made once for a
