@@ -88,32 +88,32 @@ __device__ __forceinline__ int32_t rot_plain(int32_t x, int32_t cs, int32_t y, i
 // A row of the batch: its sequence (rows ascend: b goes forward), position and page
 struct RowAt {
   bool in;        // a row of a sequence
-  uint64_t p;     // its position
+  bool held;      // its position has a page
+  uint32_t p;     // its position (< 2^32: positions and rows are below 2^31)
   uint64_t line;  // the page's first cached row of head 0, plus the row's place in a page
-  bool held;      // the position has a page
 };
-__device__ __forceinline__ uint32_t first_sequence(const corm_paged_cache& c, uint64_t row) {
+__device__ __forceinline__ uint32_t first_sequence(const corm_paged_cache& c, uint32_t row) {
   uint32_t b = 0, hi = c.B;  // the last b with cu[b] <= row lies in [b, hi)
   while (hi - b > 1u) {
     const uint32_t mid = (b + hi) / 2u;
-    if ((int64_t)c.cu[mid] <= (int64_t)row) b = mid;
+    if (c.cu[mid] <= (int32_t)row) b = mid;
     else hi = mid;
   }
   return b;
 }
-__device__ __forceinline__ RowAt row_at(const corm_paged_cache& c, uint64_t row, uint32_t& b) {
-  while (b + 1u < c.B && (int64_t)c.cu[b + 1] <= (int64_t)row) b++;
+__device__ __forceinline__ RowAt row_at(const corm_paged_cache& c, uint32_t row, uint32_t& b) {
+  while (b + 1u < c.B && c.cu[b + 1] <= (int32_t)row) b++;
   const SeqRows s = seq_rows(c, b, c.rows);
   RowAt o;
   o.in = row >= s.lo && row < s.lo + s.n;
-  o.p = (uint64_t)s.pos + (row - s.lo);
+  o.p = s.pos + (row - s.lo);
   o.held = false;
   o.line = 0;
   if (o.in && o.p < s.cap) {
     const uint32_t sh = 31u - __clz(c.page);
-    const int32_t pg = c.table[(uint64_t)b * c.table_width + (uint32_t)(o.p >> sh)];
+    const int32_t pg = c.table[(uint64_t)b * c.table_width + (o.p >> sh)];
     o.held = (uint32_t)pg < c.pages;
-    if (o.held) o.line = (uint64_t)(uint32_t)pg * c.KV * c.page + ((uint32_t)o.p & (c.page - 1u));
+    if (o.held) o.line = (uint64_t)((uint32_t)pg * (uint64_t)(c.KV << sh)) + (o.p & (c.page - 1u));
   }
   return o;
 }
@@ -128,9 +128,8 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
   const corm_paged_cache& c = d.c;
   const uint32_t KV = c.KV, lane = threadIdx.x % LPH, sub = (threadIdx.x & 31u) / LPH, hr = d.rot / 2u;
   const uint32_t gw = blockIdx.x * 8u + (threadIdx.x >> 5), row_step = gridDim.x * 8u / A.parts, part = gw % A.parts;
-  uint64_t row = gw / A.parts;
-  const int32_t total = c.cu[c.B];
-  const uint64_t rows = min((uint64_t)c.rows, (uint64_t)max(total, 0));
+  uint32_t row = gw / A.parts;
+  const uint32_t rows = min(c.rows, (uint32_t)max(c.cu[c.B], 0));
   if (NORM) {
     for (uint32_t i = threadIdx.x; i < 2u * HD; i += 256u) {
       const uint8_t* ne = (const uint8_t*)(i < HD ? d.nq : d.nk);
@@ -182,20 +181,26 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
       const uint32_t k0 = shifts(s, dim_a(0, s.is_v));
       kd = k0 >> 16;
       bool plain = (k0 & 0xFFFFu) == 0u && kd <= 31u && (kd >= 9u || s.is_v || 4u * lane >= hr);
+      if (!(s.is_v && (d.flags & 8u)) && !(d.flags & (s.is_q ? 1u : (s.is_v ? 4u : 2u)))) {  // an entry a dimension
+        const uint8_t* const e = (const uint8_t*)(s.is_q ? d.pq : (s.is_v ? d.pv : d.pk)) + 16ull * (s.head * HD) + 8u;
 #pragma unroll
-      for (uint32_t k = 0; k < 4; k++) plain = plain && shifts(s, dim_a(k, s.is_v)) == k0 && shifts(s, dim_b(k, s.is_v)) == k0;
+        for (uint32_t k = 0; k < 4; k++)
+          plain = plain && ((*(const uint32_t*)(e + 16u * dim_a(k, s.is_v)) ^ k0) & 0x3F3F3Fu) == 0u &&
+                  ((*(const uint32_t*)(e + 16u * dim_b(k, s.is_v)) ^ k0) & 0x3F3F3Fu) == 0u;
+      }
       if (!plain) kd = 255;
     }
     forms |= (uint64_t)kd << (8u * (it - it0));
   }
   const bool spl = 4u * lane < hr && !d.interleaved;  // VEC: alike for the lane's four pairs
+  const bool all_spl = VEC && d.rot == HD && !d.interleaved;
   // the next row's heads, q's and k's counted as one (k's head i - H), this lane's place
   // in them; the second four of its elements are `far` on (VEC)
   const uint32_t place = VEC ? (spl ? 4u : 8u) * lane : 0u, far = spl ? hr : 4u, place_v = VEC ? 8u * lane : 0u;
-  const int16_t* nq = d.q0 + row * d.ldq0 + place;
-  const int16_t* nk = d.k0 + row * d.ldk + place - (uint64_t)d.H * HD;
-  const int16_t* nv = d.v0 + row * d.ldv + place_v;
-  int16_t* yq = d.q + row * d.ldq + place;
+  const int16_t* nq = d.q0 + (uint64_t)row * d.ldq0 + place;
+  const int16_t* nk = d.k0 + (uint64_t)row * d.ldk + place - (uint64_t)d.H * HD;
+  const int16_t* nv = d.v0 + (uint64_t)row * d.ldv + place_v;
+  int16_t* yq = d.q + (uint64_t)row * d.ldq + place;
   // the 8 elements of a turn: two words of 4, the pairs' firsts and seconds where `spl`
   // (or not VEC), else as they lie
   auto load = [&](uint32_t it) {
@@ -223,7 +228,7 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
     int8_t* const vr = c.vc + at.line * rb;
     int32_t cs[4], sn[4];
     {
-      const int32_t* tr = d.rope + (uint64_t)min(at.in ? at.p : (uint64_t)0, (uint64_t)(d.rope_rows - 1u)) * d.rot;
+      const int32_t* tr = d.rope + (uint64_t)min(at.in ? at.p : 0u, d.rope_rows - 1u) * d.rot;
       if (VEC && 4u * lane < hr) {
         const int4 c4 = __ldg((const int4*)(tr + 4u * lane)), s4 = __ldg((const int4*)(tr + hr + 4u * lane));
         cs[0] = c4.x, cs[1] = c4.y, cs[2] = c4.z, cs[3] = c4.w;
@@ -252,16 +257,14 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
       if (!at.in) continue;  // a row of no sequence
       const Slot s = slot_of(it);
       const bool sp = VEC ? spl && !s.is_v : true;
-      int32_t va[4], vb[4];
-      {
-        const int32_t v8[8] = {(int16_t)x.x, (int32_t)x.x >> 16, (int16_t)x.y, (int32_t)x.y >> 16,
-                               (int16_t)x.z, (int32_t)x.z >> 16, (int16_t)x.w, (int32_t)x.w >> 16};
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          va[k] = sp ? v8[k] : v8[2 * k];
-          vb[k] = sp ? v8[4 + k] : v8[2 * k + 1];
-        }
+      uint4 ab = x;  // the pairs' firsts, then their seconds
+      if (VEC && !(all_spl && !s.is_v)) {
+        if (!sp)
+          ab = make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.x, x.y, 0x7632),
+                          __byte_perm(x.z, x.w, 0x7632));
       }
+      int32_t va[4] = {(int16_t)ab.x, (int32_t)ab.x >> 16, (int16_t)ab.y, (int32_t)ab.y >> 16};
+      int32_t vb[4] = {(int16_t)ab.z, (int32_t)ab.z >> 16, (int16_t)ab.w, (int32_t)ab.w >> 16};
       if (NORM && !s.is_v) {  // (alike over the warp; a head's lanes all have it or not)
         uint64_t s2 = 0;
 #pragma unroll
@@ -407,9 +410,8 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__
   const uint32_t lane = threadIdx.x % LPH, sub = (threadIdx.x & 31u) / LPH, nk = d.k ? c.KV : 0u;
   const uint32_t gw = blockIdx.x * 8u + (threadIdx.x >> 5), row_step = gridDim.x * 8u / A.parts;
   const uint32_t part = gw % A.parts, it0 = part * A.per, it1 = min(it0 + A.per, A.turns);
-  uint64_t row = gw / A.parts;
-  const int32_t last = c.cu[c.B];
-  const uint64_t rows = min((uint64_t)c.rows, (uint64_t)max(last, 0));
+  uint32_t row = gw / A.parts;
+  const uint32_t rows = min(c.rows, (uint32_t)max(c.cu[c.B], 0));
   if (row >= rows || row >= row_step) return;
   const bool b8 = c.bits == 8u;
   const uint32_t rb = b8 ? HD : 2 * HD, hb = c.page * rb;  // bytes from head to head
@@ -420,8 +422,8 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__
     if (!at.in) continue;
     const int8_t* const kr = c.kc + at.line * rb + 8u * lane;
     const int8_t* const vr = c.vc + at.line * rb + 8u * lane;
-    int16_t* const ko = d.k + row * d.ldk + 8u * lane;
-    int16_t* const vo = d.v + row * d.ldv + 8u * lane;
+    int16_t* const ko = d.k + (uint64_t)row * d.ldk + 8u * lane;
+    int16_t* const vo = d.v + (uint64_t)row * d.ldv + 8u * lane;
 #pragma unroll 1
     for (uint32_t t = it0; t < it1; t += U) {
       uint2 h[U], l[U];
