@@ -1104,7 +1104,7 @@ uint32_t resident_clusters(uint32_t X, uint32_t d) {
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes) != cudaSuccess ||
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)split_smem(1)) != cudaSuccess ||
       cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
     cudaGetLastError();
     n = 0;
@@ -1152,7 +1152,8 @@ int launch_split(SplitArgs A, uint32_t tiles, cudaStream_t st) {
   A.stages = stages;
   const size_t smem = kWarps * stages * Sh::STB + (size_t)A.win * block + fixed;
   auto kern = paged_attn_split_kernel<HD, BITS>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  // (one limit for every launch: another thread's may be between its limit and its launch)
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)split_smem(1)) != cudaSuccess)
     return corm::cuda_status("llm_paged_attn");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles * X, c.KV, c.B);

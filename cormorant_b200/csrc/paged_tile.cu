@@ -3,7 +3,7 @@
 //
 // Persistent: a CTA an SM takes items = (128-row tile, sequence, KV head), the ones that
 // see most keys first, a row being (token, head of the group), token-major; with few items a
-// cluster of CTAs shares an item's keys.  As in the 16-row kernel, the unit's e(d) is a
+// cluster of CTAs shares an item's keys.  As in the 8-row kernel, the unit's e(d) is a
 // table of d = m - score, so nothing can be rescaled as a running maximum moves: three
 // phases over the scores, which stay in shared memory (int16, then e in place) where the
 // CTA's keys fit, and are formed again in windows where they do not.
@@ -1083,7 +1083,8 @@ int launch(TileArgs A, uint32_t tiles, cudaStream_t st) {
   A.win = need < 2u ? 2u : (need < most ? need : most);  // (a cluster's sums take up to two tiles' memory)
   const size_t smem = 1024u + A.stages * Sh::STAGE + (size_t)A.win * tile_bytes;
   auto kern = paged_attn_tile_kernel<HD, BITS>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  // (one limit for every launch: another thread's may be between its limit and its launch)
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem) != cudaSuccess)
     return corm::cuda_status("llm_paged_attn");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks * X);

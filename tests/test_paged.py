@@ -694,6 +694,108 @@ def test_prep_writes_what_attn_reads_chunk_by_chunk():
         assert bits == 8 or torch.equal(kvs[0][:, KV * HD:], x[2])
 
 
+CHUNKS = [  # HD, bits, page, H, KV, contexts, new rows, window
+    (64, 16, 64, 4, 1, [900, 20, 0, 1500, 300], [40, 70, 0, 33, 64], 0),
+    (64, 8, 32, 6, 2, [1100, 1100, 5], [70, 1, 65], 0),
+    (128, 16, 16, 4, 1, [1700], [129], 0),
+    (128, 8, 128, 8, 2, [600, 0, 1300, 64], [50, 50, 50, 50], 0),
+    (64, 16, 256, 3, 1, [2500, 130], [90, 90], 700)]
+
+
+@gpu
+@pytest.mark.parametrize("case", CHUNKS, ids=lambda c: "hd%d_b%d_p%d_h%d_%d_w%d" % (c[:5] + (c[7],)))
+def test_attn_chunks_over_contexts(case):
+    """Chunks of rows behind longer and shorter contexts: the sequences taken by
+    their lengths, an item's keys shared by a cluster, empty sequences between."""
+    HD, bits, page, H, KV, ctx, new, w = case
+    rng = np.random.default_rng(sum(ctx) + HD + bits)
+    pages = sum(-(-(c + n) // page) for c, n in zip(ctx, new)) + 2
+    table, cu, pos, rows = _batch(rng, pages, page, ctx, new, extra=1)
+    c = _random_cache(rng, pages, KV, page, HD, bits, 2500)
+    c.table, c.cu, c.pos = table, cu, pos
+    _run_attn(c, rows, H, _smx(H, HD, f_s=10), rng, window=w, hi=2500, max_q=max(new),
+              max_keys=max(a + b for a, b in zip(ctx, new)))
+
+
+@gpu
+@pytest.mark.parametrize("new,ctx", [([130, 7, 200], [0, 600, 40]), ([1, 2, 1], [2500, 30, 1300])], ids=["prompts", "decode"])
+def test_attn_captured_with_other_lengths(new, ctx):
+    """A captured call replayed with the rows, positions and pages of other
+    batches within its max_q and rows (the hint of the keys passed, too)."""
+    from cormorant_b200 import ops
+    HD, KV, H, page, width = 64, 2, 6, 32, 90
+    rng = np.random.default_rng(sum(new))
+    smx, rows = _smx(H, HD, f_s=10), sum(new)
+
+    def batch_of(ctx, new):
+        table, cu, pos, _ = _batch(rng, 200, page, ctx, new)
+        full = np.full((3, width), -1, np.int32)
+        full[:, :table.shape[1]] = table
+        return full, cu, pos
+    c = _random_cache(rng, 200, KV, page, HD, 16, 2500)
+    c.table, c.cu, c.pos = batch_of(ctx, new)
+    cache, batch = _handles(c, rows, max_q=max(new), max_keys=max(a + b for a, b in zip(ctx, new)))
+    qh = rng.integers(-2500, 2500, size=(rows, H * HD)).astype(np.int16)
+    q, o, sd = _dev(qh), torch.zeros((rows, H * HD), dtype=torch.int16, device="cuda"), _dev(smx)
+    ops.llm_paged_attn(cache, batch, q, o, H=H, smx=sd)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.llm_paged_attn(cache, batch, q, o, H=H, smx=sd)
+    for perm in ([0, 1, 2], [2, 0, 1], [1, 2, 0]):
+        n2 = [new[perm[0]], 0 if perm[0] == 2 else new[perm[1]], new[perm[2]]]
+        c.table, c.cu, c.pos = batch_of([ctx[i] // 2 + 9 * i for i in perm], n2)
+        for t, x in zip((batch.table, batch.cu, batch.pos), (c.table, c.cu, c.pos)):
+            t.copy_(_dev(x))
+        o.fill_(5)
+        graph.replay()
+        want = np.full((rows, H * HD), 5, np.int64)
+        OP.attn(c, qh, want, H=H, smx=smx, max_q=max(new))
+        assert np.array_equal(o.cpu().numpy(), want)
+    assert ops.device_status() == 0
+
+
+@gpu
+def test_calls_from_two_threads():
+    """Two host threads, each with its own cache, sizes and stream, at once: every
+    result is the one of the call alone."""
+    import threading
+    from cormorant_b200 import ops
+    rng = np.random.default_rng(91)
+    jobs = []
+    for HD, KV, ctx, new in ((64, 2, [3000, 40], [1, 2]), (64, 2, [5], [90]), (64, 2, [700, 0, 90], [1, 300, 40]),
+                             (128, 1, [1500], [1])):
+        page = 32
+        pages = sum(-(-(a + n) // page) for a, n in zip(ctx, new)) + 1
+        table, cu, pos, rows = _batch(rng, pages, page, ctx, new)
+        c = _random_cache(rng, pages, KV, page, HD, 16, 2500)
+        c.table, c.cu, c.pos = table, cu, pos
+        cache, batch = _handles(c, rows, max_q=max(new), max_keys=max(a + b for a, b in zip(ctx, new)))
+        q, smx = _dev(rng.integers(-2500, 2500, size=(rows, 2 * KV * HD)).astype(np.int16)), _dev(_smx(2 * KV, HD, f_s=10))
+        want = torch.zeros((rows, 2 * KV * HD), dtype=torch.int16, device="cuda")
+        ops.llm_paged_attn(cache, batch, q, want, H=2 * KV, smx=smx)
+        jobs.append((cache, batch, q, smx, 2 * KV, want))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(mine):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in range(60):
+                cache, batch, q, smx, H, want = mine[i % len(mine)]
+                o = torch.zeros_like(want)
+                ops.llm_paged_attn(cache, batch, q, o, H=H, smx=smx)
+                if i % 7 == 0 and not torch.equal(o, want):
+                    bad.append(i)
+            torch.cuda.current_stream().synchronize()
+            if not torch.equal(o, want):
+                bad.append(-1)
+    threads = [threading.Thread(target=work, args=(m,)) for m in (jobs[:2], jobs[2:])]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad and ops.device_status() == 0
+
+
 @gpu
 def test_gpu_refusals():
     """Arguments of the wrong type, size, stride or device raise; nothing runs."""
