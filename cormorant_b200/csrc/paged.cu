@@ -45,6 +45,12 @@ using namespace paged;
 // up once for all its heads, and a lane's entries once for all its rows.  Norm: the
 // squares' sum by shuffles over the head, the divisor by the unit's table and Newton
 // step, 64-bit throughout (D < 2^63, |x Rm| < 2^48, |P1 G| < 2^56).
+//
+// Bound by its instructions: a rotated element is two wide products and a rounding of
+// a 64-bit sum, a third of some 290 instructions a turn (20 k rows x 25 heads of 64: 67
+// us, 60% of the issue slots, 2.4 TB/s; a thread per 8 elements of one head, a row looked
+// up by each: 113 us).  Three blocks an SM, so 80 registers; the next turn's elements are
+// loaded before this one's are worked on, as 24 warps hold too few loads otherwise.
 constexpr uint32_t kTurns = 8;  // turns of a part: their entries' forms are a byte each of one word
 struct PrepArgs {
   corm_llm_paged_prep_desc d;
@@ -395,7 +401,9 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
 // ---------------------------------------------------------------- read-back
 // A warp per row, or per part of its heads (K's, then V's) where there are few rows;
 // HD / 8 lanes a head, 8 elements a lane: 8-byte loads of each plane, four heads' under
-// way at once, one 16-byte store (words where the output is not on 16 bytes).
+// way at once, one 16-byte store (words where the output is not on 16 bytes).  Bound by
+// the loads' latency and the copies' instructions: 3 sequences of 20 k cached rows at 8
+// bits 13.6 us (3.8 TB/s), 16 of up to 640 5.3 us.
 struct ReadArgs {
   corm_llm_paged_read_desc d;
   uint32_t vec, heads, turns, per, parts;  // heads: K's and V's, or one of them
@@ -517,6 +525,15 @@ RowGrid row_grid(uint64_t rows, uint32_t turns, uint32_t most, uint32_t blocks_s
 // tcgen05 tile, and the copies are to bound the kernel.  The contraction over the
 // keys takes them in the order in which the scores' words hold them (word i of 16
 // keys: keys i and i + 8); V's rows are transposed on the way to the registers.
+//
+// Measured (64 dimensions, 3 query heads a KV head, in a graph): 64 sequences of 128 to
+// 639 keys 12.4 us, bound by its chain of waits (page, K, maximum, sum, V; 6.4 us with one
+// sequence of 33 keys, 4 of them the kernel's); 8 sequences of 21k to 32k keys at 8 bits
+// 43 us, 3.0 TB/s: the K and V phases run at three quarters of the memory's rate, the
+// softmax between them (about 250 of 1000 instructions a block) keeps only the stages'
+// copies under way; 128 dimensions, 4 query heads, 16 bits, 16 x 4k keys: 41 us, 4.9 TB/s.
+// A ring of 64-key stages that all warps share, a copy warp and 16-row MMAs: 29 and 146
+// us for the first two.
 constexpr uint32_t kRows = 8;     // rows of a tile
 constexpr uint32_t kWarps = 8;
 constexpr uint32_t kMaxCluster = 8;

@@ -23,6 +23,16 @@
 // 16 bits: 2 x 2 planes, sums HH 2^16 + MID 2^8 + LL.  8 bits: the codes are one
 // plane; a K row's shift applies to the score, a V row's to P (three planes).
 // Every sum is modulo 2^32, the rule's own wrap.
+//
+// Bound by the row warps' integer work, phase by phase (cycles of a 128 x 128 tile of 64
+// dimensions at 16 bits): scores 1800 (the MMAs, 65 cycles each and twice that between
+// issues beside 16 busy warps, do not overlap the loads of their one set of sums: three
+// sums of 128 columns and P fill TMEM), e 2500 (16384 table lookups at random banks: 1700
+// at the least), P 2000, and about 7500 an item around them.  In windows the scores are
+// formed three times and e twice: 11600 a tile.  64 prompts of 97 to 512 rows, 15 heads
+// of 64: 189 us; one of 8192: 1257 us; 4 chunks of 257 over 1k to 8k, 16 heads of 128:
+// 364 us.  Tried and slower: tiles of 64 keys, two CTAs an SM (332 us for the prompts);
+// more score columns a load (spills); one CTA an item, not persistent (266 us).
 #include <cudaTypedefs.h>
 
 #include <atomic>
