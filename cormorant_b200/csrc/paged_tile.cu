@@ -32,7 +32,8 @@
 // formed three times and e twice: 11600 a tile.  64 prompts of 97 to 512 rows, 15 heads
 // of 64: 189 us; one of 8192: 1257 us; 4 chunks of 257 over 1k to 8k, 16 heads of 128:
 // 364 us.  Tried and slower: tiles of 64 keys, two CTAs an SM (332 us for the prompts);
-// more score columns a load (spills); one CTA an item, not persistent (266 us).
+// more score columns a load (spills); one CTA an item, not persistent (266 us); the low
+// planes made signed, so that one MMA takes both (204 us: two instructions a score more).
 #include <cudaTypedefs.h>
 
 #include <atomic>
