@@ -37,8 +37,8 @@ __device__ __forceinline__ SeqRows seq_rows(const corm_paged_cache& c, uint32_t 
 
 // ---------------------------------------------------------------- the softmax unit's integers
 // e of a score d below the row's maximum: y = (d Cm) >> Cs, TAB[y mod 4096] >>
-// (y / 4096).  The table is held less one in 16 bits (TAB is 32774 .. 65536).
-// any Cs (y may pass 32 bits below 8)
+// (y / 4096); the form for any Cs (below 8 y may pass 32 bits), the table held less
+// one in 16 bits (TAB is 32774 .. 65536)
 __device__ __forceinline__ uint32_t smx_e_wide(uint32_t d, uint32_t cm, uint32_t cs, const uint16_t* tab) {
   const uint64_t y = ((uint64_t)d * (cm & 0xFFFFFFu)) >> cs;
   return (y >> 12) > 16u ? 0u : ((uint32_t)tab[y & 4095u] + 1u) >> (uint32_t)(y >> 12);
@@ -93,7 +93,7 @@ __device__ __forceinline__ uint32_t pack16(int32_t lo, int32_t hi) {  // both al
 }
 
 // C[16 x 8] += A[16 x 32] B[32 x 8] on 8-bit operands, int32 sums modulo 2^32
-// (warp-level; used where a tile has 16 rows at most)
+// (warp-level; for tiles of 8 query rows)
 #define CORM_MMA_I8(NAME, TA, TB)                                                                                      \
   __device__ __forceinline__ void NAME(uint32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {           \
     asm("mma.sync.aligned.m16n8k32.row.col.s32." TA "." TB                                                    \
@@ -168,11 +168,6 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, uint32_t 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

@@ -330,6 +330,15 @@ def test_prep_vs_oracle(case):
 
 
 @gpu
+@pytest.mark.parametrize("case", [(128, 128, False, True, 16, 32, 40, 20, False), (256, 64, True, False, 8, 64, 33, 11, False),
+                                  (16, 16, False, False, 16, 16, 90, 45, True)], ids=["hd128", "hd256", "hd16"])
+def test_prep_and_read_of_many_heads(case):
+    """More heads than a warp takes of a row, and a read-back of as many."""
+    test_prep_vs_oracle(case)
+    test_read_vs_oracle(case[0], case[4], case[5], case[7])
+
+
+@gpu
 @pytest.mark.parametrize("case", [PREPS[1], PREPS[6], PREPS[8]], ids=["hd64", "hd128", "rot44"])
 def test_prep_views_and_wide_shifts(case):
     """Operands that are views of one wide row at an odd offset; entries whose shifts need 128-bit sums."""
