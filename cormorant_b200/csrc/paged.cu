@@ -58,17 +58,17 @@ struct PrepArgs {
   uint32_t turned, turns, per, parts;  // turns of the rotated heads, of all; a part's; parts of a row
 };
 
-// the row-ops unit's 1 / sqrt(D) ~ Rm 2^-sh for 1 <= D < 2^63
-__device__ __forceinline__ void rsqrt64(uint64_t D, uint64_t& Rm, int& sh, const uint32_t* __restrict__ rsq) {
+// the row-ops unit's 1 / sqrt(D) ~ Rm 2^-sh for 1 <= D < 2^63: Dm = D 2^-d (d even) below
+// 2^32 with one of its two top bits, a table's y0 and a Newton step, all in 32 bits but the last
+__device__ __forceinline__ void rsqrt64(uint64_t D, uint32_t& Rm, int& sh, const uint32_t* __restrict__ rsq) {
   int d = 32 - __clzll((long long)D);
   if (d & 1) d += 1;
-  const uint64_t Dm = d >= 0 ? D >> d : D << -d;  // < 2^32
-  const uint64_t y0 = __ldg(rsq + (Dm >> 19));
-  const uint64_t u = (((Dm * y0) >> 32) * y0) >> 32;
+  const uint32_t Dm = (uint32_t)((D << (32 - d)) >> 32);  // (32 - d <= the leading zeros)
+  const uint32_t y0 = __ldg(rsq + (Dm >> 19));
+  const uint32_t u = __umulhi(__umulhi(Dm, y0), y0);
   // |y0 (2^30 - u)| < 2^62: the table's y0 is within 2^-13 of 1 / sqrt
-  int64_t y1 = (int64_t)y0 + (((int64_t)y0 * ((1ll << 30) - (int64_t)u)) >> 31);
-  y1 = max(y1, (int64_t)1 << 31);
-  Rm = (uint64_t)min(y1, ((int64_t)1 << 32) - 1);
+  const int64_t y1 = (int64_t)y0 + (((int64_t)y0 * (int32_t)((1u << 30) - u)) >> 31);
+  Rm = (uint32_t)min(max(y1, (int64_t)1 << 31), ((int64_t)1 << 32) - 1);
   sh = 47 + d / 2;
 }
 
@@ -127,7 +127,8 @@ __device__ __forceinline__ RowAt row_at(const corm_paged_cache& c, uint32_t row,
 template <int HD, bool VEC, bool NORM>
 __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constant__ PrepArgs A) {
   constexpr uint32_t LPH = HD / 8, HPT = 32 / LPH;  // lanes a head, heads a turn
-  __shared__ int2 s_norm[NORM ? 2 : 1][NORM ? HD : 1];  // the norms' factors and down-shifts, q's and k's
+  // the norms' entries, q's and k's: factor, down-shift n, 2^(n - 1) - 1 (0 for n = 0)
+  __shared__ int4 s_norm[NORM ? 2 : 1][NORM ? HD : 1];
   corm_pdl_wait();
   corm_pdl_trigger();
   const corm_llm_paged_prep_desc& d = A.d;
@@ -136,12 +137,17 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
   const uint32_t gw = blockIdx.x * 8u + (threadIdx.x >> 5), row_step = gridDim.x * 8u / A.parts, part = gw % A.parts;
   uint32_t row = gw / A.parts;
   const uint32_t rows = min(c.rows, (uint32_t)max(c.cu[c.B], 0));
+  bool high = true;  // every down-shift is 32 .. 62: the usual entries
   if (NORM) {
     for (uint32_t i = threadIdx.x; i < 2u * HD; i += 256u) {
       const uint8_t* ne = (const uint8_t*)(i < HD ? d.nq : d.nk);
-      if (ne) s_norm[i / HD][i % HD] = make_int2(*(const int32_t*)(ne + 16u * (i % HD)), ne[16u * (i % HD) + 10u] & 63);
+      if (!ne) continue;
+      const uint32_t n = ne[16u * (i % HD) + 10u] & 63u;
+      const uint64_t h = n ? (1ull << (n - 1u)) - 1ull : 0ull;
+      s_norm[i / HD][i % HD] = make_int4(*(const int32_t*)(ne + 16u * (i % HD)), (int)n, (int)(uint32_t)h, (int)(uint32_t)(h >> 32));
+      high = high && n >= 32u && n <= 62u;
     }
-    __syncthreads();
+    high = __syncthreads_and(high);
   }
   if (row >= rows || row >= row_step) return;
   const uint32_t it0 = part * A.per, it1 = min(it0 + A.per, A.turns);
@@ -274,18 +280,29 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
       if (NORM && !s.is_v) {  // (alike over the warp; a head's lanes all have it or not)
         uint64_t s2 = 0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) s2 += (uint64_t)(uint32_t)(va[k] * va[k]) + (uint32_t)(vb[k] * vb[k]);
+        for (int k = 0; k < 4; k++) s2 = (uint64_t)((int64_t)vb[k] * vb[k] + (int64_t)((uint64_t)((int64_t)va[k] * va[k]) + s2));
 #pragma unroll
         for (uint32_t o = LPH / 2; o > 0; o >>= 1) s2 += __shfl_xor_sync(0xffffffffu, s2, o);
         if (s.is_q ? d.nq : d.nk) {
-          uint64_t Rm;
+          uint32_t Rm;
           int sh;
           rsqrt64(max(s2 + (s.is_q ? d.eps_q : d.eps_k), (uint64_t)1), Rm, sh, A.rsq);
           sh -= 24;
-          // |x| <= sqrt(D): x Rm 2^-sh is 2^24 at most, and the table's error
+          // |x| <= sqrt(D): P1 = floor(x Rm 2^-sh) is 2^24 at most, and the table's error;
+          // Rm has its top bit: x Rm is x times it as a signed word, and 2^32 x.  P1 G to
+          // nearest, ties to even, as rot_plain rounds: the quotient is in the high word
           auto normed = [&](int32_t x, uint32_t dim) {
-            const int2 g = s_norm[s.is_q ? 0 : 1][NORM ? dim : 0];
-            return (int32_t)corm_sat16(corm_rne_shr64f((int64_t)(int32_t)(((int64_t)x * (int64_t)Rm) >> sh) * g.x, g.y));
+            const int4 e = s_norm[s.is_q ? 0 : 1][NORM ? dim : 0];
+            const int64_t xr = (int64_t)x * (int32_t)Rm + ((int64_t)x << 32);
+            const int32_t hi = (int32_t)(xr >> 32);
+            const int32_t p1 = sh < 32 ? (int32_t)__funnelshift_r((uint32_t)xr, (uint32_t)hi, (uint32_t)sh) : hi >> (sh - 32);
+            if (high) {
+              const int64_t v = (int64_t)p1 * e.x + (int64_t)((uint64_t)(uint32_t)e.w << 32 | (uint32_t)e.z);
+              const uint32_t n = (uint32_t)e.y - 32u;
+              const int64_t u = v + (((int32_t)(v >> 32) >> n) & 1);
+              return min(max((int32_t)(u >> 32) >> n, -32768), 32767);
+            }
+            return (int32_t)corm_sat16(corm_rne_shr64f((int64_t)p1 * e.x, e.y));
           };
 #pragma unroll
           for (uint32_t k = 0; k < 4; k++) {
@@ -337,15 +354,16 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
       }
       uint32_t shift = 0;
       if (c.bits == 8u) {  // (every lane: the head's largest element)
-        uint32_t t = 0;
+        // x or its complement, two of 16 bits a word (a permutation repeats the signs)
+        auto mag = [](uint32_t w) {
+          uint32_t sign;
+          asm("prmt.b32 %0, %1, 0, 0xBB99;" : "=r"(sign) : "r"(w));
+          return w ^ sign;
+        };
+        uint32_t t = __vmaxu2(__vmaxu2(mag(w0), mag(w1)), __vmaxu2(mag(w2), mag(w3)));
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          va[k] = min(max(va[k], -32768), 32767);
-          vb[k] = min(max(vb[k], -32768), 32767);
-          t = max(t, max((uint32_t)(va[k] ^ (va[k] >> 31)), (uint32_t)(vb[k] ^ (vb[k] >> 31))));
-        }
-#pragma unroll
-        for (uint32_t o = LPH / 2; o > 0; o >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
+        for (uint32_t o = LPH / 2; o > 0; o >>= 1) t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, o));
+        t = max(t & 0xFFFFu, t >> 16);
         const int bits = 32 - __clz((int)t);
         shift = bits > 7 ? (uint32_t)(bits - 7) : 0u;
       }
@@ -354,6 +372,8 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
       if (c.bits == 8u) {
         // RNE by shift <= 8; only the upper end can round past the codes
         const int32_t h = (1 << shift) >> 1, r = h ? h - 1 : 0;
+        va[0] = (int16_t)w0, va[1] = (int32_t)w0 >> 16, va[2] = (int16_t)w1, va[3] = (int32_t)w1 >> 16;
+        vb[0] = (int16_t)w2, vb[1] = (int32_t)w2 >> 16, vb[2] = (int16_t)w3, vb[3] = (int32_t)w3 >> 16;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           va[k] = min((va[k] + r + (h ? (va[k] >> shift) & 1 : 0)) >> shift, 127);
