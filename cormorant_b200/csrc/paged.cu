@@ -127,7 +127,8 @@ __device__ __forceinline__ RowAt row_at(const corm_paged_cache& c, uint32_t row,
 template <int HD, bool VEC, bool NORM>
 __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constant__ PrepArgs A) {
   constexpr uint32_t LPH = HD / 8, HPT = 32 / LPH;  // lanes a head, heads a turn
-  // the norms' entries, q's and k's: factor, down-shift n, 2^(n - 1) - 1 (0 for n = 0)
+  // the norms' entries, q's and k's, a lane's eight LPH apart (no bank is asked twice):
+  // factor, down-shift n, 2^(n - 1) - 1 (0 for n = 0)
   __shared__ int4 s_norm[NORM ? 2 : 1][NORM ? HD : 1];
   corm_pdl_wait();
   corm_pdl_trigger();
@@ -137,14 +138,22 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
   const uint32_t gw = blockIdx.x * 8u + (threadIdx.x >> 5), row_step = gridDim.x * 8u / A.parts, part = gw % A.parts;
   uint32_t row = gw / A.parts;
   const uint32_t rows = min(c.rows, (uint32_t)max(c.cu[c.B], 0));
+  // the dimensions of a lane's pairs: a rotated pair p at (p, p + rot / 2) or
+  // (2 p, 2 p + 1); the rest of the head, and v's, in neighbouring pairs
+  auto first_of = [&](uint32_t p, bool v) { return p < hr && !d.interleaved && !v ? p : 2u * p; };
+  auto second_of = [&](uint32_t p, bool v) { return p < hr && !d.interleaved && !v ? p + hr : 2u * p + 1u; };
+  auto dim_a = [&](uint32_t k, bool v) { return first_of(4u * lane + k, v); };
+  auto dim_b = [&](uint32_t k, bool v) { return second_of(4u * lane + k, v); };
   bool high = true;  // every down-shift is 32 .. 62: the usual entries
   if (NORM) {
     for (uint32_t i = threadIdx.x; i < 2u * HD; i += 256u) {
       const uint8_t* ne = (const uint8_t*)(i < HD ? d.nq : d.nk);
       if (!ne) continue;
-      const uint32_t n = ne[16u * (i % HD) + 10u] & 63u;
+      const uint32_t l = i % LPH, e = i % HD / LPH, p = 4u * l + (e & 3u);
+      ne += 16u * (e < 4u ? first_of(p, false) : second_of(p, false));
+      const uint32_t n = ne[10] & 63u;
       const uint64_t h = n ? (1ull << (n - 1u)) - 1ull : 0ull;
-      s_norm[i / HD][i % HD] = make_int4(*(const int32_t*)(ne + 16u * (i % HD)), (int)n, (int)(uint32_t)h, (int)(uint32_t)(h >> 32));
+      s_norm[i / HD][i % HD] = make_int4(*(const int32_t*)ne, (int)n, (int)(uint32_t)h, (int)(uint32_t)(h >> 32));
       high = high && n >= 32u && n <= 62u;
     }
     high = __syncthreads_and(high);
@@ -165,16 +174,6 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
     s.is_q = !v && i < d.H;
     s.head = v || s.is_q ? i : i - d.H;
     return s;
-  };
-  // the dimensions of this lane's pairs: a rotated pair p at (p, p + rot / 2) or
-  // (2 p, 2 p + 1); the rest of the head, and v's, in neighbouring pairs
-  auto dim_a = [&](uint32_t k, bool v) {
-    const uint32_t p = 4u * lane + k;
-    return p < hr && !d.interleaved && !v ? p : 2u * p;
-  };
-  auto dim_b = [&](uint32_t k, bool v) {
-    const uint32_t p = 4u * lane + k;
-    return p < hr && !d.interleaved && !v ? p + hr : 2u * p + 1u;
   };
   auto shifts = [&](const Slot& s, uint32_t dim) -> uint32_t {  // sh_a | sh_b << 8 | sh_c << 16
     const uint8_t* ent = (const uint8_t*)(s.is_q ? d.pq : (s.is_v ? d.pv : d.pk));
@@ -291,23 +290,23 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
           // |x| <= sqrt(D): P1 = floor(x Rm 2^-sh) is 2^24 at most, and the table's error;
           // Rm has its top bit: x Rm is x times it as a signed word, and 2^32 x.  P1 G to
           // nearest, ties to even, as rot_plain rounds: the quotient is in the high word
-          auto normed = [&](int32_t x, uint32_t dim) {
-            const int4 e = s_norm[s.is_q ? 0 : 1][NORM ? dim : 0];
+          const bool fast = high && __all_sync(__activemask(), sh < 32);
+          auto normed = [&](int32_t x, uint32_t i) {
+            const int4 e = s_norm[s.is_q ? 0 : 1][NORM ? i * LPH + lane : 0];
             const int64_t xr = (int64_t)x * (int32_t)Rm + ((int64_t)x << 32);
-            const int32_t hi = (int32_t)(xr >> 32);
-            const int32_t p1 = sh < 32 ? (int32_t)__funnelshift_r((uint32_t)xr, (uint32_t)hi, (uint32_t)sh) : hi >> (sh - 32);
-            if (high) {
+            if (fast) {
+              const int32_t p1 = (int32_t)__funnelshift_r((uint32_t)xr, (uint32_t)(xr >> 32), (uint32_t)sh);
               const int64_t v = (int64_t)p1 * e.x + (int64_t)((uint64_t)(uint32_t)e.w << 32 | (uint32_t)e.z);
               const uint32_t n = (uint32_t)e.y - 32u;
               const int64_t u = v + (((int32_t)(v >> 32) >> n) & 1);
               return min(max((int32_t)(u >> 32) >> n, -32768), 32767);
             }
-            return (int32_t)corm_sat16(corm_rne_shr64f((int64_t)p1 * e.x, e.y));
+            return (int32_t)corm_sat16(corm_rne_shr64f((xr >> sh) * e.x, e.y));
           };
 #pragma unroll
           for (uint32_t k = 0; k < 4; k++) {
-            va[k] = normed(va[k], dim_a(k, false));
-            vb[k] = normed(vb[k], dim_b(k, false));
+            va[k] = normed(va[k], k);
+            vb[k] = normed(vb[k], 4u + k);
           }
         }
       }
