@@ -1153,7 +1153,7 @@ template <int HD, int BITS>
 int launch_split(SplitArgs A, uint32_t tiles, cudaStream_t st) {
   using Sh = SplitShape<HD, BITS>;
   const corm_paged_cache& c = A.d.c;
-  const uint64_t blocks = (uint64_t)c.B * c.KV * tiles;
+  const uint64_t blocks = paged::live_tiles(A.d, kRows, tiles);
   const uint32_t cap = c.table_width * c.page, keys = A.d.max_keys < cap ? A.d.max_keys : cap;
   const uint32_t span = A.d.window && A.d.window < keys ? A.d.window + A.d.max_q : keys;
   const uint32_t kblocks = (span < keys ? span : keys) / Sh::KS + 2u;
@@ -1340,7 +1340,7 @@ extern "C" int corm_llm_paged_attn(const corm_llm_paged_attn_desc* d, corm_strea
   // rows: 52 against 45)
   const uint32_t cap = c.table_width * c.page, span = A.d.window ? A.d.window + A.d.max_q : cap;
   const uint32_t keys = min(A.d.max_keys, min(cap, span < A.d.window ? cap : span));
-  const uint64_t ctas = tiles * c.B * c.KV;
+  const uint64_t ctas = paged::live_tiles(A.d, kRows, tiles);
   const bool few = rows <= 32u || (rows <= 64u && (keys > 640u || ctas <= 444u)) || (rows <= 128u && ctas <= 148u);
   if (!few && paged::tile_takes(A.d)) return paged::launch_tiles(A.d, A.tab, A.err, st);
   switch (c.HD * 2u + (c.bits == 8u)) {

@@ -1077,12 +1077,13 @@ int launch(TileArgs A, uint32_t tiles, cudaStream_t st) {
   // less than the items by those; without clusters a CTA goes from item to item.  8k keys
   // of 128 dimensions: 16 items 466 us with 1, 257 with 2, 144 with 4, 185 with 8; 36 items
   // 484, 257, 287, 279; 144 items of unlike lengths 489, 364; one prompt of 8192 1267, 1441
+  const uint64_t live = live_tiles(A.d, BMR, tiles);
   uint32_t X = 1;
   float best = 0.0f;
   for (uint32_t x = 1; x <= 8u && (x == 1u || ktiles >= 4u * x); x *= 2u) {
     const float at_once = x == 1u ? 148.0f : (float)resident_clusters<HD, BITS>(x);
     if (at_once < 1.0f) continue;
-    const float rounds = (float)blocks / at_once, least = c.B == 1u ? 2.0f : 1.5f;
+    const float rounds = (float)live / at_once, least = c.B == 1u ? 2.0f : 1.5f;
     const float cost = (rounds <= 1.0f ? 1.0f : (0.9f * rounds > least ? 0.9f * rounds : least)) * ((float)ktiles / (float)x + 3.5f);
     if (x == 1u || cost < best) X = x, best = cost;
   }
