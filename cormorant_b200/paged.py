@@ -100,10 +100,12 @@ class PagedBatch:
             tab[b, :len(t)] = t
         cu = np.concatenate([[0], np.cumsum(np.asarray(new, np.int64))]).astype(np.int32)
         dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        up = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(dev)  # noqa: E731
+        # one upload for the three
+        flat = torch.from_numpy(np.concatenate([tab.reshape(-1), cu, np.asarray(pos, np.int32).reshape(-1)])).to(dev)
+        n = tab.size
         most = max([int(p) + int(n) for p, n in zip(pos, new)] + [1])
-        return cls(up(tab), up(cu), up(np.asarray(pos)), rows=int(cu[-1]), max_q=max([int(n) for n in new] + [0]),
-                   max_keys=most)
+        return cls(flat[:n].view(tab.shape), flat[n:n + cu.size], flat[n + cu.size:], rows=int(cu[-1]),
+                   max_q=max([int(k) for k in new] + [0]), max_keys=most)
 
 
 class PagePool:
