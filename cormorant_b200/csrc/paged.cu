@@ -548,7 +548,7 @@ RowGrid row_grid(uint64_t rows, uint32_t turns, uint32_t most, uint32_t blocks_s
 // Measured (64 dimensions, 3 query heads a KV head, in a graph): 64 sequences of 128 to
 // 639 keys 12.4 us, bound by its chain of waits (page, K, maximum, sum, V; 6.4 us with one
 // sequence of 33 keys, 4 of them the kernel's); 8 sequences of 21k to 32k keys at 8 bits
-// 43 us, 3.0 TB/s: the K and V phases run at three quarters of the memory's rate, the
+// 39 us, 3.3 TB/s: the K and V phases run at three quarters of the memory's rate, the
 // softmax between them (about 250 of 1000 instructions a block) keeps only the stages'
 // copies under way; 128 dimensions, 4 query heads, 16 bits, 16 x 4k keys: 41 us, 4.9 TB/s.
 // A ring of 64-key stages that all warps share, a copy warp and 16-row MMAs: 29 and 146
@@ -592,8 +592,11 @@ __device__ __forceinline__ uint32_t score_word(uint32_t r, uint32_t i) {
   return r * PW + (i ^ (PW == 32 ? 8u * (r & 3u) : 8u * ((r >> 1) & 1u)));
 }
 
-template <int HD, int BITS>
-__global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_split_kernel(const __grid_constant__ SplitArgs A) {
+// OCC: CTAs an SM.  64 dimensions have a form of three, for batches that fill them, and
+// one of two whose registers hold the output's sums apart (8 sequences of 21k to 32k keys
+// at 8 bits 39 us against 43; 64 of 128 to 639 15.4 against 12.9)
+template <int HD, int BITS, int OCC>
+__global__ void __launch_bounds__(256, OCC) paged_attn_split_kernel(const __grid_constant__ SplitArgs A) {
   using Sh = SplitShape<HD, BITS>;
   constexpr uint32_t RB = Sh::RB, KS = Sh::KS, STB = Sh::STB, NKS = Sh::NKS, PW = Sh::PW;
   extern __shared__ __align__(128) uint8_t pa_sm[];
@@ -1003,7 +1006,7 @@ __global__ void __launch_bounds__(256, SplitShape<HD, BITS>::OCC) paged_attn_spl
     __syncwarp();
   };
   // the output's sums of weight 1, 2^8 and 2^16 apart, or (many dimensions) in one
-  constexpr bool APART = HD <= 32;
+  constexpr bool APART = HD <= 32 || (HD == 64 && OCC == 2);
   uint32_t acc[Sh::MT][4], acc1[APART ? Sh::MT : 1][4], acc2[APART ? Sh::MT : 1][4];
 #pragma unroll
   for (uint32_t j = 0; j < Sh::MT; j++)
@@ -1128,7 +1131,7 @@ uint32_t resident_clusters(uint32_t X, uint32_t d) {
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   if (dev < 16)
     if (const int n = known[dev][X][d].load(std::memory_order_relaxed)) return (uint32_t)n - 1u;
-  auto kern = paged_attn_split_kernel<HD, BITS>;
+  auto kern = paged_attn_split_kernel<HD, BITS, SplitShape<HD, BITS>::OCC>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(X * 1024u);
   cfg.blockDim = dim3(256);
@@ -1161,9 +1164,9 @@ int launch_split(SplitArgs A, uint32_t tiles, cudaStream_t st) {
   // a stage a warp, but no more than are used.  A cluster lies within a GPC, so X CTAs of
   // it are at once resident for all `blocks` when the device holds so many clusters at
   // some d CTAs an SM.  d CTAs share an SM's issue slots but hide one another's waits: the
-  // least (d + 1) / X is taken that leaves a warp two blocks (8 sequences x 5 heads of 21k
-  // to 32k keys: X = 3 77 us, 4 64, 5 56, 6 43, and 59 for 8, which is not resident at
-  // once; 4 x 5 heads at 16 bits: 104, 80, 68, 46, 8 43)
+  // least (d + 1) / X is taken that leaves a warp two blocks (in the form of three CTAs, 8
+  // sequences x 5 heads of 21k to 32k keys: X = 3 77 us, 4 64, 5 56, 6 43, and 59 for 8,
+  // which is not resident at once; 4 x 5 heads at 16 bits: 104, 80, 68, 46, 8 43)
   uint32_t X, occ = Sh::OCC, room, need, fixed;
   const uint32_t block = kWarps * A.rcap * Sh::PW * 4u;
   for (;; occ--) {
@@ -1187,7 +1190,9 @@ int launch_split(SplitArgs A, uint32_t tiles, cudaStream_t st) {
   while (stages < 4u && A.win * block + 2u * stages * kWarps * Sh::STB <= room) stages *= 2u;  // 1, 2 or 4
   A.stages = stages;
   const size_t smem = kWarps * stages * Sh::STB + (size_t)A.win * block + fixed;
-  auto kern = paged_attn_split_kernel<HD, BITS>;
+  auto kern = paged_attn_split_kernel<HD, BITS, Sh::OCC>;
+  if constexpr (HD == 64)
+    if (occ < 3u) kern = paged_attn_split_kernel<HD, BITS, 2>;
   // (one limit for every launch: another thread's may be between its limit and its launch)
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)split_smem(1)) != cudaSuccess)
     return corm::cuda_status("llm_paged_attn");
