@@ -328,19 +328,53 @@ def llm_decode_attn(qx, kc, vc, tab, ip, o, *, pos, B, KV, G, HD, rows, Q=16, wi
     check(lib().corm_llm_decode_attn(C.byref(d), st))
 
 
+def _row_stride(shape, strides, n):
+    """(rows, stride between them) of an array: a row is its trailing dimensions,
+    dense, as many as hold n elements, and the dimensions before count the rows;
+    None where it is not so laid out."""
+    k, width = len(shape), 1
+    while k > 0 and (width < n or shape[k - 1] == 1):
+        k -= 1
+        if shape[k] > 1 and strides[k] != width:
+            return None
+        width *= shape[k]
+    if width < n:
+        return None
+    rows, ld = 1, width
+    for d in range(k - 1, -1, -1):
+        if shape[d] == 1:
+            continue
+        if rows == 1:
+            ld = strides[d]
+        elif strides[d] != rows * ld:
+            return None
+        rows *= shape[d]
+    return rows, ld
+
+
 def _rows(t, name, rows, n, ld, dev):
     """(address, row stride) of a packed int16 array: rows of n elements at
-    stride ld (None: a 2-D tensor's own, or dense), a view of a wider array, too;
-    type, device and memory checked."""
+    stride ld (None: dense in a flat array, an array's own where it has more
+    dimensions, the last of which, as many as hold n elements, are a row: a view
+    of a wider array, too, such as a projection's heads; a view that is not
+    contiguous has no other).  Type, device and that the array itself holds the
+    rows checked."""
     if t.dtype is not torch.int16 or t.get_device() != dev:
         raise CormError(_lib.CORM_EINVAL, f"{name}: torch.int16 on device {dev} expected, got {t.dtype} on {t.device}")
     shape = t.shape
-    if ld is None:
-        ld = n if len(shape) != 2 or shape[0] <= 1 else t.stride(0)
-    if ld < n or t.numel() < (rows - 1) * ld + n or not t.is_contiguous():
-        room, need = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset(), (rows - 1) * ld + n if rows else 0
-        if ld < n or room < need or (t.numel() > 1 and t.stride(-1) != 1):
-            raise CormError(_lib.CORM_EINVAL, f"{name}: {rows} rows of {n} at stride {ld} expected, got {tuple(shape)}")
+    flat = len(shape) < 2 or (len(shape) == 2 and shape[0] <= 1)
+    if (flat or ld is not None) and t.is_contiguous():
+        ld = n if ld is None else ld
+        good = ld >= n and t.numel() >= (rows - 1) * ld + n
+    elif rows < 1:
+        ld, good = n if ld is None else ld, True
+    else:
+        at = _row_stride(shape, t.stride(), n)
+        good = at is not None and at[0] >= rows and (at[1] >= n or rows == 1) and ld in (None, at[1])
+        ld = max(at[1], n) if good else ld
+    if not good:
+        raise CormError(_lib.CORM_EINVAL,
+                        f"{name}: {rows} rows of {n} at stride {ld or 'their own'} expected, got {tuple(shape)} at {t.stride()}")
     return t.data_ptr(), ld
 
 

@@ -229,6 +229,49 @@ def test_host_classes_refuse():
         ops.llm_paged_read(cache, batch, None, None)
 
 
+def _row_views(H, HD):
+    """(tensor, stride of its rows) of what a program holds 8 packed rows of H heads of
+    HD in, and the tensors that do not hold them, on the CPU."""
+    n, z = H * HD, lambda *s: torch.zeros(s, dtype=torch.int16)  # noqa: E731
+    W = 3 * n
+    good = [(z(8, n), n), (z(11, n), n), (z(8 * n), n), (z(9 * n + 5), n), (z(8, W), W), (z(8, W)[:, 5:5 + n], W),
+            (z(1, 8 * n), n), (z(8, H, HD), n), (z(2, 4, n), n), (z(2, 4, H, HD), n),
+            (z(8, W)[:, :n].unflatten(1, (H, HD)), W),            # a projection's heads
+            (z(8, 2 * H + 1, HD)[:, 1:1 + H], (2 * H + 1) * HD),  # the same, from the heads' array
+            (z(2, 4, W)[..., n:2 * n], W), (z(2, 9, n)[:, ::9], 9 * n)]
+    bad = [z(7, n), z(8 * n - 1), z(16, n)[:5], z(16 * n)[:5 * n], z(16, 2 * n)[:, :n - 1], z(8, W)[:, ::2],
+           z(16, H, HD)[:7], z(n, 8).t(), z(1, n).expand(8, n), z(3, 5, W)[:2, :4, :n]]
+    if H > 1:
+        good.append((z(8, 2 * H, HD), 2 * n))                                           # its first heads
+        bad += [z(8, H, 2, HD)[:, :, 0], z(8, HD, H).transpose(1, 2), z(8, 2 * H, HD)[:, ::2]]  # heads apart
+    return good, bad
+
+
+@pytest.mark.parametrize("H,HD", [(4, 64), (1, 16), (3, 32)])
+def test_rows_of_a_view(H, HD):
+    """The stride of a packed array is its own, whatever its rank; one that does not
+    hold the rows within itself is refused, though its storage might."""
+    from cormorant_b200 import ops
+    n = H * HD
+    good, bad = _row_views(H, HD)
+    for t, ld in good:
+        rows = 8 if t.numel() >= 8 * n else 2
+        assert ops._rows(t, "x", rows, n, None, -1) == (t.data_ptr(), ld), (t.shape, t.stride())
+        assert ops._rows(t, "x", rows, n, ld, -1) == (t.data_ptr(), ld), (t.shape, t.stride())
+    for t in bad:
+        for ld in (None, n, 3 * n):
+            with pytest.raises(_lib.CormError):
+                ops._rows(t, "x", 8, n, ld, -1)
+    flat = torch.zeros(7 * 3 * n + n, dtype=torch.int16)  # a stride given for a flat array
+    assert ops._rows(flat, "x", 8, n, 3 * n, -1)[1] == 3 * n
+    assert ops._rows(torch.zeros((24, n), dtype=torch.int16), "x", 8, n, 3 * n, -1)[1] == 3 * n
+    for t, ld in ((flat, 3 * n + 1), (flat[1:], 3 * n), (flat, n - 1), (torch.zeros((8, 3 * n), dtype=torch.int16)[:, :n], n)):
+        with pytest.raises(_lib.CormError):
+            ops._rows(t, "x", 8, n, ld, -1)
+    one = torch.zeros((5, 2 * n), dtype=torch.int16)[2:3, :n]  # one row: any stride
+    assert ops._rows(one, "x", 1, n, None, -1)[0] == one.data_ptr()
+
+
 def test_page_pool():
     p = paged.PagePool(5, 16)
     a = p.extend("a", 17)
@@ -421,6 +464,55 @@ def test_read_vs_oracle(HD, bits, page, KV):
     assert np.array_equal(one.cpu().numpy(), want[1])
     ops.llm_paged_read(cache, batch, one, None)
     assert np.array_equal(one.cpu().numpy(), want[0])
+
+
+@gpu
+@pytest.mark.parametrize("case", [PREPS[1], PREPS[6]], ids=["hd64", "hd128"])
+@pytest.mark.parametrize("split", [True, False], ids=["columns", "heads"])
+def test_head_views_in_and_out(case, split):
+    """The three operators on [rows][heads][HD] views of fused arrays, cut from the
+    columns of one with two dimensions or the heads of one with three: the heads
+    between them are left as they were."""
+    from cormorant_b200 import ops
+    HD, H, KV, bc = case[0], case[6], case[7], case[8]
+    c, rows, q0, k0, v0, kw = _prep_case(np.random.default_rng(sum(map(int, case))), *case)
+    cache, batch = _handles(c, rows)
+
+    def fused(*parts):  # each part's heads, a head of -7 before, between and behind them
+        t = torch.full((rows, sum(parts) + len(parts) + 1, HD), -7, dtype=torch.int16, device="cuda")
+        ats = [1 + sum(parts[:i]) + i for i in range(len(parts))]
+        wide = t.view(rows, -1)
+        return t, [wide[:, at * HD:(at + p) * HD].unflatten(1, (p, HD)) if split else t[:, at:at + p]
+                   for at, p in zip(ats, parts)]
+
+    def check(t, views, wants):
+        for v, w in zip(views, wants):
+            assert np.array_equal(v.reshape(rows, -1).cpu().numpy(), w)
+            v.fill_(-7)
+        assert (t == -7).all()
+    t, ins = fused(H, KV, KV)
+    for v, x in zip(ins, (q0, k0, v0)):
+        v.copy_(_dev(x).view(v.shape))
+    g = {k: _dev(v) if isinstance(v, np.ndarray) else v for k, v in kw.items()}
+    qt, (q,) = fused(H)
+    ops.llm_paged_prep(cache, batch, *ins, q, H=H, pq_bc=bc, pk_bc=bc, pv_bc=bc, **g)
+    want = np.full((rows, H * HD), -7, np.int64)
+    OP.prep(c, q0, k0, v0, want, H=H, **kw)
+    _same_bytes(c, cache)
+    smx = _smx(H, HD)
+    ot, (o,) = fused(H)
+    ops.llm_paged_attn(cache, batch, q, o, H=H, smx=_dev(smx))
+    att = np.full((rows, H * HD), -7, np.int64)
+    OP.attn(c, want, att, H=H, smx=smx)
+    check(ot, [o], [att])
+    check(qt, [q], [want])
+    check(t, ins, [q0, k0, v0])
+    kvt, kv = fused(KV, KV)
+    ops.llm_paged_read(cache, batch, *kv)
+    words = [np.full((rows, KV * HD), -7, np.int64) for _ in range(2)]
+    OP.read(c, *words)
+    check(kvt, kv, words)
+    assert ops.device_status() == 0
 
 
 def _run_attn(c, rows, H, smx, rng, *, window=0, max_q=None, max_keys=None, hi=32768, odd=False):
