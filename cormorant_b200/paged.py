@@ -55,15 +55,16 @@ class PagedCache:
     def desc(self, batch: "PagedBatch") -> _lib.PagedCacheDesc:
         """The cache and the batch as the library takes them (made once for a
         pair: both keep their tensors)."""
-        if batch._pair is not self:
+        pair = batch._pair  # (cache, descriptor), replaced as one: other threads may use the batch with theirs
+        if pair is None or pair[0] is not self:
             if batch.device != self.device:
                 _bad(f"paged: the batch is on {batch.device}, the cache on {self.device}")
             ptr = [None if t is None else t.data_ptr() for t in (self.kc, self.vc, self.ks, self.vs, batch.table,
                                                                  batch.cu, batch.pos)]
-            batch._desc = _lib.PagedCacheDesc(*ptr, self.pages, self.page, self.bits, self.KV, self.HD, batch.B,
-                                              batch.width, batch.rows)
-            batch._pair = self
-        return batch._desc
+            pair = self, _lib.PagedCacheDesc(*ptr, self.pages, self.page, self.bits, self.KV, self.HD, batch.B,
+                                             batch.width, batch.rows)
+            batch._pair = pair
+        return pair[1]
 
 
 class PagedBatch:
@@ -87,7 +88,7 @@ class PagedBatch:
         self.max_q = self.rows if max_q is None else int(max_q)
         self.max_keys = 0x7FFFFFFF if max_keys is None else int(max_keys)
         self.device = table.device
-        self._pair = self._desc = None
+        self._pair = None
 
     @classmethod
     def of(cls, tables: Sequence[Sequence[int]], new: Sequence[int], pos: Sequence[int], device=None,

@@ -229,6 +229,34 @@ def test_host_classes_refuse():
         ops.llm_paged_read(cache, batch, None, None)
 
 
+def test_one_batch_with_two_caches():
+    """A batch that two threads use with a cache each: whatever the other one does
+    between two lines of a call, the descriptor is of the call's own cache."""
+    import sys
+    caches = [paged.PagedCache(4, 16, 2, 64, device="cpu") for _ in range(2)]
+    batch = paged.PagedBatch.of([[0], [1, 2]], [1, 2], [3, 20], device="cpu")
+    steps = []
+
+    def other(frame, event, arg):  # the other thread's whole call, before every line of this one's
+        if frame.f_code is paged.PagedCache.desc.__code__:
+            sys.settrace(None)
+            assert caches[1].desc(batch).kc == caches[1].kc.data_ptr()
+            steps.append(event)
+            sys.settrace(other)
+            return other
+    for _ in range(2):
+        before = sys.gettrace()
+        sys.settrace(other)
+        try:
+            got = caches[0].desc(batch)
+        finally:
+            sys.settrace(before)
+        assert (got.kc, got.vc) == (caches[0].kc.data_ptr(), caches[0].vc.data_ptr())
+        assert caches[0].desc(batch).kc == caches[0].kc.data_ptr()
+        assert caches[1].desc(batch).kc == caches[1].kc.data_ptr()
+    assert len(steps) > 6
+
+
 def _row_views(H, HD):
     """(tensor, stride of its rows) of what a program holds 8 packed rows of H heads of
     HD in, and the tensors that do not hold them, on the CPU."""
