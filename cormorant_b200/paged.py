@@ -10,6 +10,7 @@ pass replays with what they then hold.
 """
 from __future__ import annotations
 
+import weakref
 from typing import Dict, List, Optional, Sequence
 
 import numpy as np
@@ -55,15 +56,17 @@ class PagedCache:
     def desc(self, batch: "PagedBatch") -> _lib.PagedCacheDesc:
         """The cache and the batch as the library takes them (made once for a
         pair: both keep their tensors)."""
-        pair = batch._pair  # (cache, descriptor), replaced as one: other threads may use the batch with theirs
-        if pair is None or pair[0] is not self:
+        # (cache, descriptor), replaced as one: other threads may use the batch with theirs;
+        # the cache by a weak reference: its pages are not the batch's to hold
+        pair = batch._pair
+        if pair is None or pair[0]() is not self:
             if batch.device != self.device:
                 _bad(f"paged: the batch is on {batch.device}, the cache on {self.device}")
             ptr = [None if t is None else t.data_ptr() for t in (self.kc, self.vc, self.ks, self.vs, batch.table,
                                                                  batch.cu, batch.pos)]
-            pair = self, _lib.PagedCacheDesc(*ptr, self.pages, self.page, self.bits, self.KV, self.HD, batch.B,
-                                             batch.width, batch.rows)
-            batch._pair = pair
+            desc = _lib.PagedCacheDesc(*ptr, self.pages, self.page, self.bits, self.KV, self.HD, batch.B, batch.width,
+                                       batch.rows)
+            batch._pair = pair = (weakref.ref(self), desc)
         return pair[1]
 
 

@@ -257,6 +257,21 @@ def test_one_batch_with_two_caches():
     assert len(steps) > 6
 
 
+def test_a_batch_does_not_hold_a_cache():
+    """The pages go with their cache, not with the last batch used on them."""
+    import gc
+    import weakref
+    cache = paged.PagedCache(4, 16, 2, 64, device="cpu")
+    batch = paged.PagedBatch.of([[0]], [1], [3], device="cpu")
+    desc, pages = cache.desc(batch), weakref.ref(cache.kc)
+    assert cache.desc(batch) is desc
+    del cache
+    gc.collect()
+    assert pages() is None
+    cache = paged.PagedCache(4, 16, 2, 64, device="cpu")
+    assert cache.desc(batch).kc == cache.kc.data_ptr()
+
+
 def _row_views(H, HD):
     """(tensor, stride of its rows) of what a program holds 8 packed rows of H heads of
     HD in, and the tensors that do not hold them, on the CPU."""
