@@ -372,6 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               *(int4*)(dst + h * Sh::HALF_BYTES + i) = make_int4(0, 0, 0, 0);
           sm100::fence_proxy_async_smem();
         }
+        __syncwarp();  // every lane's zeros come before the arrival (a vote orders no memory)
         const uint32_t cnt = __popc(__ballot_sync(0xffffffffu, good));
         if (lane == 0) sm100::mbar_expect_tx(&kv_full[s], cnt * sub * Sh::RB);
         __syncwarp();

@@ -709,6 +709,29 @@ def test_attn_missing_pages_and_late_positions(HD, bits, new):
 
 
 @gpu
+@pytest.mark.parametrize("window", [0, 150])
+@pytest.mark.parametrize("HD,bits,page", [(64, 16, 16), (64, 8, 128), (128, 16, 64), (128, 8, 256)])
+def test_attn_tiles_of_missing_pages(HD, bits, page, window):
+    """Rows of 128-row tiles over pages that are not there: single ones, whole tiles
+    of keys (whose copies are none), one after tiles that are there; positions past
+    the table, cu and pos out of range, rows past max_q."""
+    rng = np.random.default_rng(HD + bits + window)
+    H, KV, new = 4, 2, 70
+    ctx, n = [700, 300, 0, 90], [new, new, new, new + 9]
+    table, cu, pos, rows = _batch(rng, 130, page, ctx, n, spare=0, extra=1)
+    c = _random_cache(rng, 130, KV, page, HD, bits, 3000)
+    c.table, c.cu, c.pos = table, cu, pos
+    per = max(1, 128 // page)
+    c.table[0, 2 * per:4 * per] = -1                 # two tiles of keys and more
+    c.table[0, 0], c.table[0, -1] = 130, 1 << 30
+    c.table[1, :per] = -9                            # the first tile
+    c.pos[2] = c.cap - 20                            # the last rows lie past the table
+    c.pos[3] = -4
+    c.cu[-1] = rows + 9
+    _run_attn(c, rows, H, _smx(H, HD, f_s=10), rng, window=window, hi=3000, max_q=new, max_keys=ctx[0] + new)
+
+
+@gpu
 def test_attn_equal_scores_and_extremes():
     """Zero queries (every score alike: P = 1 / keys), the most negative words
     (a score of -2^15 where every sum saturates), a single key."""
