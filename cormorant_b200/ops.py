@@ -452,13 +452,20 @@ def llm_paged_read(cache, batch, k, v, *, ldk=None, ldv=None):
 
 def greedy_embed(logits, table, out, ids=None, *, batch, vocab, dim, ld=None):
     """corm_greedy_embed: ids = first argmax of each int16 logits row; out
-    (int32) = those rows of the int32 table."""
-    _i16(logits, "logits")
-    if table.dtype != torch.int32 or out.dtype != torch.int32 or (ids is not None and ids.dtype != torch.int32):
-        raise CormError(_lib.CORM_EINVAL, "table / out / ids must be int32")
+    (int32) = those rows of the int32 table.  Every array holds what the launch
+    reads or writes of it, on the current device."""
+    dev = logits.get_device()
+    plogits, ld = _rows(logits, "logits", batch, vocab, vocab if ld is None and logits.is_contiguous() else ld, dev)
+    for t, nm, need in ((table, "table", vocab * dim), (out, "out", batch * dim), (ids, "ids", batch)):
+        if t is not None and (t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous() or
+                              t.numel() < need):
+            raise CormError(_lib.CORM_EINVAL, f"{nm}: {need} contiguous torch.int32 on device {dev} expected, got "
+                                              f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    _ptr(logits)
     st = _ready()
-    d = _lib.GreedyDesc(_ptr(logits), _ptr(table), _ptr(out), _ptr(ids), batch, vocab, dim,
-                        vocab if ld is None else ld)
+    if dev != _tls.dev:
+        raise CormError(_lib.CORM_EINVAL, f"the logits are on {logits.device}, the current device is {_tls.dev}")
+    d = _lib.GreedyDesc(plogits, _ptr(table), _ptr(out), _ptr(ids), batch, vocab, dim, ld)
     check(lib().corm_greedy_embed(C.byref(d), st))
 
 
