@@ -101,9 +101,9 @@ class PagedLlamaRunner:
         """The rows a pass is built for: graphs of few row counts serve all."""
         return rows if rows <= 16 else -(-rows // 64) * 64
 
-    def _pass(self, seqs: Sequence[Hashable], new: Sequence[int], h: torch.Tensor) -> torch.Tensor:
-        """The layers over h (int32, the new rows packed; whole padded rows), the
-        last row of every sequence through the head: its logits."""
+    def _room(self, seqs: Sequence[Hashable], new: Sequence[int]) -> List[int]:
+        """The positions of the sequences' next rows; an error where a pass over
+        ``new`` rows of each cannot be made."""
         m = self.m
         at = [self.length.get(s, 0) for s in seqs]
         if len(set(seqs)) != len(seqs) or not seqs or min(new) < 1:
@@ -114,6 +114,12 @@ class PagedLlamaRunner:
         need = sum(max(-(-(a + n) // self.pool.page) - len(self.pool.held.get(s, [])), 0) for s, a, n in zip(seqs, at, new))
         if need > len(self.pool.free):
             raise MemoryError(f"PagedLlamaRunner: {need} pages wanted, {len(self.pool.free)} free (no sequence changed)")
+        return at
+
+    def _pass(self, seqs: Sequence[Hashable], new: Sequence[int], at: Sequence[int], h: torch.Tensor) -> torch.Tensor:
+        """The layers over h (int32, the new rows packed; whole padded rows), the
+        last row of every sequence through the head: its logits.  at: ``_room``'s."""
+        m = self.m
         tables = [self.pool.extend(s, a + n) for s, a, n in zip(seqs, at, new)]
         batch = PagedBatch.of(tables, new, at, device=self.device)
         sim = self._sim(self._padded(batch.rows), False)
@@ -145,16 +151,19 @@ class PagedLlamaRunner:
         flat = np.concatenate([np.asarray(i, np.int64).reshape(-1) for i in ids]) if new else np.zeros(0, np.int64)
         if flat.size and (flat.min() < 0 or flat.max() >= self.m.vocab):
             raise CormError(CORM_EINVAL, f"PagedLlamaRunner: token ids in [0, {self.m.vocab}) expected")
+        at = self._room(seqs, new)
         h, n = self._rows(flat.size), flat.size * self.m.D
         torch.index_select(self.table, 0, torch.from_numpy(flat).to(self.device), out=h[:n].view(flat.size, self.m.D))
-        return self._pass(seqs, new, h)
+        return self._pass(seqs, new, at, h)
 
     def step(self, seqs: Sequence[Hashable], logits: torch.Tensor, ids: Optional[torch.Tensor] = None) -> torch.Tensor:
         """A greedy token for each of ``seqs`` after ``logits`` (their order),
         chosen on the device (int32 ``ids`` if given); its logits."""
+        new = [1] * len(seqs)
+        at = self._room(seqs, new)  # (before ids is written)
         h = self._rows(len(seqs))
         ops.greedy_embed(logits, self.table, h, ids, batch=len(seqs), vocab=self.m.vocab, dim=self.m.D)
-        return self._pass(seqs, [1] * len(seqs), h)
+        return self._pass(seqs, new, at, h)
 
     def generate(self, prompts: Dict[Hashable, Sequence[int]], steps: int) -> Dict[Hashable, List[int]]:
         """The prompts in one pass, then ``steps`` greedy tokens of each."""

@@ -144,6 +144,21 @@ def test_runner_refuses(paged_cpu):
     assert r.length == dict(a=17)
 
 
+def test_step_refuses_before_it_writes(paged_cpu):
+    """A step that cannot be made leaves ids, the sequences and the pool as they were."""
+    m = WL.LlamaModel(batch=1, seq=16, cache=32, seed=4, **SMALL)
+    r = PagedLlamaRunner(m, pages=3, page=16, device="cpu")
+    lg = r.append("ab", [[1] * 32, [2] * 16])
+    ids = torch.full((2,), -5, dtype=torch.int32)
+    for seqs, err in (("aa", CormError), ("", CormError), ("ab", CormError), ("b", MemoryError)):
+        with pytest.raises(err):  # twice a sequence, none, a at the model's 32 positions, no page for b's 17th token
+            r.step(seqs, lg, ids)
+        assert ids.tolist() == [-5, -5] and r.length == dict(a=32, b=16) and not r.pool.free
+    r.release("a")
+    r.step("b", lg[m.vocab:], ids)
+    assert ids[0] >= 0 and ids[1] == -5 and r.length == dict(b=17)
+
+
 @gpu
 @pytest.mark.parametrize("dims,lengths,page", [
     (dict(layers=2, hidden=64, heads=4, kv_heads=2, head_dim=16, ffn=128, vocab=300), (9, 3, 70, 40), 16),
