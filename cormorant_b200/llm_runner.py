@@ -145,10 +145,12 @@ class PagedLlamaRunner:
     def append(self, seqs: Sequence[Hashable], ids: Sequence[Sequence[int]]) -> torch.Tensor:
         """One pass over new tokens of some sequences (prompts, chunks, single
         tokens together): int16 logits [len(seqs)][vocab] of their last ones."""
-        new = [len(i) for i in ids]
-        if len(new) != len(seqs):
-            raise CormError(CORM_EINVAL, f"PagedLlamaRunner: {len(seqs)} sequences, tokens of {len(new)}")
-        flat = np.concatenate([np.asarray(i, np.int64).reshape(-1) for i in ids]) if new else np.zeros(0, np.int64)
+        tokens = [np.asarray(i, np.int64) for i in ids]
+        if len(tokens) != len(seqs) or any(t.ndim != 1 for t in tokens):
+            raise CormError(CORM_EINVAL, f"PagedLlamaRunner: a list of tokens for each of {len(seqs)} sequences expected, got "
+                                         f"{[t.shape for t in tokens]}")
+        new = [t.size for t in tokens]
+        flat = np.concatenate(tokens) if new else np.zeros(0, np.int64)
         if flat.size and (flat.min() < 0 or flat.max() >= self.m.vocab):
             raise CormError(CORM_EINVAL, f"PagedLlamaRunner: token ids in [0, {self.m.vocab}) expected")
         at = self._room(seqs, new)

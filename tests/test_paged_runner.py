@@ -144,6 +144,19 @@ def test_runner_refuses(paged_cpu):
     assert r.length == dict(a=17)
 
 
+def test_append_takes_one_list_a_sequence(paged_cpu):
+    """Tokens in an array of another shape are refused: its length is not their number."""
+    m = WL.LlamaModel(batch=1, seq=16, cache=32, seed=4, **SMALL)
+    r = PagedLlamaRunner(m, pages=3, page=16, device="cpu")
+    for bad in (np.array([[1, 2, 3]]), [[1], [2]], torch.tensor([[4, 5]]), np.array(3)):
+        with pytest.raises(CormError):
+            r.append("ab", [[1], bad])
+    assert not r.length and len(r.pool.free) == 3
+    want = r.append("a", [[1, 2, 3]])
+    for s, good in (("b", np.array([1, 2, 3], np.uint8)), ("c", torch.tensor([1, 2, 3]))):
+        assert torch.equal(r.append(s, [good])[:m.vocab], want[:m.vocab])
+
+
 def test_step_refuses_before_it_writes(paged_cpu):
     """A step that cannot be made leaves ids, the sequences and the pool as they were."""
     m = WL.LlamaModel(batch=1, seq=16, cache=32, seed=4, **SMALL)
