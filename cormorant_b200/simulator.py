@@ -1247,9 +1247,9 @@ class GpuSimulator:
         pv = None if sn.v_direct else get(sn.inputs[5])
 
         def table(key, data):  # int32, on the device once for all passes that share the weights
-            if key not in self._weights:
-                self._weights[key] = torch.from_numpy(np.ascontiguousarray(data, np.int32)).to(self.device)
-            return self._weights[key]
+            if key not in self._weights:  # (the host array beside it: its id stays its own)
+                self._weights[key] = data, torch.from_numpy(np.ascontiguousarray(data, np.int32)).to(self.device)
+            return self._weights[key][1]
         rope, smx = table(("paged.rope", id(sn.rope)), sn.rope), table(("paged.smx", sn.smx.tobytes()), sn.smx)
         q, y = self._alloc(sn.output.numel), self._alloc(sn.output.numel)
         ops.llm_paged_prep(caches[sn.layer], batch, q0, k0, v, q, H=sn.H, rope=rope, pq=pq, pk=pk, pv=pv,

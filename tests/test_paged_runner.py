@@ -157,6 +157,43 @@ def test_append_takes_one_list_a_sequence(paged_cpu):
         assert torch.equal(r.append(s, [good])[:m.vocab], want[:m.vocab])
 
 
+def test_rotation_tables_of_shared_weights(paged_cpu, monkeypatch):
+    """Simulators that share weights, each graph with a rotation table of its own: a
+    table that is gone does not serve one that came to lie at its address."""
+    import gc
+
+    from cormorant_b200 import attention as AT
+    from cormorant_b200.paged import PagedBatch, PagedCache
+    from cormorant_b200.simulator import GpuSimulator
+    m = WL.LlamaModel(batch=1, seq=16, cache=32, seed=4, **SMALL)
+    first = GpuSimulator(m.paged_graph(4), device="cpu")
+    m.rope = None
+    h = torch.from_numpy(np.rint(m.emb[[3, 9, 4, 7]] * 2.0 ** m.E["fr"]).astype(np.int32).reshape(-1))
+
+    def run(share):
+        g = m.paged_graph(4)
+        sim = GpuSimulator(g, device="cpu", share=share)
+        sim.paged = ([PagedCache(2, 16, m.KV, m.HD, device="cpu")], PagedBatch.of([[0]], [4], [5], device="cpu"))
+        out = g.output_tensors[0].onnx_name
+        res, _ = sim.forward_raw({"h_step": h}, keep=[out])
+        return res[out][:4 * m.D].clone()
+    turned = AT.paged_rope(m.sin, m.cos)  # another rotation
+    wrap = torch.from_numpy
+    monkeypatch.setattr(torch, "from_numpy", lambda a: wrap(a).clone())  # as an upload to a device does
+    m.rope = AT.paged_rope(m.cos, m.sin)
+    at, one = id(m.rope), run(first)
+    m.rope = None
+    gc.collect()
+    kept = []
+    for _ in range(2000):
+        m.rope = turned.copy()
+        if id(m.rope) == at:
+            break
+        kept.append(m.rope)
+    two = run(first)
+    assert torch.equal(two, run(None)) and not torch.equal(one, two)
+
+
 def test_step_refuses_before_it_writes(paged_cpu):
     """A step that cannot be made leaves ids, the sequences and the pool as they were."""
     m = WL.LlamaModel(batch=1, seq=16, cache=32, seed=4, **SMALL)
