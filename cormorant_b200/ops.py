@@ -397,6 +397,15 @@ def _entries(t, n, name, dev):
     return t.data_ptr()
 
 
+def _rope_rows(rope, rot, dev):
+    """The positions of a rotation table: int32 rows of rot, or those flat."""
+    if rope.dtype is not torch.int32 or rope.get_device() != dev or not rope.is_contiguous() or rot < 1 or \
+            rope.numel() < rot or (rope.shape[-1] != rot if rope.dim() > 1 else rope.numel() % rot):
+        raise CormError(_lib.CORM_EINVAL, f"rope: a contiguous int32 [positions][{rot}] table on device {dev} expected, got "
+                                          f"{tuple(rope.shape)} {rope.dtype} on {rope.device}")
+    return rope.numel() // rot
+
+
 def llm_paged_prep(cache, batch, q0, k0, v0, q, *, H, rope, pq, pk, pv=None, rot=None, interleaved=False, pq_bc=False,
                    pk_bc=False, pv_bc=False, v_direct=False, nq=None, nk=None, eps_q=0, eps_k=0, ldq0=None, ldk=None,
                    ldv=None, ldq=None):
@@ -409,9 +418,7 @@ def llm_paged_prep(cache, batch, q0, k0, v0, q, *, H, rope, pq, pk, pv=None, rot
     HD, R = cache.HD, batch.rows
     nh, nkv = H * HD, cache.KV * HD
     rot = HD if rot is None else int(rot)
-    if rope.dtype is not torch.int32 or rope.get_device() != dev or not rope.is_contiguous() or rot < 1 or \
-            rope.numel() < rot:
-        raise CormError(_lib.CORM_EINVAL, f"rope: a contiguous int32 [positions][{rot}] table on device {dev} expected")
+    positions = _rope_rows(rope, rot, dev)
     pq0, ldq0 = _rows(q0, "q0", R, nh, ldq0, dev)
     pk0, ldk = _rows(k0, "k0", R, nkv, ldk, dev)
     pv0, ldv = _rows(v0, "v0", R, nkv, ldv, dev)
@@ -421,7 +428,7 @@ def llm_paged_prep(cache, batch, q0, k0, v0, q, *, H, rope, pq, pk, pv=None, rot
         _entries(pk, 1 if pk_bc else nkv, "pk", dev),
         None if v_direct else _entries(pv, 1 if pv_bc else nkv, "pv", dev), _entries(nq, HD, "nq", dev),
         _entries(nk, HD, "nk", dev), eps_q, eps_k, ldq0, ldk, ldv, ldq, H, rot, int(bool(interleaved)),
-        rope.numel() // rot, (1 if pq_bc else 0) | (2 if pk_bc else 0) | (4 if pv_bc else 0) | (8 if v_direct else 0))
+        positions, (1 if pq_bc else 0) | (2 if pk_bc else 0) | (4 if pv_bc else 0) | (8 if v_direct else 0))
     check(lib().corm_llm_paged_prep(C.byref(d), st))
 
 

@@ -315,6 +315,18 @@ def test_rows_of_a_view(H, HD):
     assert ops._rows(one, "x", 1, n, None, -1)[0] == one.data_ptr()
 
 
+def test_rotation_table_shapes():
+    """A table's rows are rot wide: one of another width is refused, not read as more rows."""
+    from cormorant_b200 import ops
+    z = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    for t, rot, rows in ((z(8, 64), 64, 8), (z(8, 32), 32, 8), (z(256), 32, 8), (z(2, 3, 16), 16, 6)):
+        assert ops._rope_rows(t, rot, -1) == rows
+    for t, rot in ((z(8, 64), 32), (z(8, 32), 64), (z(4, 64), 128), (z(100), 64), (z(0, 64), 64), (z(63), 64), (z(8, 64), 0),
+                   (z(8, 64), -2), (z(8, 64).long(), 64), (z(8, 128)[:, :64], 64), (z(8, 64)[::2], 64)):
+        with pytest.raises(_lib.CormError, match="rope"):
+            ops._rope_rows(t, rot, -1)
+
+
 def test_page_pool():
     p = paged.PagePool(5, 16)
     a = p.extend("a", 17)
@@ -989,4 +1001,21 @@ def test_gpu_refusals():
                dict(rope=rope[:0])):
         with pytest.raises(_lib.CormError):
             ops.llm_paged_prep(cache, batch, z(256), z(128), z(128), z(256), **dict(ok, **kw))
+    assert ops.device_status() == 0
+
+
+@gpu
+def test_gpu_refused_rotation_tables():
+    """The preparation asks for a table of its rot's width."""
+    from cormorant_b200 import ops
+    cache, batch = paged.PagedCache(4, 16, 2, 64), paged.PagedBatch.of([[0, 1]], [4], [3])
+    z = lambda n: torch.zeros((4, n), dtype=torch.int16, device="cuda")  # noqa: E731
+    e = torch.zeros((1, 16), dtype=torch.uint8, device="cuda")
+    rope = torch.zeros((8, 64), dtype=torch.int32, device="cuda")
+    ok = dict(H=4, pq=e, pk=e, pv=e, pq_bc=True, pk_bc=True, pv_bc=True)
+    for kw in (dict(rope=rope), dict(rope=rope.view(-1)), dict(rope=rope[:, :32].contiguous(), rot=32)):
+        ops.llm_paged_prep(cache, batch, z(256), z(128), z(128), z(256), **ok, **kw)
+    for kw in (dict(rope=rope, rot=32), dict(rope=rope[:, :32].contiguous()), dict(rope=rope.view(-1)[:100])):
+        with pytest.raises(_lib.CormError, match="rope"):
+            ops.llm_paged_prep(cache, batch, z(256), z(128), z(128), z(256), **ok, **kw)
     assert ops.device_status() == 0
