@@ -414,6 +414,8 @@ def llm_paged_prep(cache, batch, q0, k0, v0, q, *, H, rope, pq, pk, pv=None, rot
     ``rot`` dimensions by ``rope`` int32 [positions][rot], q into ``q``, k and the
     re-rounded v0 into the cache's pages (``paged.PagedCache``, ``PagedBatch``).
     pq / pk / pv: 16-byte parameter entries (any dtype)."""
+    if not (0 <= eps_q < 1 << 62 and 0 <= eps_k < 1 << 62):
+        raise CormError(_lib.CORM_EINVAL, f"eps_q {eps_q}, eps_k {eps_k} (0 .. 2^62 - 1)")
     c, st, dev = _paged(cache, batch)
     HD, R = cache.HD, batch.rows
     nh, nkv = H * HD, cache.KV * HD
@@ -436,6 +438,8 @@ def llm_paged_attn(cache, batch, q, o, *, H, smx, window=0, ldq=None, ldo=None):
     """corm_llm_paged_attn: the causal (windowed) grouped-head attention of the
     packed q rows over the cache's pages into o; ``smx`` int32 [H][2]: each head's
     softmax registers (Cm, Cs | f_p << 8)."""
+    if not 0 <= window < 1 << 32:
+        raise CormError(_lib.CORM_EINVAL, f"window {window} (0: none, or below 2^32)")
     c, st, dev = _paged(cache, batch)
     n, R = H * cache.HD, batch.rows
     if smx.dtype is not torch.int32 or smx.get_device() != dev or not smx.is_contiguous() or smx.numel() < 2 * H:

@@ -83,13 +83,15 @@ class PagedBatch:
         for t, nm in ((table, "table"), (cu, "cu"), (pos, "pos")):
             if t.dtype != torch.int32 or not t.is_contiguous() or t.device != table.device:
                 _bad(f"PagedBatch: {nm}: contiguous int32 on one device expected, got {t.dtype} on {t.device}")
-        if table.dim() != 2 or pos.numel() != table.shape[0] or cu.numel() != table.shape[0] + 1 or rows < 0:
-            _bad("PagedBatch: table [B][blocks], cu [B + 1], pos [B], rows >= 0")
+        if table.dim() != 2 or pos.numel() != table.shape[0] or cu.numel() != table.shape[0] + 1 or \
+                not 0 <= rows < 1 << 31 or not 0 <= (0 if max_q is None else max_q) < 1 << 31:
+            _bad(f"PagedBatch: table [B][blocks], cu [B + 1], pos [B], rows and max_q 0 .. 2^31 - 1 expected, got "
+                 f"{tuple(table.shape)}, {cu.numel()}, {pos.numel()}, {rows}, {max_q}")
         self.table, self.cu, self.pos = table, cu, pos
         self.B, self.width = int(table.shape[0]), int(table.shape[1])
         self.rows = int(rows)
         self.max_q = self.rows if max_q is None else int(max_q)
-        self.max_keys = 0x7FFFFFFF if max_keys is None else int(max_keys)
+        self.max_keys = 0x7FFFFFFF if max_keys is None else min(max(int(max_keys), 0), 0x7FFFFFFF)
         self.device = table.device
         self._pair = None
 

@@ -327,6 +327,28 @@ def test_rotation_table_shapes():
             ops._rope_rows(t, rot, -1)
 
 
+def test_numbers_that_do_not_fit():
+    """Lengths, windows and eps that the descriptors' fields would wrap are refused (the
+    hint of the keys, of which any value is right, is cut to its range)."""
+    from cormorant_b200 import ops
+    i32 = dict(dtype=torch.int32)
+    a = torch.zeros((1, 2), **i32), torch.zeros(2, **i32), torch.zeros(1, **i32)
+    for bad in (dict(rows=-1), dict(rows=1 << 31), dict(rows=1 << 32), dict(rows=4, max_q=-1), dict(rows=4, max_q=1 << 32)):
+        with pytest.raises(_lib.CormError, match="PagedBatch"):
+            paged.PagedBatch(*a, **bad)
+    assert paged.PagedBatch(*a, rows=4, max_keys=-3).max_keys == 0
+    assert paged.PagedBatch(*a, rows=4, max_keys=1 << 40).max_keys == 0x7FFFFFFF
+    assert paged.PagedBatch(*a, rows=4, max_q=9).max_q == 9
+    cache, batch = paged.PagedCache(4, 16, 2, 64, device="cpu"), paged.PagedBatch(*a, rows=4)
+    t = torch.zeros(4, 256, dtype=torch.int16)
+    for w in (-1, 1 << 32, (1 << 32) + 5):
+        with pytest.raises(_lib.CormError, match="window"):
+            ops.llm_paged_attn(cache, batch, t, t, H=4, smx=torch.zeros((4, 2), **i32), window=w)
+    for kw in (dict(eps_q=-1), dict(eps_k=1 << 62), dict(eps_q=1 << 64), dict(eps_k=(1 << 64) + 3)):
+        with pytest.raises(_lib.CormError, match="eps"):
+            ops.llm_paged_prep(cache, batch, t, t, t, t, H=4, rope=torch.zeros((8, 64), **i32), pq=None, pk=None, **kw)
+
+
 def test_page_pool():
     p = paged.PagePool(5, 16)
     a = p.extend("a", 17)
