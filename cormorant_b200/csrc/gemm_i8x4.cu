@@ -1060,6 +1060,8 @@ std::atomic<long long> g_wait_limit{kWaitDefault};
 
 }  // namespace
 
+long long wait_limit() { return g_wait_limit.load(std::memory_order_relaxed); }
+
 int* device_error_word() {
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1207,7 +1209,7 @@ int gemm_i8x4(const GemmJob& j, cudaStream_t stream) {
   ep.kb_per_split = sp.kps;
   ep.partial = nullptr;
   ep.err = err;
-  ep.wait_limit = g_wait_limit.load(std::memory_order_relaxed);
+  ep.wait_limit = wait_limit();
   ep.raw_tma = raw_tma ? 1u : 0u;
   ep.b_tma_planes = b_planes_in ? 1u : 0u;
   ep.a_box_rows = a_box_rows;
@@ -1279,7 +1281,7 @@ extern "C" int corm_device_status(int* code) {
   return CORM_OK;
 }
 
-// Bounds every mbarrier wait of the GEMM launches that follow (clock cycles;
+// Bounds every mbarrier wait of the GEMM and paged attention launches that follow (clock cycles;
 // <= 0 restores the default of about 2 s).  A diagnostic: limits below 2^20
 // cycles read the clock on every probe, so a test can make a wait run out.
 extern "C" int corm_set_wait_limit(long long cycles) {

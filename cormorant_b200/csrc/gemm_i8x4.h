@@ -91,6 +91,8 @@ int split_planes2(const SplitSeg& a, const SplitSeg& b, cudaStream_t stream);
 
 // Per-device word the kernels' bounded waits write on a timeout.
 int* device_error_word();
+// Clock cycles that a bounded wait may take (corm_set_wait_limit's, or the default).
+long long wait_limit();
 
 // Read (after the work on `stream` — nullptr: the legacy default stream — has
 // finished) and clear the status word of the allocation-free MatMul jobs on

@@ -561,6 +561,7 @@ struct SplitArgs {
   corm_llm_paged_attn_desc d;
   const int32_t* tab;
   int* err;
+  Waits waits;
   uint32_t G, Ginv, X, stages, win, rcap;  // Ginv: ceil(2^16 / G); stages of a warp; win: blocks of a warp's window; rcap: rows held
 };
 
@@ -836,7 +837,7 @@ __global__ void __launch_bounds__(256, OCC) paged_attn_split_kernel(const __grid
     __syncthreads();
     if (X > 1) {
       if (tid < X) mbar_arrive_remote(&cbar, tid);
-      if (ok) ok = mbar_wait_cluster(&cbar, cphase, A.err, 303);
+      if (ok) ok = mbar_wait_cluster(&cbar, cphase, A.err, 303, A.waits);
       cphase ^= 1u;
     }
   };
@@ -1331,6 +1332,7 @@ extern "C" int corm_llm_paged_attn(const corm_llm_paged_attn_desc* d, corm_strea
   A.tab = tb->smx_tab;
   A.err = corm::device_error_word();
   if (!A.err) return CORM_ECUDA;
+  A.waits = paged::waits();
   A.G = d->H / c.KV;
   const uint64_t rows = (uint64_t)A.d.max_q * A.G;
   A.rcap = rows < kRows ? (uint32_t)rows : kRows;

@@ -11,6 +11,7 @@
 
 #include "corm_common.cuh"
 #include "corm_sm100.cuh"
+#include "gemm_i8x4.h"
 
 namespace paged {
 
@@ -135,24 +136,36 @@ __device__ __forceinline__ void ldmatrix_t8(uint32_t (&r)[4], uint32_t a) {
 }
 
 // ---------------------------------------------------------------- waits
-// Bounded like sm100::mbar_wait; each look may suspend the warp for up to 20 us, so
-// that the many warps that wait here leave the issue slots to those that work.
-__device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity) {
+// How long a kernel's waits may take: clock cycles, about 2 s unless the host set
+// another limit (corm_set_wait_limit).  nap: each look may suspend the warp for so many
+// nanoseconds (20 us, so that the many warps that wait leave the issue slots to those that
+// work; 0 with a short limit, so that it counts).
+struct Waits {
+  long long limit;
+  uint32_t nap;
+};
+constexpr Waits kWaits = {4000000000ll, 20000u};
+inline Waits waits() {
+  const long long limit = corm::wait_limit();
+  return {limit, limit < sm100::kShortWaitLimit ? 0u : kWaits.nap};
+}
+__device__ __forceinline__ bool try_wait_nap(uint64_t* bar, uint32_t parity, uint32_t nap) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(sm100::smem_u32(bar)), "r"(parity), "r"(20000u)
+      : "r"(sm100::smem_u32(bar)), "r"(parity), "r"(nap)
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* err, int code) {
-  if (try_wait_long(bar, parity)) return true;
+// Bounded like sm100::mbar_wait
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* err, int code, Waits w) {
+  if (try_wait_nap(bar, parity, w.nap)) return true;
   const long long t0 = clock64();
-  while (!try_wait_long(bar, parity)) {
-    if (clock64() - t0 > 4000000000ll) {
+  while (!try_wait_nap(bar, parity, w.nap)) {
+    if (clock64() - t0 > w.limit) {
       if (err) atomicCAS(err, 0, code);
       return false;
     }
@@ -187,21 +200,23 @@ __device__ __forceinline__ unsigned long long cluster_ld64(uint32_t a) {
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
   return v;
 }
-// bounded, acquiring what the cluster's CTAs released by their arrivals
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* err, int code) {
+// bounded, acquiring what the cluster's CTAs released by their arrivals (a look that
+// suspends the warp as long as the hardware likes; with a short limit one look that does not)
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* err, int code, const Waits& w) {
   const long long t0 = clock64();
-  for (;;) {
+  do {
     uint32_t ok;
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %3, 0;\n\t"
+        "@q mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "@!q mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(sm100::smem_u32(bar)), "r"(parity)
+        : "r"(sm100::smem_u32(bar)), "r"(parity), "r"(w.nap)
         : "memory");
     if (ok) return true;
-    if (clock64() - t0 > 4000000000ll) break;
-  }
+  } while (clock64() - t0 <= w.limit);
   atomicCAS(err, 0, code);
   return false;
 }

@@ -78,6 +78,7 @@ struct TileArgs {
   corm_llm_paged_attn_desc d;
   const int32_t* tab;
   int* err;
+  Waits waits;
   uint32_t G, X, stages, win;  // win: tiles of a window
   uint32_t tiles;              // row tiles of the longest sequence
   uint32_t by_seq;             // items in the order of the sequences' lengths
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t gi = 0, asked = 0, answered = 0;
     bool ok = true;
     auto item_slot = [&]() {  // the slot's readers of ITEMS items ago are done
-      if (ok) ok = wait_for(&item_free[islot], ipar ^ 1u, A.err, 321);
+      if (ok) ok = wait_for(&item_free[islot], ipar ^ 1u, A.err, 321, A.waits);
       ok = __all_sync(0xffffffffu, ok);
     };
     auto publish = [&](const Item* o) {
@@ -325,7 +326,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     auto taken = [&]() -> int32_t {
       if (asked == answered) return -1;
-      ok = __all_sync(0xffffffffu, wait_for(&taken_bar, answered & 1u, A.err, 322)) && ok;
+      if (!__all_sync(0xffffffffu, wait_for(&taken_bar, answered & 1u, A.err, 322, A.waits))) {
+        ok = false;  // (the answer is waited for at the end)
+        return -1;
+      }
       answered++;
       const int32_t at = ok ? next_taken(&s_taken) : -1;
       __syncwarp();
@@ -352,10 +356,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       int32_t ids = -1;
       auto emit = [&](bool is_v, uint32_t t) {
         const uint32_t s = gi % NST;
-        if (gi >= NST && ok) ok = wait_for(&kv_empty[s], ((gi / NST) - 1u) & 1u, A.err, 311);
+        if (gi >= NST && ok) ok = wait_for(&kv_empty[s], ((gi / NST) - 1u) & 1u, A.err, 311, A.waits);
         ok = __all_sync(0xffffffffu, ok);
-        gi++;
         if (!ok) return;
+        gi++;
         const uint32_t b0 = (t * BK) >> psh, b1 = (t * BK + BK - 1u) >> psh;
         if (b0 < base || b1 >= base + 32u) {  // 32 table entries at a time
           base = b0;
@@ -401,8 +405,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       it = nx;
       more = some;
     }
-    // every copy lands before the CTA's shared memory goes away
-    for (uint32_t q = gi > NST ? gi - NST : 0u; ok && q < gi; q++) wait_for(&kv_full[q % NST], (q / NST) & 1u, nullptr, 0);
+    // every copy made, and the last answer, lands before the CTA's shared memory goes
+    // away, whoever gave up before (they need nobody: no diagnostic limit)
+    for (uint32_t q = gi > NST ? gi - NST : 0u; q < gi; q++) wait_for(&kv_full[q % NST], (q / NST) & 1u, nullptr, 0, kWaits);
+    if (asked != answered) wait_for(&taken_bar, answered & 1u, nullptr, 0, kWaits);
     __syncwarp();
   } else if (warp == RW + 1u) {
     // ---------------- the MMAs (one lane)
@@ -422,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t use = 0, pu = 0;          // uses of the scores' columns; P buffers
       bool ok = true;
       auto stage_in = [&]() -> uint32_t {  // the next stage, full: its address / 16
-        if (ok) ok = wait_for(&kv_full[s], sp, A.err, 312);
+        if (ok) ok = wait_for(&kv_full[s], sp, A.err, 312, A.waits);
         return (ring_a + s * Sh::STAGE) >> 4;
       };
       auto stage_out = [&]() {
@@ -431,7 +437,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       auto scores = [&]() {  // one tile's q.K^T
         const uint32_t b = (uint32_t)k0 + stage_in();
-        if (ok) ok = wait_for(&s_free, use & 1u, A.err, 313);
+        if (ok) ok = wait_for(&s_free, use & 1u, A.err, 313, A.waits);
         use++;
         if (ok) {
           sm100::tc_fence_after();
@@ -465,7 +471,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (uint32_t ch = 0; ch < Sh::CH; ch++, pu++) {
           const uint32_t buf = pu & 1u;
-          if (ok) ok = wait_for(&p_full[buf], (pu >> 1) & 1u, A.err, 315);
+          if (ok) ok = wait_for(&p_full[buf], (pu >> 1) & 1u, A.err, 315, A.waits);
           if (!ok) continue;
           sm100::tc_fence_after();
           const uint32_t p = tmem + Sh::P0 + buf * Sh::PCOLS;
@@ -502,7 +508,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       // (one lane walks the items: the others' candidates by itself)
       while (true) {
-        if (ok) ok = wait_for(&item_full[islot], ipar, A.err, 320);
+        if (ok) ok = wait_for(&item_full[islot], ipar, A.err, 320, A.waits);
         const Item& it = s_item[islot];
         const bool end = !ok || !s_more[islot];
         const uint32_t t0 = it.t0, t1 = it.t1;
@@ -511,7 +517,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (++islot == ITEMS) islot = 0, ipar ^= 1u;
         const bool again = t1 - t0 > WIN;
         auto taken = [&]() {
-          if (ok) ok = wait_for(&s_free, use & 1u, A.err, 314);
+          if (ok) ok = wait_for(&s_free, use & 1u, A.err, 314, A.waits);
           use++;
         };
         if (t0 == t1) taken();  // no key is seen: the next item's q comes with the next release
@@ -589,7 +595,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // across a barrier, so that all leave together whatever ran out
     auto look = [&](uint32_t slot, uint32_t par) {
       if (warp != 0) return;
-      if (ok) ok = wait_for(&item_full[slot], par, A.err, 323);
+      if (ok) ok = wait_for(&item_full[slot], par, A.err, 323, A.waits);
       const bool some = __all_sync(0xffffffffu, ok && s_more[slot] != 0u);
       if (lane == 0) s_go = some;
     };
@@ -608,7 +614,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       rows_sync();
       if (X > 1) {
         if (tid < X) mbar_arrive_remote(&cbar, tid);
-        if (ok) ok = mbar_wait_cluster(&cbar, cphase, A.err, 317);
+        if (ok) ok = mbar_wait_cluster(&cbar, cphase, A.err, 317, A.waits);
         cphase ^= 1u;
       }
     };
@@ -654,7 +660,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // tile t's scores.  Phase 0: their maximum, and the scores into the window where it
       // holds all; in windows, phase 1: the sum of e, 2: e into the window
       auto score_pass = [&](uint32_t t, uint32_t a, const uint32_t phase) {
-        if (ok) ok = wait_for(&s_full, su & 1u, A.err, 316);
+        if (ok) ok = wait_for(&s_full, su & 1u, A.err, 316, A.waits);
         su++;
         __syncwarp();
         sm100::tc_fence_after();
@@ -803,7 +809,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
         }
-        if (uses && ok) ok = wait_for(&p_empty[buf], (uses - 1u) & 1u, A.err, 318);
+        if (uses && ok) ok = wait_for(&p_empty[buf], (uses - 1u) & 1u, A.err, 318, A.waits);
         __syncwarp();
         sm100::tc_fence_after();
         const uint32_t ta = lane_base + Sh::P0 + buf * Sh::PCOLS + (part % (Sh::PCH / 32u)) * 8u;
@@ -882,7 +888,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const bool last = e == t1;
         if (last ? more : Sh::Q_OVER) fetch_q(s_item[last ? islot : cur], qn);  // (its latency under the wait)
         // the window's P.V: this part's dimensions
-        if (ok) ok = wait_for(&o_full, ou & 1u, A.err, 319);
+        if (ok) ok = wait_for(&o_full, ou & 1u, A.err, 319, A.waits);
         ou++;
         __syncwarp();
         sm100::tc_fence_after();
@@ -1130,6 +1136,7 @@ int launch_tiles(const corm_llm_paged_attn_desc& d, const int32_t* tab, int* err
   A.d = d;
   A.tab = tab;
   A.err = err;
+  A.waits = waits();
   A.G = d.H / d.c.KV;
   const uint32_t tiles = (uint32_t)(((uint64_t)d.max_q * A.G + BMR - 1u) / BMR);
   switch (d.c.HD * 2u + (d.c.bits == 8u)) {

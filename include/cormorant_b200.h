@@ -577,11 +577,11 @@ int corm_bind_device(int device);
  * kernels' bounded waits set when a wait times out (0 = none).  Replaces the
  * reference's kernel_wait timeout accounting (runtime/inference_irq.c:259-264). */
 int corm_device_status(int* code);
-/* Bounds every mbarrier wait of the tensor-core GEMM launches issued after the
- * call, in clock cycles (<= 0 restores the default of about 2 s).  A test and
- * diagnostic knob: below 2^20 cycles the waits read the clock on every probe,
- * so a short limit makes a GEMM's wait run out on purpose; the launch then
- * unwinds and reports through the status words above. */
+/* Bounds every mbarrier wait of the tensor-core GEMM and paged attention launches
+ * issued after the call, in clock cycles (<= 0 restores the default of about 2 s).
+ * A test and diagnostic knob: below 2^20 cycles the waits read the clock on every
+ * probe, so a short limit makes a wait run out on purpose; the launch then unwinds
+ * and reports through the status words above. */
 int corm_set_wait_limit(long long cycles);
 /* 1 when every job issued to the stream has finished, 0 while work remains
  * (the drivers' IsDone / IsIdle), or a negative CUDA error. */

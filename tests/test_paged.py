@@ -1041,3 +1041,34 @@ def test_gpu_refused_rotation_tables():
         with pytest.raises(_lib.CormError, match="rope"):
             ops.llm_paged_prep(cache, batch, z(256), z(128), z(128), z(256), **ok, **kw)
     assert ops.device_status() == 0
+
+
+@gpu
+@pytest.mark.parametrize("ctx,new,codes", [([0, 0], [300, 140], range(311, 324)), ([6000], [100], range(311, 324)),
+                                           ([6000], [1], [303])], ids=["tiles", "tile_cluster", "cluster"])
+@pytest.mark.parametrize("HD,bits", [(64, 16), (128, 8)])
+def test_attn_waits_that_run_out(HD, bits, ctx, new, codes):
+    """Waits of 200 cycles, far below a copy's time, run out: the launch ends, its status
+    is read once, and the next launch with the usual limit is exact."""
+    from cormorant_b200 import ops
+    rng = np.random.default_rng(HD + new[0])
+    H, KV, page = 4, 2, 64
+    pages = sum(-(-(a + n) // page) for a, n in zip(ctx, new))
+    table, cu, pos, rows = _batch(rng, pages, page, ctx, new)
+    c = _random_cache(rng, pages, KV, page, HD, bits, 2500)
+    c.table, c.cu, c.pos = table, cu, pos
+    kw = dict(max_q=max(new), max_keys=max(a + n for a, n in zip(ctx, new)))
+    cache, batch = _handles(c, rows, **kw)
+    smx = _smx(H, HD, f_s=10)
+    q, o = (torch.zeros((rows, H * HD), dtype=torch.int16, device="cuda") for _ in range(2))
+    assert ops.device_status() == 0
+    L = _lib.lib()
+    try:
+        assert L.corm_set_wait_limit(200) == 0
+        ops.llm_paged_attn(cache, batch, q, o, H=H, smx=_dev(smx))
+        torch.cuda.synchronize()
+    finally:
+        assert L.corm_set_wait_limit(0) == 0
+    assert ops.device_status() in codes
+    assert ops.device_status() == 0
+    _run_attn(c, rows, H, smx, rng, hi=2500, **kw)
