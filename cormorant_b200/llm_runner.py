@@ -12,6 +12,8 @@ them and single tokens of several sequences in one pass over a paged KV cache
 """
 from __future__ import annotations
 
+import threading
+from contextlib import contextmanager
 from typing import Dict, Hashable, List, Optional, Sequence
 
 import numpy as np
@@ -75,7 +77,8 @@ class PagedLlamaRunner:
     ``release``.  Every pass takes the unit's softmax, a prompt's and a single
     token's alike, so at 16 bits a token's words do not depend on how its sequence
     was cut into passes nor on what ran beside it (with 8 bits nor do they: a row's
-    codes are its own)."""
+    codes are its own).  Calls from several threads take turns, and passes on
+    different streams follow one another on the device."""
 
     def __init__(self, model, pages: int, page: int = 64, bits: int = 16, device=None, fuse: bool = True):
         self.m, self.fuse = model, fuse
@@ -87,6 +90,33 @@ class PagedLlamaRunner:
         self.table = torch.from_numpy(emb).to(self.device)
         self._sims: Dict[tuple, GpuSimulator] = {}
         self._share: Optional[GpuSimulator] = None
+        self._lock = threading.RLock()
+        # the last pass, and its stream
+        self._done = torch.cuda.Event() if self.device.type == "cuda" else None
+        self._stream: Optional[int] = None
+
+    @contextmanager
+    def _turn(self, *used: Optional[torch.Tensor]):
+        """One call at a time, its device work behind the last call's: they share the
+        pool, the pages, the weights and the simulators.  used: the caller's tensors,
+        perhaps another stream's."""
+        with self._lock:
+            if self._done is None:
+                yield
+                return
+            stream = torch.cuda.current_stream(self.device)
+            stream.wait_event(self._done)
+            if stream.cuda_stream != self._stream:  # workspaces stay with the stream that they were allocated on
+                self._stream = stream.cuda_stream
+                for s in self._sims.values():
+                    s._ws = None
+            for t in used:
+                if t is not None and t.is_cuda:
+                    t.record_stream(stream)
+            try:
+                yield
+            finally:
+                self._done.record(stream)
 
     def _sim(self, rows: int, head: bool) -> GpuSimulator:
         key = (rows, head)
@@ -153,19 +183,21 @@ class PagedLlamaRunner:
         flat = np.concatenate(tokens) if new else np.zeros(0, np.int64)
         if flat.size and (flat.min() < 0 or flat.max() >= self.m.vocab):
             raise CormError(CORM_EINVAL, f"PagedLlamaRunner: token ids in [0, {self.m.vocab}) expected")
-        at = self._room(seqs, new)
-        h, n = self._rows(flat.size), flat.size * self.m.D
-        torch.index_select(self.table, 0, torch.from_numpy(flat).to(self.device), out=h[:n].view(flat.size, self.m.D))
-        return self._pass(seqs, new, at, h)
+        with self._turn():
+            at = self._room(seqs, new)
+            h, n = self._rows(flat.size), flat.size * self.m.D
+            torch.index_select(self.table, 0, torch.from_numpy(flat).to(self.device), out=h[:n].view(flat.size, self.m.D))
+            return self._pass(seqs, new, at, h)
 
     def step(self, seqs: Sequence[Hashable], logits: torch.Tensor, ids: Optional[torch.Tensor] = None) -> torch.Tensor:
         """A greedy token for each of ``seqs`` after ``logits`` (their order),
         chosen on the device (int32 ``ids`` if given); its logits."""
         new = [1] * len(seqs)
-        at = self._room(seqs, new)  # (before ids is written)
-        h = self._rows(len(seqs))
-        ops.greedy_embed(logits, self.table, h, ids, batch=len(seqs), vocab=self.m.vocab, dim=self.m.D)
-        return self._pass(seqs, new, at, h)
+        with self._turn(logits, ids):
+            at = self._room(seqs, new)  # (before ids is written)
+            h = self._rows(len(seqs))
+            ops.greedy_embed(logits, self.table, h, ids, batch=len(seqs), vocab=self.m.vocab, dim=self.m.D)
+            return self._pass(seqs, new, at, h)
 
     def generate(self, prompts: Dict[Hashable, Sequence[int]], steps: int) -> Dict[Hashable, List[int]]:
         """The prompts in one pass, then ``steps`` greedy tokens of each."""
@@ -179,5 +211,6 @@ class PagedLlamaRunner:
 
     def release(self, seq: Hashable) -> None:
         """Ends a sequence; its pages are free."""
-        self.pool.release(seq)
-        self.length.pop(seq, None)
+        with self._lock:
+            self.pool.release(seq)
+            self.length.pop(seq, None)

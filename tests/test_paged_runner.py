@@ -209,6 +209,50 @@ def test_step_refuses_before_it_writes(paged_cpu):
     assert ids[0] >= 0 and ids[1] == -5 and r.length == dict(b=17)
 
 
+def test_runner_on_two_threads(paged_cpu, monkeypatch):
+    """Two threads on one runner, each with sequences of its own: every pass's logits are
+    those of the sequence alone, wherever the other thread's passes fall."""
+    import threading
+    import time
+
+    from cormorant_b200 import ops
+    m = WL.LlamaModel(batch=1, seq=16, cache=32, seed=4, **SMALL)
+    inner = ops.llm_paged_prep
+
+    def slow(*a, **kw):  # the other thread has its turn in the middle of a pass
+        time.sleep(0.005)
+        inner(*a, **kw)
+    monkeypatch.setattr(ops, "llm_paged_prep", slow)
+
+    def serve(r, s, first):
+        got = []
+        for i in range(4):
+            ids = torch.empty(1, dtype=torch.int32)
+            lg = r.append([(s, i)], [[first + i, 7, 3]])
+            got.append(_words(lg, 1, m.vocab))
+            got.append(_words(r.step([(s, i)], lg, ids), 1, m.vocab))
+            if i % 2:
+                r.release((s, i))
+        return np.stack(got)
+    alone = [serve(PagedLlamaRunner(m, pages=4, page=16, device="cpu"), s, 9 * s) for s in range(2)]
+    r = PagedLlamaRunner(m, pages=8, page=16, device="cpu")
+    out, errors = [None, None], []
+
+    def work(s):
+        try:
+            out[s] = serve(r, s, 9 * s)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(s,)) for s in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    assert np.array_equal(out[0], alone[0]) and np.array_equal(out[1], alone[1])
+    assert sorted(r.length) == [(0, 0), (0, 2), (1, 0), (1, 2)] and len(r.pool.free) == 4
+
+
 @gpu
 @pytest.mark.parametrize("dims,lengths,page", [
     (dict(layers=2, hidden=64, heads=4, kv_heads=2, head_dim=16, ffn=128, vocab=300), (9, 3, 70, 40), 16),
@@ -256,3 +300,39 @@ def test_gpu_runner_generate():
     both = r.generate(prompts, 5)
     for s, p in prompts.items():
         assert PagedLlamaRunner(m, pages=2, page=64).generate({s: p}, 5)[s] == both[s]
+
+
+@gpu
+def test_gpu_runner_on_streams():
+    """A runner's passes on one stream after another, nothing waited for between them,
+    and from two threads on two streams: the words of one stream's."""
+    import threading
+    dims = dict(layers=2, hidden=960, heads=15, kv_heads=5, head_dim=64, ffn=256, vocab=500, seed=2)
+    m = WL.LlamaModel(batch=1, seq=64, **dims)
+    prompts = {s: np.random.default_rng(s).integers(0, 500, 5 + 9 * s).tolist() for s in range(4)}
+    want = {s: PagedLlamaRunner(m, pages=2, page=64).generate({s: p}, 6)[s] for s, p in prompts.items()}
+    r = PagedLlamaRunner(m, pages=8, page=64)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    ids = torch.empty((6, 4), dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[0]):
+        lg = r.append(list(prompts), list(prompts.values()))
+    for i in range(6):
+        with torch.cuda.stream(streams[(i + 1) % 3]):
+            lg = r.step(list(prompts), lg, ids[i])
+    torch.cuda.synchronize()
+    assert ids.cpu().numpy().T.tolist() == [want[s] for s in prompts]
+    for s in prompts:
+        r.release(s)
+    got = {}
+
+    def work(mine):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for s in mine:
+                got.update(r.generate({s: prompts[s]}, 6))
+    threads = [threading.Thread(target=work, args=(t,)) for t in ((0, 2), (1, 3))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert got == want
