@@ -253,6 +253,23 @@ def test_runner_on_two_threads(paged_cpu, monkeypatch):
     assert sorted(r.length) == [(0, 0), (0, 2), (1, 0), (1, 2)] and len(r.pool.free) == 4
 
 
+def test_runner_keeps_few_graphs(paged_cpu, monkeypatch):
+    """Passes of ever other row counts: the graphs kept are bounded, the last used stay,
+    one workspace serves all, and a pass over a graph built again gives the same words."""
+    m = WL.LlamaModel(batch=1, seq=16, cache=32, seed=4, **SMALL)
+    r = PagedLlamaRunner(m, pages=2, page=16, device="cpu")
+    monkeypatch.setattr(PagedLlamaRunner, "GRAPHS", 5, raising=False)
+    want = {}
+    for n in list(range(1, 13)) + [1, 12, 3]:
+        got = r.append("a", [list(range(1, n + 1))])[:m.vocab].clone()
+        assert torch.equal(want.setdefault(n, got), got)
+        r.release("a")
+        assert len(r._sims) <= 5 and (n, False) in r._sims and (1, True) in r._sims
+        assert all(s._ws is None for s in r._sims.values())
+    assert list(r._sims)[-2:] == [(3, False), (1, True)]
+    assert 1 < PagedLlamaRunner(m, pages=2, page=16, device="cpu").GRAPHS
+
+
 @gpu
 @pytest.mark.parametrize("dims,lengths,page", [
     (dict(layers=2, hidden=64, heads=4, kv_heads=2, head_dim=16, ffn=128, vocab=300), (9, 3, 70, 40), 16),
